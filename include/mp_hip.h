@@ -203,6 +203,122 @@ int mp_hip_paged_attention_decode_noalloc(const float* q, const float* keys, con
                                           int32_t layers, int32_t block_tokens, int32_t heads,
                                           int32_t kv_heads, int32_t dim, float* out, void* stream);
 
+/* ---- A paged K/V cache in 8 bits -----------------------------------------
+ * (no counterpart in the reference, whose pools are FP32). Stand-alone like
+ * the attention calls above: caller-owned DEVICE buffers, a caller's stream
+ * (NULL: the null stream), asynchronous, no allocation, no state kept between
+ * calls, lengths read on the device, so that a call can be captured into a
+ * HIP graph and replayed with new lengths. Calls run on the stream's device.
+ * Refusals are MP_INVALID_ARGUMENT with a message in mp_hip_last_error(NULL).
+ *
+ * Format. A page is block_tokens tokens (16, 32, 64 or 128) of one layer. Per
+ * KV head it holds dim bytes a token (dim 64, 128 or 256) in each of `keys`
+ * and `values`, [blocks][layers][kv_heads][block_tokens * dim], and in
+ * `scales`, [blocks][layers][kv_heads][2], the scale of the head's keys and
+ * that of its values. A byte b stands for scale * (b - 128) (MP_KV8_INT8; 0
+ * is not written) or scale times the E4M3 number b (MP_KV8_E4M3: 448 largest,
+ * 0x7F and 0xFF NaN). Scales are powers of two from 2^-126 on, so that raising
+ * one moves codes without another rounding of the scale, and every value is
+ * exact in FP32, BF16 and (in its range) FP16. Order of a head's bytes: tiles
+ * of 16 tokens; inside a tile keys are [dim/16][slot][16 dims], values
+ * [dim/64][slot/4][dim%16][dim%64/16][slot%4]: the matrix cores' operands,
+ * 16 bytes a lane. A block is contiguous in all three arrays: copying one on
+ * write is three plain copies. keys and values are 16-byte aligned, scales
+ * 8-byte.
+ *
+ * Rows. q, k, v and out are FP32, BF16 or FP16 (MP_TYPE_*), one row a token,
+ * heads adjacent, `stride` elements from row to row (a fused q|k|v matrix is
+ * three pointers with one stride); any alignment of their type, 16 bytes for
+ * full speed. Rows are packed: sequence s has rows starts[s] ..
+ * starts[s+1]-1 (device int32, sequences + 1 of them, not decreasing), at
+ * positions used[s], used[s]+1, ... (device int32), and page table tables +
+ * s*table_stride (device int32). Rows outside starts[0] .. starts[sequences]-1
+ * are not touched. A sequence without rows is nothing, and neither is one to
+ * append or read with used[s] outside 0 .. 2^30.
+ *
+ * What the device finds: a token whose page id is not in 0 .. blocks-1 or
+ * whose page lies past table_stride is not written; an attention that needs
+ * such a page gives NaN, as it does for a row longer than max_length and for
+ * a NaN in the cache or in q. */
+enum { MP_TYPE_F32 = 0, MP_TYPE_BF16 = 1, MP_TYPE_F16 = 2 };
+enum { MP_KV8_INT8 = 0, MP_KV8_E4M3 = 1 };
+
+typedef struct mp_kv8_cache {
+    uint8_t* keys;
+    uint8_t* values;
+    float* scales;
+    int32_t blocks, layers, block_tokens, kv_heads, dim, format;
+} mp_kv8_cache;
+
+/* Rotary positions: cos and sin of `positions` positions, device FP32
+ * [positions][dims/2], whatever angles the model has (a context stretched by
+ * interpolation is a matter of these tables). The first `dims` dims of every
+ * head turn, the rest pass: pairs are (i, i + dims/2), or with `interleaved`
+ * (2i, 2i + 1); a' = a cos - b sin, b' = b cos + a sin, each operation rounded
+ * to FP32. dims is even; 0: no rotation, and the tables may be NULL. */
+typedef struct mp_rope {
+    const float* cos;
+    const float* sin;
+    int32_t positions, dims, interleaved;
+} mp_rope;
+
+/* Appends the rows' keys (rotated) and values to their pages of `layer`, and
+ * writes the rotated queries to q_out (which may be q; q NULL: none; `heads`
+ * query heads). Per page, head and kind: where the first new token takes slot
+ * 0 the page starts anew; otherwise the slots before it are kept. The scale
+ * is the smallest power of two that holds the new tokens, not smaller than
+ * that of the kept ones; where it grows, the kept codes are rounded again
+ * (nearest, ties to even, as are the new ones). Slots behind the last new
+ * token keep their bytes. After a step that was taken back its positions are
+ * simply appended again; a scale that the step had raised stays as it is.
+ * A NaN or infinity in the new tokens makes the scale NaN, and with it the
+ * head's keys (or values) of the page, until the page is written from slot 0.
+ * Rows at or past rope->positions are not written, and their q_out is NaN.
+ * `rope` may be NULL. k and v must not overlap the cache; sequences that
+ * write must not share the page that they write. */
+int mp_hip_kv8_append(const mp_kv8_cache* cache, int32_t layer, const void* k, int64_t k_stride, const void* v,
+                      int64_t v_stride, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride,
+                      int32_t heads, int32_t type, const mp_rope* rope, const int32_t* tables, int32_t table_stride,
+                      const int32_t* starts, const int32_t* used, int32_t sequences, int32_t rows, void* stream);
+
+/* Reads tokens back as rows of values: row i of sequence s is the token at
+ * position used[s] + i - starts[s], as the pages hold it (rotated keys).
+ * NaN for tokens without a valid page. Values outside the range of FP16 are
+ * rounded as its conversion does. */
+int mp_hip_kv8_read(const mp_kv8_cache* cache, int32_t layer, const int32_t* tables, int32_t table_stride,
+                    const int32_t* starts, const int32_t* used, int32_t sequences, int32_t rows, int32_t type,
+                    void* k, int64_t k_stride, void* v, int64_t v_stride, void* stream);
+
+/* Bytes of workspace with which both attention calls below run `rows` rows of
+ * `sequences` sequences (decode: as many as rows) of up to max_length tokens.
+ * 0 is possible, and then the pointer may be NULL. A workspace holds nothing
+ * between calls; calls that may overlap, replayed graphs among them, need
+ * workspaces of their own. */
+int mp_hip_kv8_attention_workspace(const mp_kv8_cache* cache, int32_t rows, int32_t sequences, int32_t heads,
+                                   int32_t max_length, size_t* bytes);
+
+/* Decode attention: row r, at position lengths[r] - 1, attends the
+ * lengths[r] tokens of its page table tables + r*table_stride (device int32,
+ * at most max_length): out = sum_t softmax_t(scale * q.k_t) v_t, query head h
+ * on KV head h / (heads / kv_heads), at most 16 query heads per KV head. A
+ * row of no tokens (length 0 or less) gives zeros. `scale` is finite and not
+ * negative. Sums are FP32 (about 1e-6 of the 64-bit result for FP32 rows). */
+int mp_hip_kv8_attention_decode(const mp_kv8_cache* cache, int32_t layer, const void* q, int64_t q_stride,
+                                int32_t type, const int32_t* tables, int32_t table_stride, const int32_t* lengths,
+                                int32_t rows, int32_t heads, int32_t max_length, float scale, void* out,
+                                int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Prefill attention of packed rows, causal: the row at position p attends
+ * tokens 0 .. p of its sequence, all of them in the pages already (append
+ * first); used[s] + the rows of s is at most max_length. Any mix of counts,
+ * single tokens among them. FP32 rows keep FP32 accuracy; for BF16 and FP16
+ * rows the probabilities are rounded to FP16 for the product with the values. */
+int mp_hip_kv8_attention_prefill(const mp_kv8_cache* cache, int32_t layer, const void* q, int64_t q_stride,
+                                 int32_t type, const int32_t* tables, int32_t table_stride, const int32_t* starts,
+                                 const int32_t* used, int32_t sequences, int32_t rows, int32_t heads,
+                                 int32_t max_length, float scale, void* out, int64_t out_stride, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
 /* Applies queued table entries and copies, then waits for all work on the
  * context's stream (StreamBlas::synchronize). */
 int mp_hip_sync(mp_hip* h);

@@ -1,0 +1,692 @@
+"""The 8-bit paged K/V cache on the GPU, through its C entries, against the
+definition in numpy (kv8_reference.py): bytes and scales bit for bit, attention
+within the bound that its arithmetic gives (kv8_reference.bound, plus the
+rounding of the row type: half a step of the result, and for FP16 and BF16
+prefill rows half an FP16 step of every probability)."""
+import numpy as np
+import pytest
+
+from tinyinfer_amd import backend as mp
+
+from .kv8_reference import BF16, E4M3, F16, F32, INT8, VALUES, Cache, rounded
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = pytest.mark.parametrize("fmt", [INT8, E4M3], ids=["int8", "e4m3"])
+TYPES = {F32: "float32", BF16: "bfloat16", F16: "float16"}
+HALF_STEP = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+
+
+class Device:
+    """A numpy Cache's pools on the GPU, and calls on them."""
+
+    def __init__(self, torch, cache: Cache):
+        self.torch, self.cache = torch, cache
+        self.bytes = [torch.from_numpy(b.copy()).cuda() for b in cache.bytes]
+        self.scales = torch.from_numpy(cache.scales.copy()).cuda()
+        self.view = mp.Kv8Cache(self.bytes[0].data_ptr(), self.bytes[1].data_ptr(), self.scales.data_ptr(),
+                                cache.blocks, cache.layers, cache.bt, cache.kv_heads, cache.dim, cache.fmt)
+
+    def ints(self, a):
+        return self.torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda()
+
+    def rows(self, x, kind, pad=0, shift=0):
+        """x [rows, width] float32 as a row matrix of a type: (tensor kept alive, address, stride); `pad` elements
+        behind every row, the first `shift` elements from the buffer's start. Padding is NaN."""
+        t = self.torch
+        n, width = x.shape
+        buffer = t.full((n * (width + pad) + shift,), float("nan"), dtype=getattr(t, TYPES[kind]), device="cuda")
+        matrix = buffer[shift:].view(n, width + pad)
+        matrix[:, :width] = t.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).cuda()
+        return matrix, matrix.data_ptr(), width + pad
+
+    def back(self, matrix, width):
+        self.torch.cuda.synchronize()
+        return matrix[:, :width].float().cpu().numpy()
+
+    def check_bytes(self, want: Cache):
+        """Scales and bytes equal, but for the bytes of what reads as NaN."""
+        self.torch.cuda.synchronize()
+        scales = self.scales.cpu().numpy()
+        assert np.array_equal(scales, want.scales, equal_nan=True)
+        for kind in range(2):
+            got, readable = self.bytes[kind].cpu().numpy(), ~np.isnan(want.scales[..., kind])
+            assert np.array_equal(got[readable], want.bytes[kind][readable]), f"kind {kind}"
+
+
+def tables_for(rng, blocks, lengths, bt, spare=1):
+    pages = [-(-max(n, 1) // bt) for n in lengths]
+    order = rng.permutation(blocks)
+    assert sum(pages) <= blocks
+    tables = np.full((len(lengths), max(pages) + spare), -1, dtype=np.int32)
+    at = 0
+    for s, p in enumerate(pages):
+        tables[s, :p] = order[at:at + p]
+        at += p
+    return tables
+
+
+def blocks_for(lengths, bt):
+    return sum(-(-max(n, 1) // bt) for n in lengths) + 2
+
+
+def angles(positions, dims):
+    a = np.arange(positions)[:, None] * 10000.0 ** (-np.arange(max(dims // 2, 1)) / max(dims // 2, 1))
+    return np.cos(a).astype(np.float32), np.sin(a).astype(np.float32)
+
+
+def starts_of(counts, first=0):
+    return np.concatenate(([first], first + np.cumsum(counts))).astype(np.int32)
+
+
+# ---- appending and reading ----------------------------------------------------
+
+APPENDS = [
+    # kv_heads, heads, dim, bt, rotated, interleaved, type, pad, shift
+    (3, 9, 64, 16, 64, False, F32, 0, 0),
+    (3, 9, 64, 16, 64, True, BF16, 4, 0),
+    (1, 2, 64, 32, 20, False, F32, 1, 1),   # rows and pairs that are not aligned
+    (2, 2, 64, 64, 6, True, F16, 0, 1),
+    (2, 6, 128, 64, 64, False, BF16, 8, 0),
+    (1, 4, 128, 128, 128, False, F32, 0, 0),
+    (1, 3, 256, 32, 32, True, F16, 12, 0),
+    (2, 4, 256, 16, 0, False, F32, 0, 0),
+]
+
+
+@FORMATS
+@pytest.mark.parametrize("kv_heads, heads, dim, bt, dims, interleaved, kind, pad, shift", APPENDS)
+def test_append_and_read(torch_cuda, fmt, kv_heads, heads, dim, bt, dims, interleaved, kind, pad, shift):
+    """Three calls in a row, each going on where the one before ended (in the middle of pages, with larger tokens, so
+    that scales grow): counts of 0, 1 and more than two pages, rows before the first and behind the last sequence,
+    layer 1 of 2. Then everything read back."""
+    rng = np.random.default_rng(dim + bt + fmt)
+    total = [0, 2 * bt + 5, 3, bt, 1, 3 * bt - 1]
+    steps = [[0, bt + 3, 1, bt - 1, 0, bt], [0, 1, 1, 1, 1, bt + 2], [0, bt + 1, 1, 0, 0, bt - 3]]
+    assert [sum(s) for s in zip(*steps)] == total
+    cache = Cache(blocks_for(total, bt), 2, kv_heads, bt, dim, fmt, rng)
+    device = Device(torch_cuda, cache)
+    tables = tables_for(rng, cache.blocks, total, bt)
+    cos, sin = angles(max(total), dims)
+    d_tables, d_cos, d_sin = device.ints(tables), torch_cuda.from_numpy(cos).cuda(), torch_cuda.from_numpy(sin).cuda()
+    rope = mp.Rope(d_cos.data_ptr(), d_sin.data_ptr(), len(cos), dims, int(interleaved))
+    used = np.zeros(len(total), dtype=np.int32)
+    for step, counts in enumerate(steps):
+        starts = starts_of(counts, first=2)
+        rows = int(starts[-1]) + 3
+        q, k, v = (rounded(rng.standard_normal((rows, h, dim)) * 3.0 ** step, kind)
+                   for h in (heads, kv_heads, kv_heads))
+        mq, q_at, q_stride = device.rows(q.reshape(rows, -1), kind, pad, shift)
+        mk, k_at, k_stride = device.rows(k.reshape(rows, -1), kind, pad, shift)
+        mv, v_at, v_stride = device.rows(v.reshape(rows, -1), kind, pad, shift)
+        mo, o_at, o_stride = device.rows(np.full((rows, heads * dim), 7.0), kind, pad, shift)
+        d_starts, d_used = device.ints(starts), device.ints(used)
+        mp.kv8_append(device.view, 1, k_at, k_stride, v_at, v_stride, kind, d_tables.data_ptr(), tables.shape[1],
+                      d_starts.data_ptr(), d_used.data_ptr(), len(total), rows, rope=rope, q=q_at, q_stride=q_stride,
+                      q_out=o_at, q_out_stride=o_stride, heads=heads)
+        cache.append(1, k, v, tables, starts, used, (cos, sin, dims, interleaved))
+        device.check_bytes(cache)
+        # Queries: rotated in float32, rounded once; other rows as they were.
+        from .kv8_reference import rotate
+        want = np.full((rows, heads, dim), 7.0, dtype=np.float32)
+        for s in range(len(total)):
+            for i in range(counts[s]):
+                r, position = starts[s] + i, used[s] + i
+                want[r] = rounded(rotate(q[r], cos[position], sin[position], dims, interleaved), kind) if dims else q[r]
+        assert np.array_equal(device.back(mo, heads * dim), want.reshape(rows, -1))
+        assert bool(mo[:, heads * dim:].isnan().all())
+        used = used + np.array(counts, dtype=np.int32)
+    # Reading: every token, and the ends alone.
+    for first in (np.zeros(len(total), dtype=np.int32), np.array([max(n - 2, 0) for n in total], dtype=np.int32)):
+        counts = np.array(total) - first
+        starts = starts_of(counts, first=1)
+        rows = int(starts[-1]) + 2
+        out = [device.rows(np.full((rows, kv_heads * dim), 5.0), kind, pad, shift) for _ in range(2)]
+        d_starts, d_used = device.ints(starts), device.ints(first)
+        mp.kv8_read(device.view, 1, d_tables.data_ptr(), tables.shape[1], d_starts.data_ptr(), d_used.data_ptr(),
+                    len(total), rows, kind, out[0][1], out[0][2], out[1][1], out[1][2])
+        for which in range(2):
+            want = np.full((rows, kv_heads, dim), 5.0)
+            for s in range(len(total)):
+                values = cache.tokens(1, which, tables[s], total[s])[:, first[s]:]
+                want[starts[s]:starts[s + 1]] = values.transpose(1, 0, 2)
+            assert np.array_equal(device.back(out[which][0], kv_heads * dim), rounded(want.reshape(rows, -1), kind))
+
+
+def append_plain(device, layer, k, v, tables, starts, used, rope=None, keep=None):
+    """FP32 rows without padding or queries."""
+    rows = k.shape[0]
+    mk, k_at, k_stride = device.rows(k.reshape(rows, -1), F32)
+    mv, v_at, v_stride = device.rows(v.reshape(rows, -1), F32)
+    ints = [device.ints(a) for a in (tables, starts, used)]
+    mp.kv8_append(device.view, layer, k_at, k_stride, v_at, v_stride, F32, ints[0].data_ptr(), tables.shape[1],
+                  ints[1].data_ptr(), ints[2].data_ptr(), len(used), rows, rope=rope)
+    device.torch.cuda.synchronize()
+
+
+@FORMATS
+def test_append_extremes(torch_cuda, fmt):
+    """Zeros, denormals, the largest numbers, and magnitudes on both sides of where the scale steps."""
+    rng = np.random.default_rng(3)
+    top = 127.0 if fmt == INT8 else 448.0
+    peaks = [0.0, 2.0 ** -149, 2.0 ** -130, 2.0 ** -126, top * 2.0 ** -126, np.nextafter(np.float32(top / 8), np.float32(1e9)),
+             top / 8, np.nextafter(np.float32(top / 8), np.float32(0)), 1.0, 3e38, float(np.finfo(np.float32).max)]
+    cache = Cache(len(peaks) + 1, 1, 1, 16, 64, fmt, rng)
+    device = Device(torch_cuda, cache)
+    tables = np.arange(len(peaks), dtype=np.int32)[:, None]
+    x = rng.uniform(-1, 1, (len(peaks), 1, 64))
+    x[:, 0, 17] = -1
+    x = (x * np.array(peaks, dtype=np.float64)[:, None, None]).astype(np.float32)
+    starts, used = starts_of([1] * len(peaks)), np.zeros(len(peaks), dtype=np.int32)
+    append_plain(device, 0, x, -x, tables, starts, used)
+    cache.append(0, x, -x, tables, starts, used)
+    device.check_bytes(cache)
+    for at, s in enumerate(cache.scales[:len(peaks), 0, 0, 0]):
+        assert s >= 2.0 ** -126 and np.frexp(s)[0] == 0.5 and peaks[at] <= top * float(s)
+
+
+@FORMATS
+def test_token_by_token_is_within_a_step_of_a_chunk(torch_cuda, fmt):
+    """Rounded again at each growth, a token's INT8 code is off its own rounding by less than one step of the final
+    scale (1/2 + 1/4 + ...); an E4M3 value by half a step of 2^-3 twice at most where it falls below the normal range."""
+    rng = np.random.default_rng(4)
+    x = (rng.standard_normal((32, 2, 64)) * 2.0 ** (np.arange(32) % 16 / 3)[:, None, None]).astype(np.float32)
+    tables = np.array([[1, 2]], dtype=np.int32)
+    whole, single = (Cache(3, 1, 2, 16, 64, fmt, rng) for _ in range(2))
+    a, b = Device(torch_cuda, whole), Device(torch_cuda, single)
+    append_plain(a, 0, x, x, tables, np.array([0, 32]), np.array([0]))
+    whole.append(0, x, x, tables, [0, 32], [0])
+    a.check_bytes(whole)
+    for i in range(32):
+        append_plain(b, 0, x[i:i + 1], x[i:i + 1], tables, np.array([0, 1]), np.array([i]))
+        single.append(0, x[i:i + 1], x[i:i + 1], tables, [0, 1], [i])
+    b.check_bytes(single)
+    assert np.array_equal(whole.scales[1:], single.scales[1:])
+    scale = np.repeat(whole.scales[1:, 0, :, 0], 16, axis=0)[..., None].astype(np.float64)
+    for cache in (whole, single):
+        got = cache.tokens(0, 0, tables[0], 32).transpose(1, 0, 2)
+        off = np.abs(got - x)
+        if fmt == INT8:
+            assert np.all(off < (0.5 if cache is whole else 1.0) * scale)
+        else:
+            assert np.all(off <= np.maximum(np.abs(x) * 2.0 ** -4, scale * 2.0 ** -9))
+
+
+@FORMATS
+def test_a_step_taken_back_and_a_poisoned_page(torch_cuda, fmt):
+    """NaN and infinity make a head's keys of the page NaN and nothing else; writing the page from slot 0 heals it;
+    a token written again gives its codes again."""
+    rng = np.random.default_rng(5)
+    cache = Cache(4, 2, 2, 16, 64, fmt, rng)
+    device = Device(torch_cuda, cache)
+    tables = np.array([[2, 0]], dtype=np.int32)
+    x = rng.standard_normal((20, 2, 64)).astype(np.float32)
+
+    def step(rows, at, k, v):
+        append_plain(device, 1, k, v, tables, np.array([0, rows]), np.array([at]))
+        cache.append(1, k, v, tables, [0, rows], [at])
+        device.check_bytes(cache)
+
+    step(20, 0, x, x)
+    step(1, 5, x[5:6], x[5:6])
+    bad = x[6:7].copy()
+    bad[0, 1, 3] = np.nan
+    step(1, 6, bad, x[6:7])
+    assert np.isnan(cache.scales[2, 1, 1, 0]) and np.isnan(cache.scales).sum() == 1
+    step(1, 6, x[6:7], x[6:7])
+    assert np.isnan(cache.scales[2, 1, 1, 0]) and np.isnan(cache.scales).sum() == 1
+    step(20, 0, x, x)
+    assert not np.isnan(cache.scales).any()
+    bad = x[:1].copy()
+    bad[0, 0, 0] = -np.inf
+    step(1, 19, x[19:20], bad)
+    assert np.isnan(cache.scales[0, 1, 0, 1]) and np.isnan(cache.scales).sum() == 1
+
+
+def test_append_beyond_pages_and_angles(torch_cuda):
+    """Page ids outside the pool, pages past the table and positions past the rotation tables: those tokens are not
+    written, all others are; a query past the tables is NaN. Sequences that start below 0 are left out."""
+    rng = np.random.default_rng(6)
+    cache = Cache(6, 1, 1, 16, 64, INT8, rng)
+    device = Device(torch_cuda, cache)
+    tables = np.array([[0, -1, 1], [2, 6, 3], [4, 2147483647, 5], [1, 1, 1]], dtype=np.int32)
+    counts, used = [40, 60, 20, 3], np.array([0, 0, 25, -7], dtype=np.int32)
+    starts = starts_of(counts)
+    rows = int(starts[-1])
+    k, v, q = (rng.standard_normal((rows, 1, 64)).astype(np.float32) for _ in range(3))
+    cos, sin = angles(38, 64)
+    d_cos, d_sin = torch_cuda.from_numpy(cos).cuda(), torch_cuda.from_numpy(sin).cuda()
+    rope = mp.Rope(d_cos.data_ptr(), d_sin.data_ptr(), 38, 64, 0)
+    mk, k_at, _ = device.rows(k.reshape(rows, -1), F32)
+    mv, v_at, _ = device.rows(v.reshape(rows, -1), F32)
+    mq, q_at, _ = device.rows(q.reshape(rows, -1), F32)
+    ints = [device.ints(a) for a in (tables, starts, used)]
+    mp.kv8_append(device.view, 0, k_at, 64, v_at, 64, F32, ints[0].data_ptr(), 3, ints[1].data_ptr(),
+                  ints[2].data_ptr(), 4, rows, rope=rope, q=q_at, q_stride=64, q_out=q_at, q_out_stride=64, heads=1)
+    cache.append(0, k, v, tables[:3], starts[:4], used[:3], (cos, sin, 64, False))
+    device.check_bytes(cache)
+    got = device.back(mq, 64)
+    position = np.concatenate([u + np.arange(c) for u, c in zip(used, counts)])
+    lost = (position >= 38) | (np.arange(rows) >= starts[3])
+    assert np.array_equal(np.isnan(got).all(1), lost) and np.array_equal(np.isnan(got).any(1), lost)
+    # Reading gives NaN for the same pages.
+    out = [device.rows(np.zeros((rows, 64)), F32) for _ in range(2)]
+    mp.kv8_read(device.view, 0, ints[0].data_ptr(), 3, ints[1].data_ptr(), ints[2].data_ptr(), 3, rows, F32,
+                out[0][1], 64, out[1][1], 64)
+    got = device.back(out[0][0], 64)
+    page = position // 16
+    sequence = np.repeat(np.arange(4), counts)
+    missing = np.array([p >= 3 or not 0 <= tables[s, min(p, 2)] < 6 for s, p in zip(sequence, page)])
+    inside = np.arange(rows) < starts[3]
+    assert np.array_equal(np.isnan(got).all(1)[inside], missing[inside])
+    assert np.all(got[~inside] == 0)
+
+
+# ---- attention ------------------------------------------------------------------
+
+
+def fill(cache, rng, tables, lengths, spread=1.0):
+    """Tokens of all layers appended by the reference; in the slots behind them stays whatever there was."""
+    for layer in range(cache.layers):
+        for s, n in enumerate(lengths):
+            if n > 0:
+                k, v = (rng.standard_normal((n, cache.kv_heads, cache.dim)).astype(np.float32) for _ in range(2))
+                k *= spread * np.exp(0.5 * rng.standard_normal(cache.dim)).astype(np.float32)
+                cache.append(layer, k, v, tables[s:s + 1], [0, n], [0])
+
+
+def workspace_for(device, rows, sequences, heads, max_length):
+    size = mp.kv8_attention_workspace(device.view, rows, sequences, heads, max_length)
+    return device.torch.full((max(size, 1),), 255, dtype=device.torch.uint8, device="cuda"), size
+
+
+def run_decode(device, layer, q, kind, tables, lengths, max_length, scale, pad=0, shift=0):
+    rows, width = q.shape[0], q.shape[1] * q.shape[2]
+    mq, q_at, q_stride = device.rows(q.reshape(rows, -1), kind, pad, shift)
+    mo, o_at, o_stride = device.rows(np.full((rows, width), 7.0), kind, pad, shift)
+    d_tables, d_lengths = device.ints(tables), device.ints(lengths)
+    space, size = workspace_for(device, rows, rows, q.shape[1], max_length)
+    mp.kv8_attention_decode(device.view, layer, q_at, q_stride, kind, d_tables.data_ptr(), tables.shape[1],
+                            d_lengths.data_ptr(), rows, q.shape[1], max_length, scale, o_at, o_stride,
+                            space.data_ptr(), size)
+    got = device.back(mo, width)
+    assert bool(mo[:, width:].isnan().all())
+    return got.reshape(q.shape)
+
+
+def run_prefill(device, layer, q, kind, tables, starts, used, max_length, scale, pad=0, shift=0):
+    rows, width = q.shape[0], q.shape[1] * q.shape[2]
+    mq, q_at, q_stride = device.rows(q.reshape(rows, -1), kind, pad, shift)
+    mo, o_at, o_stride = device.rows(np.full((rows, width), 7.0), kind, pad, shift)
+    ints = [device.ints(a) for a in (tables, starts, used)]
+    space, size = workspace_for(device, rows, len(used), q.shape[1], max_length)
+    mp.kv8_attention_prefill(device.view, layer, q_at, q_stride, kind, ints[0].data_ptr(), tables.shape[1],
+                             ints[1].data_ptr(), ints[2].data_ptr(), len(used), rows, q.shape[1], max_length, scale,
+                             o_at, o_stride, space.data_ptr(), size)
+    got = device.back(mo, width)
+    assert bool(mo[:, width:].isnan().all())
+    return got.reshape(q.shape)
+
+
+def check_row(got, want, err, kind, v_max, prefill, what):
+    limit = err + HALF_STEP[kind] * np.abs(want) + (HALF_STEP[F16] * v_max if prefill and kind != F32 else 0)
+    off = np.abs(got - want)
+    assert np.all(off <= limit), f"{what}: off by {off.max():.3e}, at most {float(np.max(limit)):.3e}"
+
+
+SHAPES = [
+    # kv_heads, heads, dim, bt, type, pad, shift
+    (3, 9, 64, 16, F32, 0, 0),
+    (1, 1, 64, 16, F32, 3, 1),
+    (2, 16, 64, 32, BF16, 8, 0),
+    (1, 12, 64, 64, F32, 0, 0),
+    (2, 8, 128, 16, F16, 0, 1),
+    (1, 16, 128, 128, F32, 4, 0),
+    (1, 5, 256, 16, F32, 0, 0),
+    (1, 11, 256, 64, BF16, 0, 0),
+]
+LENGTHS = [1, 2, 15, 16, 17, 31, 32, 33, 63, 65, 127, 128, 129, 300, 0, 511, -3, 777]
+
+
+@FORMATS
+@pytest.mark.parametrize("kv_heads, heads, dim, bt, kind, pad, shift", SHAPES)
+def test_decode(torch_cuda, fmt, kv_heads, heads, dim, bt, kind, pad, shift):
+    """Rows of every length at once, two layers, slots behind the last token holding anything (E4M3 NaN codes among
+    them); then a few of them alone with a larger max_length, so that their tokens are split."""
+    rng = np.random.default_rng(heads * dim + bt)
+    cache = Cache(blocks_for(LENGTHS, bt), 2, kv_heads, bt, dim, fmt, rng)
+    tables = tables_for(rng, cache.blocks, LENGTHS, bt)
+    fill(cache, rng, tables, LENGTHS)
+    device = Device(torch_cuda, cache)
+    q = rounded(rng.standard_normal((len(LENGTHS), heads, dim)), kind)
+    scale = 1.3 / dim ** 0.5
+    v_max = max(np.nanmax(np.abs(cache.tokens(1, 1, t, max(n, 1)))) for t, n in zip(tables, LENGTHS) if n > 0)
+    for pick, longest in ((range(len(LENGTHS)), 777), ((13, 17, 0), 5000), ((17,), 100000), ((12, 14), 129)):
+        pick = list(pick)
+        got = run_decode(device, 1, q[pick], kind, tables[pick], [LENGTHS[i] for i in pick], longest, scale, pad, shift)
+        for j, i in enumerate(pick):
+            want, err = cache.attention(1, q[i], tables[i], LENGTHS[i], scale)
+            check_row(got[j], want, err, kind, v_max, False, f"length {LENGTHS[i]} of at most {longest}")
+
+
+PREFILLS = [
+    # used, counts: whole prompts, chunks behind a history, single tokens among them, sequences without rows
+    ([0, 0, 0, 0], [1, 17, 100, 33]),
+    ([300, 0, 47, 16, 5], [1, 0, 61, 16, 1]),
+    ([900], [40]),
+    ([0], [260]),
+    ([31, 15, 2, 600], [1, 1, 1, 1]),
+]
+
+
+@FORMATS
+@pytest.mark.parametrize("kv_heads, heads, dim, bt, kind, pad, shift", SHAPES)
+def test_prefill(torch_cuda, fmt, kv_heads, heads, dim, bt, kind, pad, shift):
+    for case, (used, counts) in enumerate(PREFILLS):
+        rng = np.random.default_rng(heads + dim + bt + case)
+        lengths = [u + c for u, c in zip(used, counts)]
+        cache = Cache(blocks_for(lengths, bt), 2, kv_heads, bt, dim, fmt, rng)
+        tables = tables_for(rng, cache.blocks, lengths, bt)
+        fill(cache, rng, tables, lengths)
+        device = Device(torch_cuda, cache)
+        starts = starts_of(counts, first=1)
+        rows = int(starts[-1]) + 2
+        q = rounded(rng.standard_normal((rows, heads, dim)), kind)
+        scale = 1 / dim ** 0.5
+        for longest in (max(lengths), 40000):
+            got = run_prefill(device, 1, q, kind, tables, starts, used, longest, scale, pad, shift)
+            assert np.all(got[:1] == 7) and np.all(got[-2:] == 7)
+            for s, u in enumerate(used):
+                v_max = np.abs(cache.tokens(1, 1, tables[s], max(lengths[s], 1))).max()
+                rows_of = range(counts[s]) if counts[s] <= 40 else sorted({0, 1, 15, 16, counts[s] // 2, counts[s] - 2, counts[s] - 1})
+                for i in rows_of:
+                    r = starts[s] + i
+                    want, err = cache.attention(1, q[r], tables[s], u + i + 1, scale)
+                    check_row(got[r], want, err, kind, v_max, True, f"case {case}, position {u + i} of {longest}")
+
+
+def test_prefill_of_many_rows(torch_cuda):
+    """Enough rows that every wavefront takes several column tiles: 70 sequences of 60 to 129 rows (many of them
+    prompts), more sequences than a wavefront has lanes; sampled rows."""
+    for dim, kind, fmt in ((64, F32, INT8), (128, BF16, E4M3), (128, F32, E4M3), (256, F16, INT8)):
+        rng = np.random.default_rng(dim + kind)
+        kv_heads, heads, bt = 2, 6, 16
+        counts = [60 + s for s in range(70)]
+        used = [0 if s % 3 else 2 * s + 1 for s in range(70)]
+        lengths = [u + c for u, c in zip(used, counts)]
+        cache = Cache(blocks_for(lengths, bt), 1, kv_heads, bt, dim, fmt, rng)
+        # Random codes under the scales that are there: quicker than appending.
+        if fmt == E4M3:
+            for b in cache.bytes:
+                b[(b & 127) == 127] = 0
+        tables = tables_for(rng, cache.blocks, lengths, bt)
+        device = Device(torch_cuda, cache)
+        starts = starts_of(counts)
+        q = rounded(rng.standard_normal((int(starts[-1]), heads, dim)) * 0.02, kind)
+        got = run_prefill(device, 0, q, kind, tables, starts, used, max(lengths), 1 / dim ** 0.5)
+        assert np.isfinite(got).all()
+        for s in (0, 1, 2, 33, 63, 64, 65, 69):
+            v_max = np.abs(cache.tokens(0, 1, tables[s], lengths[s])).max()
+            for i in (0, 1, counts[s] // 2, counts[s] - 1):
+                r = starts[s] + i
+                want, err = cache.attention(0, q[r], tables[s], used[s] + i + 1, 1 / dim ** 0.5)
+                check_row(got[r], want, err, kind, v_max, True, f"dim {dim}, sequence {s}, row {i}")
+
+
+@FORMATS
+def test_attention_closed_form(torch_cuda, fmt):
+    """Scores of -1000 to 1001, and scales that differ by 2^40 between pages: exact powers, so the answer is known.
+    Keys are 8 in one dim, queries pick the score; values are one number a page."""
+    rng = np.random.default_rng(9)
+    bt, dim, pages = 16, 64, 6
+    cache = Cache(pages + 1, 1, 1, bt, dim, fmt, rng)
+    tables = np.arange(pages, dtype=np.int32)[None]
+    length = pages * bt
+    for kind in range(2):
+        cache.bytes[kind][:] = 128 if fmt == INT8 else 0
+    one = {INT8: 129, E4M3: int(np.flatnonzero(VALUES[E4M3] == 1)[0])}[fmt]
+    cache.bytes[0][:, :, :, cache.places[0][:, 0]] = one
+    cache.bytes[1][:, :, :, cache.places[1][:, 5]] = one
+    # Keys: page p scores 100 p (scale 1 after the softmax scale below), the last page the most.
+    scores = np.array([1, 2, 4, 8, 16, 32], dtype=np.float32)
+    cache.scales[:pages, 0, 0, 0] = scores
+    cache.scales[:pages, 0, 0, 1] = 2.0 ** np.array([40, -3, 5, 0, 2, -6])
+    device = Device(torch_cuda, cache)
+    q = np.zeros((3, 1, dim), dtype=np.float32)
+    q[:, 0, 0] = [1000, -1000, 1e-3]
+    got = run_decode(device, 0, q, F32, np.repeat(tables, 3, 0), [length] * 3, length, 1.0)
+    pre = run_prefill(device, 0, q[:1], F32, tables, [0, 1], [length - 1], length, 1.0)
+    # Far apart: one page takes all.
+    assert got[0, 0, 5] == 2.0 ** -6 and got[1, 0, 5] == 2.0 ** 40 and pre[0, 0, 5] == 2.0 ** -6
+    want, err = cache.attention(0, q[2], tables[0], length, 1.0)
+    assert np.all(np.abs(got[2] - want) <= err)
+    assert np.all(np.delete(got, 5, axis=2) == 0)
+
+
+def test_attention_beyond_what_is_there(torch_cuda):
+    """Page ids outside the pool, a page past the table, a row longer than max_length, NaN in a page or in q: NaN in
+    those rows and heads and nowhere else."""
+    rng = np.random.default_rng(10)
+    cache = Cache(12, 1, 2, 16, 64, INT8, rng)
+    tables = np.array([[0, 1, 2], [3, -1, 4], [5, 12, 6], [7, 8, 9], [7, 8, 9], [10, 8, 9], [0, 1, 2]], dtype=np.int32)
+    lengths = [48, 20, 33, 49, 48, 9, 48]
+    cache.scales[10, 0, 1, 1] = np.nan
+    q = rng.standard_normal((7, 4, 64)).astype(np.float32)
+    q[6, 2, 7] = np.inf
+    device = Device(torch_cuda, cache)
+    lost = np.zeros((7, 4), dtype=bool)
+    lost[[1, 2, 3]] = True
+    lost[5, 2:] = True
+    lost[6, 2] = True
+    for longest in (64, 4000):
+        got = run_decode(device, 0, q, F32, tables, lengths, longest, 0.1)
+        assert np.array_equal(np.isnan(got).all(2), lost) and np.array_equal(np.isnan(got).any(2), lost)
+        got = run_prefill(device, 0, q, F32, tables, range(8), [n - 1 for n in lengths], longest, 0.1)
+        assert np.array_equal(np.isnan(got).all(2), lost) and np.array_equal(np.isnan(got).any(2), lost)
+    lost[[0, 4, 6]] = True
+    got = run_decode(device, 0, q, F32, tables, lengths, 47, 0.1)
+    assert np.array_equal(np.isnan(got).all(2), lost)
+    got = run_prefill(device, 0, q, F32, tables, range(8), [n - 1 for n in lengths], 47, 0.1)
+    assert np.array_equal(np.isnan(got).all(2), lost)
+    got = run_prefill(device, 0, q, F32, tables, range(8), [-1, -5, 2 ** 31 - 1, 2 ** 30, 47, 8, 47], 64, 0.1)
+    lost[[0, 1, 2, 3]] = True
+    lost[4] = lost[6] = False
+    lost[6, 2] = True
+    assert np.array_equal(np.isnan(got).all(2), lost)
+
+
+def test_long_context(torch_cuda):
+    """70,000 tokens of which the pool holds 128 pages again and again: splits of more than one batch, positions past
+    16 bits; decode and a chunk of the last rows."""
+    rng = np.random.default_rng(11)
+    n, bt = 70001, 16
+    cache = Cache(128, 1, 1, bt, 64, INT8, rng)
+    tables = np.tile(np.arange(128, dtype=np.int32), -(-n // bt // 128) + 1)[None, :-(-n // bt)]
+    device = Device(torch_cuda, cache)
+    q = rng.standard_normal((3, 3, 64)).astype(np.float32) * 0.05
+    got = run_decode(device, 0, q[2:], F32, tables, [n], n, 0.125)[0]
+    pre = run_prefill(device, 0, q, F32, tables, [0, 3], [n - 3], n, 0.125)
+    v_max = np.abs(cache.tokens(0, 1, tables[0], n)).max()
+    for i in range(3):
+        want, err = cache.attention(0, q[i], tables[0], n - 2 + i, 0.125)
+        check_row(pre[i], want, err, F32, v_max, True, f"row {i}")
+        if i == 2:
+            check_row(got, want, err, F32, v_max, False, "decode")
+
+
+# ---- together ----------------------------------------------------------------
+
+
+def test_pool_past_four_gigabytes(torch_cuda):
+    """A pool whose last pages lie past 2^32 bytes: append there, read and attend."""
+    torch, blocks = torch_cuda, (1 << 32) // (16 * 64) + 40
+    pools = [torch.full((blocks, 16 * 64), 128, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = torch.ones((blocks, 2), device="cuda")
+    view = mp.Kv8Cache(pools[0].data_ptr(), pools[1].data_ptr(), scales.data_ptr(), blocks, 1, 16, 1, 64, INT8)
+    rng = np.random.default_rng(12)
+    small = Cache(4, 1, 1, 16, 64, INT8, rng)
+    k, v = (rng.standard_normal((30, 1, 64)).astype(np.float32) for _ in range(2))
+    small.append(0, k, v, np.array([[1, 3]]), [0, 30], [0])
+    ints = [torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([[blocks - 3, blocks - 1]], [0, 30], [0], [30])]
+    rows = [torch.from_numpy(a.reshape(30, 64)).cuda() for a in (k, v)]
+    mp.kv8_append(view, 0, rows[0].data_ptr(), 64, rows[1].data_ptr(), 64, F32, ints[0].data_ptr(), 2,
+                  ints[1].data_ptr(), ints[2].data_ptr(), 1, 30)
+    q = rng.standard_normal((1, 2, 64)).astype(np.float32)
+    dq, out = torch.from_numpy(q.reshape(1, -1)).cuda(), torch.zeros((1, 128), device="cuda")
+    mp.kv8_attention_decode(view, 0, dq.data_ptr(), 128, F32, ints[0].data_ptr(), 2, ints[3].data_ptr(), 1, 2, 32,
+                            0.125, out.data_ptr(), 128)
+    back = [torch.zeros((30, 64), device="cuda") for _ in range(2)]
+    mp.kv8_read(view, 0, ints[0].data_ptr(), 2, ints[1].data_ptr(), ints[2].data_ptr(), 1, 30, F32,
+                back[0].data_ptr(), 64, back[1].data_ptr(), 64)
+    torch.cuda.synchronize()
+    for kind in range(2):
+        assert np.array_equal(back[kind].cpu().numpy(), small.tokens(0, kind, [1, 3], 30)[0].astype(np.float32))
+        assert bool((pools[kind][:40] == 128).all())
+    want, err = small.attention(0, q[0], [1, 3], 30, 0.125)
+    check_row(out.cpu().numpy().reshape(2, 64), want, err, F32, 0, False, "decode")
+
+
+class Service:
+    """Three sequences over a two-layer cache: a prompt step, then decode steps, each layer an append and an
+    attention, on a stream of its own."""
+
+    def __init__(self, torch, fmt, kind):
+        self.torch, self.kind, self.rng = torch, kind, np.random.default_rng(13 + fmt)
+        self.kv_heads, self.heads, self.dim, self.bt, self.layers, self.most = 2, 6, 64, 16, 2, 400
+        self.counts = [37, 150, 5]
+        self.cache = Cache(3 * 25 + 1, 2, 2, 16, 64, fmt, self.rng)
+        self.device = Device(torch, self.cache)
+        self.tables = self.rng.permutation(75).astype(np.int32).reshape(3, 25)
+        self.d_tables = self.device.ints(self.tables)
+        self.cos, self.sin = angles(self.most, 64)
+        self.angles = [torch.from_numpy(a).cuda() for a in (self.cos, self.sin)]
+        self.rope = mp.Rope(self.angles[0].data_ptr(), self.angles[1].data_ptr(), self.most, 64, 0)
+        self.space, self.size = workspace_for(self.device, 192, 3, 6, self.most)
+
+    def rows(self, n):
+        return [rounded(self.rng.standard_normal((n, 6 + 2 + 2, 64)), self.kind) for _ in range(self.layers)]
+
+    def want(self, qkv, starts, used):
+        """The reference's step: outputs and bounds of every row and layer."""
+        from .kv8_reference import rotate
+        out = []
+        for layer in range(self.layers):
+            x = qkv[layer]
+            self.cache.append(layer, x[:, 6:8], x[:, 8:], self.tables, starts, used, (self.cos, self.sin, 64, False))
+            rows = []
+            for s in range(3):
+                for i in range(starts[s + 1] - starts[s]):
+                    p = used[s] + i
+                    q = rounded(rotate(x[starts[s] + i, :6], self.cos[p], self.sin[p], 64, False), self.kind)
+                    rows.append(self.cache.attention(layer, q, self.tables[s], p + 1, 0.125))
+            out.append(rows)
+        return out
+
+    def launch(self, qkv, out, starts, used, lengths, n, stream):
+        """qkv, out: per layer a device matrix; lengths: None for a prompt step."""
+        for layer in range(self.layers):
+            size = qkv[layer].element_size()
+            at, width, o = qkv[layer].data_ptr(), 10 * 64, out[layer].data_ptr()
+            mp.kv8_append(self.device.view, layer, at + 6 * 64 * size, width, at + 8 * 64 * size, width, self.kind,
+                          self.d_tables.data_ptr(), 25, starts.data_ptr(), used.data_ptr(), 3, n, rope=self.rope, q=at,
+                          q_stride=width, q_out=at, q_out_stride=width, heads=6, stream=stream)
+            if lengths is None:
+                mp.kv8_attention_prefill(self.device.view, layer, at, width, self.kind, self.d_tables.data_ptr(), 25,
+                                         starts.data_ptr(), used.data_ptr(), 3, n, 6, self.most, 0.125, o, 384,
+                                         self.space.data_ptr(), self.size, stream=stream)
+            else:
+                mp.kv8_attention_decode(self.device.view, layer, at, width, self.kind, self.d_tables.data_ptr(), 25,
+                                        lengths.data_ptr(), n, 6, self.most, 0.125, o, 384, self.space.data_ptr(),
+                                        self.size, stream=stream)
+
+    def check(self, got, want, prefill, what):
+        for layer in range(self.layers):
+            x = got[layer].float().cpu().numpy().reshape(-1, 6, 64)
+            v_max = max(np.nanmax(np.abs(self.cache.tokens(layer, 1, t, self.bt))) for t in self.tables) * 4
+            for r, (w, err) in enumerate(want[layer]):
+                check_row(x[r], w, err, self.kind, v_max, prefill, f"{what}, layer {layer}, row {r}")
+
+
+@FORMATS
+@pytest.mark.parametrize("kind", [F32, BF16], ids=["f32", "bf16"])
+def test_serving_with_a_replayed_graph(torch_cuda, fmt, kind):
+    """A prompt step, one direct decode step, then decode steps replayed from one graph of both layers' calls, whose
+    positions and rows change in place, with other work between the replays."""
+    torch = torch_cuda
+    service = Service(torch, fmt, kind)
+    dtype = getattr(torch, TYPES[kind])
+    stream = torch.cuda.Stream()
+    starts, used = starts_of(service.counts), np.zeros(3, dtype=np.int32)
+    n = int(starts[-1])
+    x = service.rows(n)
+    d = [torch.from_numpy(a.reshape(n, -1)).to("cuda", dtype) for a in x]
+    out = [torch.zeros((n, 384), dtype=dtype, device="cuda") for _ in range(2)]
+    d_starts, d_used = service.device.ints(starts), service.device.ints(used)
+    torch.cuda.synchronize()
+    service.launch(d, out, d_starts, d_used, None, n, stream.cuda_stream)
+    stream.synchronize()
+    service.check(out, service.want(x, starts, used), True, "prompt")
+    used = np.array(service.counts, dtype=np.int32)
+    one = service.device.ints([0, 1, 2, 3])
+    d_used, d_lengths = service.device.ints(used), service.device.ints(used + 1)
+    step = [torch.zeros((3, 640), dtype=dtype, device="cuda") for _ in range(2)]
+    result = [torch.zeros((3, 384), dtype=dtype, device="cuda") for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    for i in range(7):
+        x = service.rows(3)
+        for a, b in zip(step, x):
+            a.copy_(torch.from_numpy(b.reshape(3, -1)))
+        d_used.copy_(torch.from_numpy(used))
+        d_lengths.copy_(torch.from_numpy(used + 1))
+        torch.cuda.synchronize()
+        if i == 0:
+            service.launch(step, result, one, d_used, d_lengths, 3, stream.cuda_stream)
+            stream.synchronize()
+        else:
+            if i == 1:
+                with torch.cuda.graph(graph, stream=stream):
+                    service.launch(step, result, one, d_used, d_lengths, 3, stream.cuda_stream)
+                service.space.fill_(255)
+            graph.replay()
+            torch.cuda.synchronize()
+        service.check(result, service.want(x, [0, 1, 2, 3], used), False, f"step {i}")
+        service.device.check_bytes(service.cache)
+        used = used + 1
+
+
+def test_two_streams_with_workspaces_of_their_own(torch_cuda):
+    """Two decode calls that may overlap give what each gives alone, bit for bit, again and again."""
+    torch = torch_cuda
+    rng = np.random.default_rng(14)
+    cache = Cache(400, 1, 3, 16, 64, INT8, rng)
+    device = Device(torch, cache)
+    calls = []
+    for i, longest in enumerate((3000, 2500)):
+        tables = rng.integers(0, 400, (4, 188)).astype(np.int32)
+        lengths = [longest, 1, longest // 2, 700]
+        q = torch.from_numpy((rng.standard_normal((4, 576)) * 0.05).astype(np.float32)).cuda()
+        space, size = workspace_for(device, 4, 4, 9, longest)
+        calls.append((q, device.ints(tables), device.ints(lengths), longest, space, size,
+                      torch.zeros((4, 576), device="cuda"), torch.cuda.Stream()))
+
+    def launch(c, stream):
+        q, tables, lengths, longest, space, size, out, _ = c
+        mp.kv8_attention_decode(device.view, 0, q.data_ptr(), 576, F32, tables.data_ptr(), 188, lengths.data_ptr(), 4,
+                                9, longest, 0.125, out.data_ptr(), 576, space.data_ptr(), size, stream=stream)
+
+    torch.cuda.synchronize()
+    alone = []
+    for c in calls:
+        launch(c, None)
+        torch.cuda.synchronize()
+        alone.append(c[6].clone())
+        assert bool(c[6].isfinite().all())
+    for _ in range(20):
+        for c in calls:
+            c[6].zero_()
+        torch.cuda.synchronize()
+        for c in calls:
+            launch(c, c[7].cuda_stream)
+        torch.cuda.synchronize()
+        for c, want in zip(calls, alone):
+            assert torch.equal(c[6], want)

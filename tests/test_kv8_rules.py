@@ -1,0 +1,134 @@
+"""The 8-bit K/V cache without a GPU: what its calls touch and how they are
+divided (tests/native/kv8_rules_tests.cpp), and what the C entries refuse
+before any launch."""
+import ctypes
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from tinyinfer_amd import backend as mp
+
+ROOT = Path(__file__).resolve().parent.parent
+GXX = shutil.which("g++")
+P = 4096  # an aligned address that is never read: a refused call launches nothing
+
+
+@pytest.mark.skipif(GXX is None, reason="g++ not available")
+def test_kv8_rules(tmp_path):
+    exe = tmp_path / "kv8_rules_tests"
+    subprocess.run([GXX, "-std=c++17", "-Wall", "-Werror", "-g", "-fsanitize=address,undefined",
+                    "-fno-sanitize-recover=undefined", f"-I{ROOT / 'tinyinfer_amd' / 'csrc' / 'backend'}",
+                    str(ROOT / "tests" / "native" / "kv8_rules_tests.cpp"), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and run.stdout == "ok\n", run.stderr
+
+
+def cache(**changes):
+    c = dict(keys=P, values=P, scales=P, blocks=8, layers=2, block_tokens=16, kv_heads=3, dim=64, format=mp.KV8_INT8)
+    c.update(changes)
+    return mp.Kv8Cache(*[c[n] for n, _ in mp.Kv8Cache._fields_])
+
+
+def append(c=None, layer=0, **changes):
+    a = dict(k=P, k_stride=192, v=P, v_stride=192, type=mp.TYPE_F32, tables=P, table_stride=4, starts=P, used=P,
+             sequences=2, rows=5, rope=None, q=P, q_stride=576, q_out=P, q_out_stride=576, heads=9)
+    a.update(changes)
+    mp.kv8_append(c or cache(), layer, **a)
+
+
+def read(c=None, layer=0, **changes):
+    a = dict(tables=P, table_stride=4, starts=P, used=P, sequences=2, rows=5, type=mp.TYPE_F32, k=P, k_stride=192,
+             v=P, v_stride=192)
+    a.update(changes)
+    mp.kv8_read(c or cache(), layer, **a)
+
+
+def decode(c=None, layer=0, **changes):
+    a = dict(q=P, q_stride=576, type=mp.TYPE_F32, tables=P, table_stride=4, lengths=P, rows=5, heads=9, max_length=64,
+             scale=0.125, out=P, out_stride=576)
+    a.update(changes)
+    mp.kv8_attention_decode(c or cache(), layer, **a)
+
+
+def prefill(c=None, layer=0, **changes):
+    a = dict(q=P, q_stride=576, type=mp.TYPE_F32, tables=P, table_stride=4, starts=P, used=P, sequences=2, rows=5,
+             heads=9, max_length=64, scale=0.125, out=P, out_stride=576)
+    a.update(changes)
+    mp.kv8_attention_prefill(c or cache(), layer, **a)
+
+
+def workspace(c=None, rows=5, sequences=2, heads=9, max_length=64):
+    return mp.kv8_attention_workspace(c or cache(), rows, sequences, heads, max_length)
+
+
+BAD_CACHES = [dict(keys=None), dict(values=None), dict(scales=None), dict(keys=P + 8), dict(values=P + 4),
+              dict(scales=P + 4), dict(block_tokens=8), dict(block_tokens=24), dict(block_tokens=256),
+              dict(block_tokens=0), dict(dim=32), dict(dim=96), dict(dim=512), dict(format=2), dict(format=-1),
+              dict(blocks=0), dict(layers=0), dict(kv_heads=0), dict(kv_heads=2000)]
+
+
+def refused(call, text):
+    with pytest.raises(mp.BackendError, match=text) as e:
+        call()
+    assert e.value.status == mp.MP_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("changes", BAD_CACHES, ids=str)
+def test_bad_caches_are_refused(changes):
+    for call in (append, read, decode, prefill):
+        refused(lambda: call(cache(**changes)), "8-bit")
+    if not {"keys", "values", "scales"} & set(changes):
+        refused(lambda: workspace(cache(**changes)), "8-bit")
+
+
+def test_bad_layers_are_refused():
+    for call in (append, read, decode, prefill):
+        for layer in (-1, 2):
+            refused(lambda: call(layer=layer), "no such layer")
+
+
+@pytest.mark.parametrize("call, changes, text", [
+    (append, dict(k=None), "row matrix"), (append, dict(v=P + 2), "row matrix"), (append, dict(k_stride=191), "stride"),
+    (append, dict(v_stride=-192), "stride"), (append, dict(type=3), "element type"), (append, dict(q_out=None), "row matrix"),
+    (append, dict(q_stride=575), "stride"), (append, dict(q_out_stride=600), "in place"), (append, dict(heads=0), "heads"),
+    (append, dict(tables=None), "tables"), (append, dict(table_stride=0), "table_stride"), (append, dict(starts=None), "starts"),
+    (append, dict(used=P + 2), "starts or used"), (append, dict(rows=-1), "rows"), (append, dict(rows=(1 << 20) + 1), "rows"),
+    (append, dict(sequences=-1), "sequences"),
+    (append, dict(rope=mp.Rope(P, P, 10, 63, 0)), "rotated dims"), (append, dict(rope=mp.Rope(P, P, 10, 66, 0)), "rotated dims"),
+    (append, dict(rope=mp.Rope(P, P, 10, -2, 0)), "rotated dims"), (append, dict(rope=mp.Rope(None, P, 10, 64, 0)), "tables"),
+    (append, dict(rope=mp.Rope(P, P, 0, 64, 0)), "tables"),
+    (append, dict(rows=1 << 20, k_stride=65536, v_stride=65536, c=cache(kv_heads=1024), q=None), "too many"),
+    (read, dict(k=None), "row matrix"), (read, dict(v_stride=100), "stride"), (read, dict(starts=None), "starts"),
+    (read, dict(type=-1), "element type"),
+    (decode, dict(q=None), "row matrix"), (decode, dict(out=None), "row matrix"), (decode, dict(q_stride=64), "stride"),
+    (decode, dict(lengths=None), "lengths"), (decode, dict(heads=10), "multiple of kv_heads"),
+    (decode, dict(heads=51, q_stride=51 * 64, out_stride=51 * 64), "at most 16"), (decode, dict(heads=0), "heads"),
+    (decode, dict(max_length=-1), "max_length"), (decode, dict(max_length=(1 << 30) + 1), "max_length"),
+    (decode, dict(scale=float("nan")), "scale"), (decode, dict(scale=float("inf")), "scale"),
+    (decode, dict(scale=-1.0), "scale"), (decode, dict(max_length=10000), "workspace"),
+    (decode, dict(max_length=10000, workspace=P + 4, workspace_bytes=1 << 30), "aligned"),
+    (decode, dict(max_length=10000, workspace=None, workspace_bytes=1 << 30), "workspace"),
+    (prefill, dict(starts=None), "starts"), (prefill, dict(used=None), "used"), (prefill, dict(scale=float("nan")), "scale"),
+    (prefill, dict(max_length=100000), "workspace"), (prefill, dict(out_stride=10), "stride"),
+], ids=lambda v: getattr(v, "__name__", str(v)))
+def test_bad_arguments_are_refused(call, changes, text):
+    refused(lambda: call(**changes), text)
+
+
+def test_nothing_to_do_launches_nothing():
+    for call in (append, read, prefill):
+        call(rows=0)
+        call(sequences=0)
+    decode(rows=0)
+    assert workspace(rows=0) == 0 and workspace(max_length=0) == 0
+
+
+def test_workspace_sizes():
+    # One row needs none while one work-group's chunk holds it; long ones do.
+    assert workspace(rows=1, sequences=1, max_length=128) == 0
+    assert workspace(rows=1, sequences=1, max_length=16384) >= 9 * 66 * 4
+    size = ctypes.c_size_t()
+    assert mp.lib().mp_hip_kv8_attention_workspace(cache(), 1, 1, 9, 64, None) == mp.MP_INVALID_ARGUMENT
+    assert mp.lib().mp_hip_kv8_attention_workspace(None, 1, 1, 9, 64, ctypes.byref(size)) == mp.MP_INVALID_ARGUMENT

@@ -44,6 +44,20 @@ class KernelTimes(ctypes.Structure):
 
 
 TIME_ATTENTION, TIME_PROJECTION, TIME_HEAD, TIME_SAMPLED = 1, 2, 4, 8
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+KV8_INT8, KV8_E4M3 = 0, 1
+
+
+class Kv8Cache(ctypes.Structure):
+    """A paged K/V cache in 8 bits on the caller's device buffers (mp_kv8_cache)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("keys", "values", "scales")] + [
+        (n, ctypes.c_int32) for n in ("blocks", "layers", "block_tokens", "kv_heads", "dim", "format")]
+
+
+class Rope(ctypes.Structure):
+    """Rotary tables on the device and how heads turn by them (mp_rope)."""
+    _fields_ = [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p)] + [
+        (n, ctypes.c_int32) for n in ("positions", "dims", "interleaved")]
 
 
 class BackendError(RuntimeError):
@@ -70,6 +84,15 @@ def _bind(lib):
     lib.mp_hip_paged_attention_decode_noalloc.argtypes = [vp, vp, vp, vp] + [ctypes.c_int32] * 7 + [vp, vp]
     lib.mp_hip_paged_attention_decode_fast.argtypes = [vp, vp, vp, vp, ctypes.c_int32, I32P] + \
         [ctypes.c_int32] * 7 + [vp, vp]
+    i32, i64, size, cache = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.POINTER(Kv8Cache)
+    lib.mp_hip_kv8_append.argtypes = [cache, i32, vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, ctypes.POINTER(Rope),
+                                      vp, i32, vp, vp, i32, i32, vp]
+    lib.mp_hip_kv8_read.argtypes = [cache, i32, vp, i32, vp, vp, i32, i32, i32, vp, i64, vp, i64, vp]
+    lib.mp_hip_kv8_attention_workspace.argtypes = [cache, i32, i32, i32, i32, ctypes.POINTER(size)]
+    lib.mp_hip_kv8_attention_decode.argtypes = [cache, i32, vp, i64, i32, vp, i32, vp, i32, i32, i32, ctypes.c_float,
+                                                vp, i64, vp, size, vp]
+    lib.mp_hip_kv8_attention_prefill.argtypes = [cache, i32, vp, i64, i32, vp, i32, vp, vp, i32, i32, i32, i32,
+                                                 ctypes.c_float, vp, i64, vp, size, vp]
     lib.mp_hip_sync.argtypes = [vp]
     lib.mp_hip_stats.argtypes = [vp, ctypes.POINTER(Counters)]
     lib.mp_hip_kv_pools.argtypes = [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_size_t)]
@@ -232,3 +255,55 @@ def paged_attention_decode_fast(q, keys, values, tables, table_stride: int, leng
     if status:
         message = (lib().mp_hip_last_error(None) or b"").decode()
         raise BackendError(status, f"mp_hip_paged_attention_decode_fast failed ({status}): {message}")
+
+
+def _kv8_check(status: int, name: str):
+    if status:
+        message = (lib().mp_hip_last_error(None) or b"").decode()
+        raise BackendError(status, f"{name} failed ({status}): {message}")
+
+
+def kv8_append(cache: Kv8Cache, layer: int, k, k_stride: int, v, v_stride: int, type: int, tables, table_stride: int,
+               starts, used, sequences: int, rows: int, rope: Rope | None = None, q=None, q_stride: int = 0,
+               q_out=None, q_out_stride: int = 0, heads: int = 0, stream: int | None = None):
+    """New tokens' keys (rotated by `rope`) and values into the pages of an
+    8-bit cache, and the rotated queries to q_out (raw device pointers;
+    strides in elements). Asynchronous on `stream`."""
+    _kv8_check(lib().mp_hip_kv8_append(cache, layer, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride,
+                                       heads, type, rope, tables, table_stride, starts, used, sequences, rows,
+                                       stream), "mp_hip_kv8_append")
+
+
+def kv8_read(cache: Kv8Cache, layer: int, tables, table_stride: int, starts, used, sequences: int, rows: int,
+             type: int, k, k_stride: int, v, v_stride: int, stream: int | None = None):
+    """Tokens of an 8-bit cache as rows of values. Asynchronous on `stream`."""
+    _kv8_check(lib().mp_hip_kv8_read(cache, layer, tables, table_stride, starts, used, sequences, rows, type, k,
+                                     k_stride, v, v_stride, stream), "mp_hip_kv8_read")
+
+
+def kv8_attention_workspace(cache: Kv8Cache, rows: int, sequences: int, heads: int, max_length: int) -> int:
+    """Workspace bytes for the attention calls of up to these sizes."""
+    size = ctypes.c_size_t()
+    _kv8_check(lib().mp_hip_kv8_attention_workspace(cache, rows, sequences, heads, max_length, ctypes.byref(size)),
+               "mp_hip_kv8_attention_workspace")
+    return size.value
+
+
+def kv8_attention_decode(cache: Kv8Cache, layer: int, q, q_stride: int, type: int, tables, table_stride: int,
+                         lengths, rows: int, heads: int, max_length: int, scale: float, out, out_stride: int,
+                         workspace=None, workspace_bytes: int = 0, stream: int | None = None):
+    """Attention of one query row per sequence over an 8-bit cache; `lengths`
+    on the device. Asynchronous on `stream`."""
+    _kv8_check(lib().mp_hip_kv8_attention_decode(cache, layer, q, q_stride, type, tables, table_stride, lengths, rows,
+                                                 heads, max_length, scale, out, out_stride, workspace,
+                                                 workspace_bytes, stream), "mp_hip_kv8_attention_decode")
+
+
+def kv8_attention_prefill(cache: Kv8Cache, layer: int, q, q_stride: int, type: int, tables, table_stride: int,
+                          starts, used, sequences: int, rows: int, heads: int, max_length: int, scale: float, out,
+                          out_stride: int, workspace=None, workspace_bytes: int = 0, stream: int | None = None):
+    """Causal attention of packed rows over an 8-bit cache that holds them
+    already. Asynchronous on `stream`."""
+    _kv8_check(lib().mp_hip_kv8_attention_prefill(cache, layer, q, q_stride, type, tables, table_stride, starts, used,
+                                                  sequences, rows, heads, max_length, scale, out, out_stride,
+                                                  workspace, workspace_bytes, stream), "mp_hip_kv8_attention_prefill")

@@ -1,0 +1,113 @@
+// What a call on the 8-bit cache touches and how it is divided among
+// work-groups: plain functions (no HIP; the kernels call the constexpr ones),
+// so that they can be checked without a GPU.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+namespace mphip {
+
+constexpr int kTile = 16;  // tokens of a tile
+constexpr int kKv8MaxRows = 1 << 20, kKv8MaxHeads = 1024, kKv8MaxGroup = 16, kKv8MaxLength = 1 << 30;
+
+// Rows start .. next-1 of a sequence inside 0 .. rows-1, whatever the two are.
+struct Kv8Span {
+    int row0, count;
+};
+constexpr Kv8Span kv8_span(int start, int next, int rows) {
+    const int row0 = start < 0 ? 0 : start > rows ? rows : start;
+    const int row1 = next < row0 ? row0 : next > rows ? rows : next;
+    return {row0, row1 - row0};
+}
+
+// Pages that `count` (at least 1) tokens from position `used` on touch; none
+// for a position that no sequence has.
+constexpr int kv8_pages(int count, int used, int page_shift) {
+    const int bt = 1 << page_shift;
+    return used < 0 || used > kKv8MaxLength ? 0 : ((used & (bt - 1)) + count + bt - 1) >> page_shift;
+}
+// The `index`-th of those pages: its number in the table, its slots that the
+// tokens take and the token (of `count`) that takes the first of them.
+struct Kv8Page {
+    int page, first, last, token;
+};
+constexpr Kv8Page kv8_page(int count, int used, int index, int page_shift) {
+    const int page = (used >> page_shift) + index, begin = page << page_shift, end = used + count - begin;
+    const int first = used > begin ? used - begin : 0, bt = 1 << page_shift;
+    return {page, first, end < bt ? end : bt, begin + first - used};
+}
+// Pages that `rows` rows of `sequences` sequences touch at most: all but the
+// first and last of a sequence are filled, and each has a row at least.
+constexpr int64_t kv8_most_pages(int rows, int sequences, int bt) {
+    const int64_t by_pages = ((int64_t)rows + (int64_t)sequences * (2 * bt - 2)) / bt;
+    return by_pages < rows ? by_pages : rows;
+}
+// A table's page `page` if it is one of the pool's, else -1.
+constexpr int kv8_block(const int32_t* table, int stride, int page, int blocks) {
+    if (page < 0 || page >= stride) return -1;
+    const int block = table[page];
+    return block >= 0 && block < blocks ? block : -1;
+}
+
+// A work-group takes 16 * column_tiles columns (a column is one row's query
+// head) of a KV head and `chunk` of their tokens; its `waves` wavefronts deal
+// the chunk's pairs of 16-token tiles among themselves. With more than one
+// chunk the results meet in a second launch.
+struct Kv8Plan {
+    int column_tiles, waves, chunk, splits;
+};
+
+constexpr int kKv8Pair = 32;          // tokens of two tiles, a step of a wavefront
+constexpr int kKv8Groups = 1024;      // work-groups that splitting over tokens aims at
+constexpr int kKv8LeastChunk = 128;   // tokens
+
+constexpr int64_t kv8_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tokens a chunk and how many chunks, for `items` work-groups a chunk.
+inline void kv8_split(Kv8Plan* p, int64_t items, int max_length) {
+    const int64_t step = (int64_t)kKv8Pair * p->waves;
+    const int64_t length = max_length > 0 ? max_length : 1;
+    int64_t splits = kv8_ceil(kKv8Groups, items > 0 ? items : 1);
+    int64_t chunk = kv8_ceil(kv8_ceil(length, splits), step) * step;
+    if (chunk < kKv8LeastChunk) chunk = kKv8LeastChunk;
+    p->chunk = (int)chunk;
+    p->splits = (int)kv8_ceil(length, chunk);
+}
+
+inline Kv8Plan kv8_decode_plan(int rows, int kv_heads, int max_length) {
+    Kv8Plan p{1, 4, 0, 0};
+    kv8_split(&p, (int64_t)rows * kv_heads, max_length);
+    return p;
+}
+
+// Column tiles of all sequences: every sequence's last one may be part empty.
+inline int64_t kv8_items(int rows, int sequences, int group, int column_tiles) {
+    const int64_t columns = 16 * column_tiles, by_tiles = (int64_t)rows * group / columns + sequences;
+    return by_tiles < rows * (int64_t)group ? by_tiles : rows * (int64_t)group;
+}
+
+// most_tiles: the column tiles a wavefront's registers hold.
+inline Kv8Plan kv8_prefill_plan(int rows, int sequences, int kv_heads, int group, int most_tiles, int max_length) {
+    Kv8Plan p{most_tiles, 8, 0, 0};
+    while (p.column_tiles > 1 && kv8_items(rows, sequences, group, p.column_tiles) * kv_heads < 512) p.column_tiles /= 2;
+    kv8_split(&p, kv8_items(rows, sequences, group, p.column_tiles) * kv_heads, max_length);
+    return p;
+}
+
+// Floats that a plan's partial results take.
+inline size_t kv8_partial_floats(const Kv8Plan& p, int rows, int heads, int dim) {
+    return p.splits > 1 ? (size_t)rows * heads * p.splits * (dim + 2) : 0;
+}
+
+// Floats that hold the partial results of any call of up to these sizes:
+// items * splits < 2 * kKv8Groups while there is more than one split.
+inline size_t kv8_workspace_floats(int rows, int sequences, int heads, int kv_heads, int dim, int max_length) {
+    (void)sequences;
+    const int64_t splits = kv8_ceil(max_length > 0 ? max_length : 1, kKv8LeastChunk);
+    if (splits <= 1) return 0;
+    const int64_t columns = 16 * 4;  // of the largest work-group
+    const int64_t by_rows = (int64_t)rows * heads * splits, by_groups = 2ll * kKv8Groups * columns;
+    return (size_t)(by_rows < by_groups ? by_rows : by_groups) * (dim + 2);
+}
+
+}  // namespace mphip
