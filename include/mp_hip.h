@@ -219,7 +219,8 @@ int mp_hip_paged_attention_decode_noalloc(const float* q, const float* keys, con
  * is not written) or scale times the E4M3 number b (MP_KV8_E4M3: 448 largest,
  * 0x7F and 0xFF NaN). Scales are powers of two from 2^-126 on, so that raising
  * one moves codes without another rounding of the scale, and every value is
- * exact in FP32, BF16 and (in its range) FP16. Order of a head's bytes: tiles
+ * exact in FP32, BF16 and (in its range) FP16. A block takes less than 2 GiB
+ * of keys. Order of a head's bytes: tiles
  * of 16 tokens; inside a tile keys are [dim/16][slot][16 dims], values
  * [dim/64][slot/4][dim%16][dim%64/16][slot%4]: the matrix cores' operands,
  * 16 bytes a lane. A block is contiguous in all three arrays: copying one on

@@ -66,7 +66,7 @@ def workspace(c=None, rows=5, sequences=2, heads=9, max_length=64):
 BAD_CACHES = [dict(keys=None), dict(values=None), dict(scales=None), dict(keys=P + 8), dict(values=P + 4),
               dict(scales=P + 4), dict(block_tokens=8), dict(block_tokens=24), dict(block_tokens=256),
               dict(block_tokens=0), dict(dim=32), dict(dim=96), dict(dim=512), dict(format=2), dict(format=-1),
-              dict(blocks=0), dict(layers=0), dict(kv_heads=0), dict(kv_heads=2000)]
+              dict(blocks=0), dict(layers=0), dict(layers=1 << 20), dict(blocks=1 << 28), dict(kv_heads=0), dict(kv_heads=2000)]
 
 
 def refused(call, text):

@@ -188,6 +188,10 @@ inline const char* kv8_wrong_cache(const mp_kv8_cache* c, int layer) {
     if (c->format != MP_KV8_INT8 && c->format != MP_KV8_E4M3) return "8-bit cache: unknown format";
     if (c->blocks < 1 || c->layers < 1 || c->kv_heads < 1 || c->kv_heads > kKv8MaxHeads)
         return "8-bit cache: blocks, layers and kv_heads must be positive (kv_heads at most 1024)";
+    if ((int64_t)c->layers * c->kv_heads * c->block_tokens * c->dim >= (int64_t)1 << 31)
+        return "8-bit cache: a block's keys must be smaller than 2 GiB";
+    if ((int64_t)c->blocks * c->layers >= ((int64_t)1 << 29) / c->kv_heads)  // 512 GiB of keys at the least
+        return "8-bit cache: blocks * layers * kv_heads must be smaller than 2^29";
     if (layer < 0 || layer >= c->layers) return "8-bit cache: no such layer";
     return nullptr;
 }

@@ -26,6 +26,8 @@
 // The key scale multiplies the score with the softmax scale; the value scale,
 // as a power of two relative to the largest met so far, is applied with the
 // conversion of the value codes, where it is exact.
+#include <type_traits>
+
 #include "kernels.h"
 #include "kv8.h"
 
@@ -65,10 +67,6 @@ __device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7FC00000
 __device__ __forceinline__ float column_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ __forceinline__ float column_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
 }
 
 // Four codes times a power of two as FP16. INT8: a byte b under 0x64 is the
@@ -117,41 +115,52 @@ union Half8 {
     _Float16 one[8];
 };
 
-// One tile's bytes as a lane holds them, and its scales' bits (uniform).
-template <int DIM>
-struct RawTile {
-    u4 k[DIM / 64], v[DIM / 64];
-    uint32_t k_scale, v_scale;
-};
+// A load through the scalar cache, at byte `offset` of an array that no kernel
+// beside this one writes; uniform over the wavefront.
+__device__ __forceinline__ int scalar_int(const void* p, uint32_t offset) {
+    return *(const __attribute__((address_space(4))) int32_t*)((uintptr_t)p + offset);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
-template <int DIM>
-__device__ __forceinline__ void load_tile(const Kv8Layer& kv, int head, int block, int tile, int lane,
-                                          RawTile<DIM>* out) {
-    const size_t index = kv8_head(kv, max(block, 0), head);
-    const size_t base = index * ((size_t)DIM << kv.page_shift) +
-                        (tile & ((1 << (kv.page_shift - 4)) - 1)) * (kTile * DIM) + 16 * lane;
-#pragma unroll
-    for (int j = 0; j < DIM / 64; ++j) {
-        out->k[j] = *reinterpret_cast<const u4*>(kv.keys + base + 1024 * j);
-        out->v[j] = *reinterpret_cast<const u4*>(kv.values + base + 1024 * j);
-    }
-    const float2 s = kv.scales[index];
-    const uint32_t bad = 0x7FC00000u;  // NaN for a page that is none
-    out->k_scale = __builtin_amdgcn_readfirstlane(block < 0 ? bad : __float_as_uint(s.x));
-    out->v_scale = __builtin_amdgcn_readfirstlane(block < 0 ? bad : __float_as_uint(s.y));
+// x - (float)half of the low or high half, times `factor`: factor * half + x.
+__device__ __forceinline__ float mix_low(h2 half, float factor, float x) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(half), "v"(factor), "v"(x));
+    return r;
+}
+__device__ __forceinline__ float mix_high(h2 half, float factor, float x) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(half), "v"(factor), "v"(x));
+    return r;
+}
+
+// 16-dim tiles of every wavefront that meet in LDS at a time, in 32 KB of it
+// where that holds one: 1 KB a tile, wavefront and column tile.
+constexpr int join_dims(int waves, int column_tiles, int dims) {
+    const int fit = 32 / (waves * column_tiles);
+    return fit < 1 ? 1 : fit < dims ? fit : dims;
+}
+constexpr size_t join_bytes(int waves, int column_tiles, int dims) {
+    return waves == 1 ? 0 : (size_t)waves * column_tiles * join_dims(waves <= 4 ? 4 : kKv8MostWaves, column_tiles, dims) * 1024;
 }
 
 // DECODE: one row a sequence, its columns the KV head's query heads; else
 // columns are those of a sequence's rows, row major.
 template <int FORMAT, int DIM, int NT, int MODE, bool DECODE>
-__global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(AttentionArgs a) {
+    constexpr int kDepth = DECODE ? 2 : 1;
     constexpr int kSteps = DIM / 32;             // of the contraction over dims
     constexpr int kDims = DIM / 16;              // 16-dim tiles of the output
     constexpr int kParts = MODE == kTwo ? 2 : 1;  // operands of a query or probability
     constexpr int kColumns = MODE == kPacked ? 8 : 16;
     static_assert(MODE != kPacked || (NT == 1 && DECODE), "one row's heads");
-    __shared__ f4 o_s[8][NT][64];
-    __shared__ float2 ml_s[8][NT][16];
+    extern __shared__ f4 shared_s[];  // join_bytes
+    f4(*const o_s)[64] = reinterpret_cast<f4(*)[64]>(shared_s);
+    float2(*const ml_s)[NT][16] = reinterpret_cast<float2(*)[NT][16]>(shared_s);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int head = blockIdx.y, split = blockIdx.z;
@@ -162,7 +171,7 @@ __global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) 
     if (DECODE) {
         sequence = row0 = blockIdx.x;
         count = 1;
-        const int length = a.rows.used[sequence];
+        const int length = scalar_int(a.rows.used, (uint32_t)sequence * 4u);
         used = min(length, a.max_length + 1) - 1;
         first = 0;
         if (length <= 0) {  // nothing to see: zeros
@@ -212,28 +221,140 @@ __global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) 
         q_at[t] = (row0 + row) * a.q_stride + ((int64_t)head * a.group + column % a.group) * DIM;
     }
 
-    // Pairs of tiles: first + wave, + waves, ... of the chunk's.
+    // This wavefront's pairs of tiles: pair0, + waves, ... of the chunk's, `n`
+    // of them done, `pairs` in all.
     const int32_t* const table = a.rows.tables + (size_t)sequence * a.rows.table_stride;
-    const int tile_end = (end + kTile - 1) / kTile;
-    const int pair_end = (tile_end + 1) / 2;
-    int pair = begin / kKv8Pair + wave;
-    RawTile<DIM> next[2];
-    int block[2];
-    const auto find_blocks = [&](int p) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            block[h] = __builtin_amdgcn_readfirstlane(
-                kv8_block(table, a.rows.table_stride, min(2 * p + h, tile_end - 1) >> (a.kv.page_shift - 4),
-                          a.kv.blocks));
+    const int tile_end = (end + kTile - 1) / kTile, pair0 = begin / kKv8Pair + wave;
+    const int pairs = max((tile_end + 1) / 2 - pair0 + waves - 1, 0) / waves;
+
+    // The loop runs on pairs in two strands that do not wait for each other:
+    // the scores of pair n+1 are multiplied while the probabilities of pair n
+    // are formed and multiplied with its values. Keys are loaded kDepth + 1
+    // and values kDepth pairs ahead, into the registers just used up. Behind
+    // the last pair the loads are of no bytes: their number is the same at
+    // every step, and so is what a step waits for.
+    //
+    // Where tiles lie and their scales are worked out by the lanes: lane l
+    // holds tile l%2 of the pairs whose number is l/2 modulo 32, and a step
+    // reads what it needs from a lane. Every 16 pairs half the lanes go on to
+    // the pairs 32 on, whose scales were fetched 16 pairs and whose table
+    // entries 32 pairs before. A page that is none reads page 0 and has NaN
+    // scales; a tile behind the last (of a row that ends in a pair's first
+    // tile) reads page 0 and has scales 0.
+    const uint32_t block_scales = (uint32_t)a.kv.layers * a.kv.kv_heads;  // heads of a block
+    const uint32_t block_bytes = block_scales * DIM << a.kv.page_shift;
+    const uint32_t head_bytes = (uint32_t)(a.kv.layer * a.kv.kv_heads + head) * DIM << a.kv.page_shift;
+    const float2* const scales = a.kv.scales + (a.kv.layer * a.kv.kv_heads + head);
+    struct Tiles {
+        uint64_t base;
+        float2 bits;
+        uint32_t none, present;  // bits of NaN or 0; all bits or 0
     };
-    const auto load_pair = [&](int p) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) load_tile<DIM>(a.kv, head, block[h], min(2 * p + h, tile_end - 1), lane, &next[h]);
+    uint32_t at_low, at_high, at_k, at_v;  // this lane's tile: where, and its scales' bits
+    Tiles soon;                            // of the pairs 32 on
+    int found;                             // their successors' table entry
+    const auto tile_of = [&](int n) { return 2 * (pair0 + n * waves) + (lane & 1); };
+    const auto find_block = [&](int n) {
+        return table[min(tile_of(n) >> (a.kv.page_shift - 4), a.rows.table_stride - 1)];
     };
-    if (pair < pair_end) {
-        find_blocks(pair);
-        load_pair(pair);
-        find_blocks(min(pair + waves, pair_end - 1));
+    const auto find_tile = [&](int n, int block) {
+        const int tile = tile_of(n);
+        const bool is = (unsigned)block < (unsigned)a.kv.blocks;
+        const uint32_t at = is && tile < tile_end ? block : 0;
+        Tiles t;
+        t.none = is ? 0u : 0x7FC00000u;
+        t.present = tile < tile_end ? ~0u : 0u;
+        t.base = (uint64_t)at * block_bytes + (head_bytes + (tile & ((1 << (a.kv.page_shift - 4)) - 1)) * (kTile * DIM));
+        t.bits = scales[(size_t)at * block_scales];
+        return t;
+    };
+    const auto take_tile = [&](const Tiles& t) {
+        at_low = (uint32_t)t.base;
+        at_high = (uint32_t)(t.base >> 32);
+        at_k = (__float_as_uint(t.bits.x) | t.none) & t.present;
+        at_v = (__float_as_uint(t.bits.y) | t.none) & t.present;
+    };
+    // Before pair n's keys are looked for.
+    const auto go_on = [&](int n) {
+        if (n & 15 || n < 32 || n >= pairs) return;
+        if ((lane >> 5) == ((n >> 4) & 1)) take_tile(soon);
+        soon = find_tile(n + 16 + (lane >> 1 & 15), found);
+        found = find_block(n + 32 + (lane >> 1 & 15));
+    };
+    u4 raw_k[kDepth][2][DIM / 64], raw_v[kDepth][2][DIM / 64];
+    uint64_t base[2], base_v[2];  // of the newest pair; of the one before
+    int size, size_v;
+    const auto find_pair = [&](int n) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int from = 2 * (n & 31) + h;
+            base[h] = (uint32_t)__builtin_amdgcn_readlane(at_low, from) |
+                      (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_high, from) << 32;
+        }
+        size = n < pairs ? kTile * DIM : 0;
+    };
+    const auto load = [&](uint8_t* pool, const uint64_t (&at)[2], int bytes, u4 (&raw)[2][DIM / 64]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const auto tile = __builtin_amdgcn_make_buffer_rsrc(pool + at[h], 0, bytes, 0x27000);
+#pragma unroll
+            for (int j = 0; j < DIM / 64; ++j)
+                raw[h][j] = __builtin_amdgcn_raw_buffer_load_b128(tile, 16 * lane + 1024 * j, 0, 0);
+        }
+    };
+    const int first_block = find_block(lane >> 1);
+    // The queries' bytes: all loads before any use, and before those of keys
+    // and values, which wait for the table.
+    const bool f32 = DECODE ? a.type == MP_TYPE_F32 : MODE == kTwo;
+    u4 raw_q[NT][DIM / 64][4];  // 16 elements; the last two unused for 16-bit types
+    const auto raw_queries = [&](auto get) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < DIM / 64; ++j) get(raw_q[t][j], q_at[t] + 64 * j + 16 * g);
+    };
+    if (f32) {
+        const float* const from = static_cast<const float*>(a.q);
+        if (a.q_wide)
+            raw_queries([&](u4 (&to)[4], int64_t i) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to[k] = *reinterpret_cast<const u4*>(from + i + 4 * k);
+            });
+        else
+            raw_queries([&](u4 (&to)[4], int64_t i) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) to[k / 4][k % 4] = __float_as_uint(from[i + k]);
+            });
+    } else {
+        typedef u4 u4_by_8 __attribute__((aligned(8)));
+        const uint16_t* const from = static_cast<const uint16_t*>(a.q);
+        if (a.q_wide)
+            raw_queries([&](u4 (&to)[4], int64_t i) {
+                to[0] = *reinterpret_cast<const u4_by_8*>(from + i);
+                to[1] = *reinterpret_cast<const u4_by_8*>(from + i + 8);
+            });
+        else
+            raw_queries([&](u4 (&to)[4], int64_t i) {
+#pragma unroll
+                for (int k = 0; k < 16; k += 2)
+                    to[k / 8][k / 2 % 4] = from[i + k] | (uint32_t)from[i + k + 1] << 16;
+            });
+    }
+    {
+        const Tiles t = find_tile(lane >> 1, first_block);
+        at_low = (uint32_t)t.base;
+        at_high = (uint32_t)(t.base >> 32);
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+            find_pair(d);
+            load(a.kv.keys, base, size, raw_k[d]);
+            load(a.kv.values, base, size, raw_v[d]);
+        }
+        take_tile(t);
+    }
+    if (pairs > 32) {
+        soon = find_tile(32 + (lane >> 1 & 15), find_block(32 + (lane >> 1 & 15)));
+        found = find_block(48 + (lane >> 1 & 15));
     }
 
     // Queries: part, column tile, step (j, h): dims 64j + 16g + 8h .. +7.
@@ -244,62 +365,81 @@ __global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) 
         float x[DIM / 64][16];
         uint32_t amax = 0;
 #pragma unroll
-        for (int j = 0; j < DIM / 64; ++j) {
-            load_row<16>(a.q, a.type, a.q_wide, q_at[t] + 64 * j + 16 * g, x[j]);
+        for (int j = 0; j < DIM / 64; ++j)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) amax = max(amax, __float_as_uint(x[j][i]) & 0x7FFFFFFFu);
-        }
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t two = raw_q[t][j][i / 8][i / 2 % 4];
+                x[j][i] = f32                          ? __uint_as_float(raw_q[t][j][i / 4][i % 4])
+                          : a.type == MP_TYPE_BF16     ? __uint_as_float(i % 2 ? two & 0xFFFF0000u : two << 16)
+                                                       : from_f16(i % 2 ? two >> 16 : two & 0xFFFF);
+                amax = max(amax, __float_as_uint(x[j][i]) & 0x7FFFFFFFu);
+            }
         amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
         amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
         const int power = min(127 + 14 - (int)(amax >> 23), 126);  // at least -113
         const float up = __uint_as_float((uint32_t)(127 + power) << 23);
-        factor[t] = amax >= 0x7F800000u ? quiet_nan() : a.scale * __uint_as_float((uint32_t)(127 - power) << 23);
+        // NaN for a row that is not finite or whose pages the table has not.
+        const bool lost = amax >= 0x7F800000u || qpos[t] >> a.kv.page_shift >= a.rows.table_stride;
+        factor[t] = lost ? quiet_nan() : a.scale * __uint_as_float((uint32_t)(127 - power) << 23);
 #pragma unroll
         for (int j = 0; j < DIM / 64; ++j)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float v = x[j][i] * up;
-                const _Float16 high = (_Float16)v, low = (_Float16)(v - (float)high);
-                if (MODE == kPacked) q[0][t][2 * j + i / 8].one[i % 8] = c & 8 ? low : high;
-                else q[0][t][2 * j + i / 8].one[i % 8] = high;
-                if (MODE == kTwo) q[kParts - 1][t][2 * j + i / 8].one[i % 8] = low;
+            for (int i = 0; i < 16; i += 2) {
+                const float u = x[j][i] * up, v = x[j][i + 1] * up;
+                const h2 high = {(_Float16)u, (_Float16)v};
+                const h2 low = {(_Float16)(u - (float)high[0]), (_Float16)(v - (float)high[1])};
+                h2& first = q[0][t][2 * j + i / 8].two[i % 8 / 2];
+                if (MODE == kPacked) first = c & 8 ? low : high;
+                else first = high;
+                if (MODE == kTwo) q[kParts - 1][t][2 * j + i / 8].two[i % 8 / 2] = low;
             }
     }
 
-    f4 o[NT][kDims];
-    float ref[NT], sum[NT];  // reference less kShift, this lane's share of the sum
+    // o, and the sum of the probabilities as one more row of the product with
+    // the values (a matrix of ones), whose four registers are the same.
+    f4 o[NT][kDims], l[NT];
+    float ref[NT], limit[NT];  // reference less kShift; a score above the limit raises it
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        ref[t] = -infinity();
-        sum[t] = 0.0f;
+        ref[t] = 0.0f;
+        limit[t] = -infinity();  // the first score that is seen
+        l[t] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < kDims; ++n) o[t][n] = f4{0.f, 0.f, 0.f, 0.f};
     }
     uint32_t v_top = 0;  // bits of the value scale that o is held in
+    const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    const float part_factor = MODE == kPacked && !(c & 8) ? 0.0f : -1.0f;
 
-    for (; pair < pair_end; pair += waves) {
-        RawTile<DIM> now[2] = {next[0], next[1]};
-        if (pair + waves < pair_end) {
-            load_pair(pair + waves);
-            find_blocks(min(pair + 2 * waves, pair_end - 1));
-        }
-        f4 s[NT][2];
+    const auto scores = [&](const u4 (&raw)[2][DIM / 64], f4 (&to)[NT][2]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) s[t][h] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < NT; ++t) to[t][h] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 Half8 k;
-                Convert<FORMAT>::plain(now[h].k[i / 2][2 * (i % 2)], &k.two[0], &k.two[1]);
-                Convert<FORMAT>::plain(now[h].k[i / 2][2 * (i % 2) + 1], &k.two[2], &k.two[3]);
+                Convert<FORMAT>::plain(raw[h][i / 2][2 * (i % 2)], &k.two[0], &k.two[1]);
+                Convert<FORMAT>::plain(raw[h][i / 2][2 * (i % 2) + 1], &k.two[2], &k.two[3]);
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int part = 0; part < kParts; ++part)
 #pragma unroll
-                    for (int part = 0; part < kParts; ++part)
-                        s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.all, q[part][t][i].all, s[t][h], 0, 0, 0);
+                    for (int t = 0; t < NT; ++t)
+                        to[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.all, q[part][t][i].all, to[t][h], 0, 0, 0);
             }
         }
+    };
+    f4 s[NT][2];
+    scores(raw_k[0], s);
+    find_pair(kDepth);
+    load(a.kv.keys, base, size, raw_k[0]);
+
+    // `k_next`: the next pair's keys, `v`: this one's values.
+    const auto step = [&](int n, u4 (&k_next)[2][DIM / 64], u4 (&v)[2][DIM / 64]) {
+        const uint32_t k_bits[2] = {(uint32_t)__builtin_amdgcn_readlane(at_k, 2 * (n & 31)),
+                                    (uint32_t)__builtin_amdgcn_readlane(at_k, 2 * (n & 31) + 1)};
+        const uint32_t v_bits[2] = {(uint32_t)__builtin_amdgcn_readlane(at_v, 2 * (n & 31)),
+                                    (uint32_t)__builtin_amdgcn_readlane(at_v, 2 * (n & 31) + 1)};
         if (MODE == kPacked) {  // the low parts' scores are 8 columns on
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -308,47 +448,67 @@ __global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) 
                     s[0][h][i] += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
                         0, __float_as_int(s[0][h][i]), 0x128, 0xF, 0xF, true));
         }
-        const int token0 = pair * kKv8Pair;
-        const bool masked = token0 + kKv8Pair - 1 > (DECODE ? last : used + first / a.group);
-        const float k_scale[2] = {__uint_as_float(now[0].k_scale), __uint_as_float(now[1].k_scale)};
-        // Scores in powers of two less the reference; the reference is
-        // raised only where one is past kRaise.
+        const int token0 = (pair0 + n * waves) * kKv8Pair;
+        // Scores in powers of two less the reference.
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float f = factor[t] * __uint_as_float(k_bits[h]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][h][i] = __builtin_fmaf(s[t][h][i], f, -ref[t]);
+            }
+        if (token0 + kKv8Pair - 1 > (DECODE ? last : used + first / a.group)) {  // past some row's position
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (token0 + kTile * h + 4 * g + i > qpos[t]) s[t][h][i] = -infinity();
+            // Slots past the last row's position may hold anything: as bytes
+            // they are made 0 where an E4M3 NaN could be (INT8 codes are
+            // finite, and their probability is 0).
+            if (FORMAT == MP_KV8_E4M3 && token0 + kKv8Pair - 1 > last) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int left = last + 1 - token0 - kTile * h - 4 * g;
+                    const uint32_t keep = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+#pragma unroll
+                    for (int j = 0; j < DIM / 64; ++j) v[h][j] &= keep;
+                }
+            }
+        }
+        // The reference is raised only where a score is past the limit.
         bool need = false;
+        float top[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            float f[2] = {factor[t] * k_scale[0], factor[t] * k_scale[1]};
-            float top = -infinity();
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[t][h][i] *= f[h];
-                    if (masked && token0 + kTile * h + 4 * g + i > qpos[t]) s[t][h][i] = -infinity();
-                    top = fmaxf(top, s[t][h][i]);
-                }
-            need |= top > ref[t] + kRaise;
+            top[t] = max3(max3(s[t][0][0], s[t][0][1], s[t][0][2]), max3(s[t][0][3], s[t][1][0], s[t][1][1]),
+                          fmaxf(s[t][1][2], s[t][1][3]));
+            need |= top[t] > limit[t];
         }
         if (__builtin_amdgcn_ballot_w64(need)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float top = -infinity();
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][h][i]);
-                top = column_max(top);
-                if (top > ref[t] + kRaise) {
-                    const float to = top - kShift;
-                    const float keep = __builtin_amdgcn_exp2f(ref[t] - to);  // 0 from -inf
-                    ref[t] = to;
-                    sum[t] *= keep;
+                const float most = column_max(top[t]);
+                if (most > limit[t]) {
+                    const float by = most - kShift;
+                    const float keep = limit[t] == -infinity() ? 0.0f : __builtin_amdgcn_exp2f(-by);
+                    ref[t] += by;
+                    limit[t] = kRaise;
+                    l[t] *= keep;
 #pragma unroll
                     for (int n = 0; n < kDims; ++n) o[t][n] *= keep;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[t][h][i] -= by;
                 }
             }
         }
         // The value scale: o is held in the largest met so far.
-        const uint32_t v_now = max(now[0].v_scale, now[1].v_scale);
+        const uint32_t v_now = max(v_bits[0], v_bits[1]);
         if (v_now > v_top) {
             if (v_top) {
                 const float keep = __uint_as_float(v_top) / __uint_as_float(v_now);
@@ -359,62 +519,72 @@ __global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) 
             }
             v_top = v_now;
         }
+        // Powers of two of the tiles' values; 2^-40 of the top one is nothing.
+        const auto power = [&](uint32_t bits) {
+            return __uint_as_float((uint32_t)max((int)(bits - v_top) + (127 << 23), (127 - 40) << 23));
+        };
+        const Convert<FORMAT> convert0(power(v_bits[0])), convert1(power(v_bits[1]));
+        base_v[0] = base[0], base_v[1] = base[1], size_v = size;
+        find_pair(n + kDepth + 1);
+        f4 s_next[NT][2];
+        scores(k_next, s_next);
+        load(a.kv.keys, base, size, k_next);
         Half8 p[kParts][NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const float base = ref[t] == -infinity() ? 0.0f : ref[t];
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(s[t][h][i] - base);
-                    sum[t] += e;
-                    const _Float16 high = (_Float16)e;
-                    const _Float16 low = (_Float16)(e - (float)high);
-                    if (MODE == kPacked) p[0][t].one[4 * h + i] = c & 8 ? low : high;
-                    else p[0][t].one[4 * h + i] = high;
-                    if (MODE == kTwo) p[kParts - 1][t].one[4 * h + i] = low;
+                for (int i = 0; i < 4; i += 2) {
+                    const float x = __builtin_amdgcn_exp2f(s[t][h][i]), y = __builtin_amdgcn_exp2f(s[t][h][i + 1]);
+                    const h2 high = {(_Float16)x, (_Float16)y};
+                    if (MODE != kPacked) p[0][t].two[2 * h + i / 2] = high;
+                    if (MODE != kOne)
+                        p[kParts - 1][t].two[2 * h + i / 2] =
+                            h2{(_Float16)mix_low(high, part_factor, x), (_Float16)mix_high(high, part_factor, y)};
                 }
-        }
-        // Powers of two of the tiles' values; 2^-40 of the top one is nothing.
-        const auto power = [&](uint32_t v) {
-            return __uint_as_float((uint32_t)max((int)(v - v_top) + (127 << 23), (127 - 40) << 23));
-        };
-        const Convert<FORMAT> convert0(power(now[0].v_scale)), convert1(power(now[1].v_scale));
-        // Slots past the last row's position may hold anything: as bytes they
-        // are made 0 where an E4M3 NaN could be (INT8 codes are finite, and
-        // their probability is 0).
-        uint32_t keep0 = ~0u, keep1 = ~0u;
-        if (FORMAT == MP_KV8_E4M3 && token0 + kKv8Pair - 1 > last) {
-            const int left0 = last + 1 - token0 - 4 * g, left1 = left0 - kTile;
-            keep0 = left0 >= 4 ? ~0u : left0 <= 0 ? 0u : (1u << (8 * left0)) - 1;
-            keep1 = left1 >= 4 ? ~0u : left1 <= 0 ? 0u : (1u << (8 * left1)) - 1;
-        }
 #pragma unroll
-        for (int n = 0; n < kDims; ++n) {
-            Half8 v;
-            convert0(now[0].v[n / 4][n % 4] & keep0, &v.two[0], &v.two[1]);
-            convert1(now[1].v[n / 4][n % 4] & keep1, &v.two[2], &v.two[3]);
+        for (int part = 0; part < kParts; ++part)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
+                l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[part][t].all, l[t], 0, 0, 0);
 #pragma unroll
-                for (int part = 0; part < kParts; ++part)
-                    o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.all, p[part][t].all, o[t][n], 0, 0, 0);
+        for (int n = 0; n < kDims; ++n) {
+            Half8 w;
+            convert0(v[0][n / 4][n % 4], &w.two[0], &w.two[1]);
+            convert1(v[1][n / 4][n % 4], &w.two[2], &w.two[3]);
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.all, p[part][t].all, o[t][n], 0, 0, 0);
+        }
+        load(a.kv.values, base_v, size_v, v);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][0] = s_next[t][0], s[t][1] = s_next[t][1];
+    };
+    for (int n = 0; n < pairs;) {
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+            go_on(n + kDepth + 1);
+            step(n, raw_k[(d + 1) % kDepth], raw_v[d]);
+            if (++n >= pairs && d + 1 < kDepth) break;
         }
     }
 
-    // Each wavefront's result as values: o / sum in the value scale.
-    float weight[NT];
+    // Each wavefront's reference and sum (-inf and 0 where it saw nothing).
+    float sum[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        sum[t] = column_sum(sum[t]);
+        sum[t] = l[t][0];
+        if (limit[t] == -infinity() && sum[t] == sum[t]) ref[t] = -infinity();
         if (MODE == kPacked) {
+            sum[t] += __shfl_xor(sum[t], 8);
 #pragma unroll
             for (int n = 0; n < kDims; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[t][n][i] += __shfl_xor(o[t][n][i], 8);
         }
-        weight[t] = sum[t] == 0.0f ? 0.0f : __uint_as_float(v_top) / sum[t];
     }
     float best[NT], total[NT];
     if (waves > 1) {
@@ -423,13 +593,14 @@ __global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) 
             if (g == 0) ml_s[wave][t][c] = make_float2(ref[t], sum[t]);
         __syncthreads();
     }
-    // Reference and sum over the wavefronts, and this one's share.
-    float share[NT];
+    // Reference and sum over the wavefronts; what turns this one's o into its
+    // share of the result, as values.
+    float weight[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         best[t] = ref[t];
         total[t] = sum[t];
-        share[t] = sum[t];
+        float scaled = 1.0f;
         if (waves > 1) {
             best[t] = -infinity();
             for (int w = 0; w < waves; ++w) best[t] = fmaxf(best[t], ml_s[w][t][c].x);
@@ -438,9 +609,9 @@ __global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) 
                 const float2 ml = ml_s[w][t][c];
                 if (ml.y != 0.0f) total[t] += ml.y * __builtin_amdgcn_exp2f(ml.x - best[t]);
             }
-            share[t] = sum[t] == 0.0f ? 0.0f : sum[t] * __builtin_amdgcn_exp2f(ref[t] - best[t]);
+            scaled = __builtin_amdgcn_exp2f(ref[t] - best[t]);
         }
-        weight[t] = share[t] == 0.0f ? 0.0f : weight[t] * (share[t] / total[t]);
+        weight[t] = sum[t] == 0.0f ? 0.0f : scaled / total[t] * __uint_as_float(v_top);
     }
     const auto store = [&](int t, int n, f4 x) {
         const int column = first + 16 * t + c;
@@ -464,28 +635,41 @@ __global__ __launch_bounds__(512, 2) void kv8_attention_kernel(AttentionArgs a) 
             for (int n = 0; n < kDims; ++n) store(t, n, o[t][n] * weight[t]);
         return;
     }
+    // The shares meet in LDS, `kAt` tiles of 16 dims at a time, the fewer the
+    // more wavefronts there are; output tiles are dealt to the wavefronts.
+    const auto join = [&](auto at_a_time) {
+        constexpr int kAt = decltype(at_a_time)::value;
 #pragma unroll
-    for (int n = 0; n < kDims; ++n) {
+        for (int n0 = 0; n0 < kDims; n0 += kAt) {
+            if (n0) __syncthreads();
 #pragma unroll
-        for (int t = 0; t < NT; ++t) o_s[wave][t][lane] = o[t][n] * weight[t];
-        __syncthreads();
-        for (int t = wave; t < NT; t += waves) {
-            f4 x = o_s[0][t][lane];
-            for (int w = 1; w < waves; ++w) x += o_s[w][t][lane];
+            for (int n = 0; n < kAt; ++n)
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
-                if (u == t) store(u, n, x);
+                for (int t = 0; t < NT; ++t) o_s[(wave * kAt + n) * NT + t][lane] = o[t][n0 + n] * weight[t];
+            __syncthreads();
+            for (int i = wave; i < kAt * NT; i += waves) {
+                f4 x = o_s[i][lane];
+                for (int w = 1; w < waves; ++w) x += o_s[w * kAt * NT + i][lane];
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+                    if (u == i % NT) store(u, n0 + i / NT, x);
+            }
         }
-        __syncthreads();
-    }
+    };
+    __syncthreads();  // the references and sums lie where the shares will
+    if (waves <= 4) join(std::integral_constant<int, join_dims(4, NT, kDims)>());
+    else join(std::integral_constant<int, join_dims(kKv8MostWaves, NT, kDims)>());
 }
 
-// Joins the chunks of rows that have several: one wavefront a (row, head),
-// lanes over dims. `columns_tile`: columns of an attention work-group.
-template <bool DECODE>
+// Joins the chunks of rows that have several: WAVES wavefronts a (row, head),
+// four (row, head) or one a work-group. `columns_tile`: columns of an
+// attention work-group.
+template <bool DECODE, int WAVES>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(AttentionArgs a, int columns_tile) {
+    __shared__ f4 out_s[WAVES][64];
     const int lane = threadIdx.x & 63, dim = a.kv.dim;
-    const int index = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int in_group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int index = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + in_group, wave = WAVES > 1 ? in_group : 0;
     const int head = index % a.heads;
     int row = index / a.heads, last;
     if (row >= a.rows.rows) return;
@@ -504,31 +688,42 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(AttentionArgs a, int col
     if (last < a.chunk || last >= a.max_length) return;
     const int chunks = last / a.chunk + 1;
     const size_t at = ((size_t)row * a.heads + head) * a.splits;
+    // Every wavefront finds the reference and the weights' sum, and joins its
+    // share of the chunks: dim/4 lanes a chunk.
     float best = -infinity();
     for (int b = lane; b < chunks; b += 64) best = fmaxf(best, a.partial_ml[at + b].x);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) best = fmaxf(best, __shfl_xor(best, d));
-    float total = 0.0f, out[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int b = 0; b < chunks; b += 64) {
-        float w = 0.0f;
-        if (b + lane < chunks) {
-            const float2 ml = a.partial_ml[at + b + lane];
-            if (ml.y != 0.0f) w = ml.y * __builtin_amdgcn_exp2f(ml.x - best);
-        }
-        const int n = min(64, chunks - b);
-        for (int i = 0; i < n; ++i) {
-            const float wi = __shfl(w, i);
-            total += wi;
-            const float* part = a.partial_out + (at + b + i) * dim + lane;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (64 * k < dim) out[k] += wi * part[64 * k];
-        }
+    float total = 0.0f;
+    for (int b = lane; b < chunks; b += 64) {
+        const float2 ml = a.partial_ml[at + b];
+        if (ml.y != 0.0f) total += ml.y * __builtin_amdgcn_exp2f(ml.x - best);
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (64 * k < dim)
-            store_one(a.out, a.type, row * a.out_stride + (int64_t)head * dim + 64 * k + lane, out[k] / total);
+    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+    const int lanes = dim / 4, each = 64 / lanes, d4 = lane % lanes;
+    f4 out = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int b = wave * each + lane / lanes; b < chunks; b += WAVES * each) {
+        const float2 ml = a.partial_ml[at + b];
+        const float w = ml.y != 0.0f ? ml.y * __builtin_amdgcn_exp2f(ml.x - best) / total : 0.0f;
+        const float2* const part = reinterpret_cast<const float2*>(a.partial_out + (at + b) * dim + 4 * d4);
+        const float2 x = part[0], y = part[1];
+        out += f4{x.x, x.y, y.x, y.y} * w;
+    }
+    for (int d = lanes; d < 64; d *= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] += __shfl_xor(out[i], d);
+    if (WAVES > 1) {
+        out_s[wave][lane] = out;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) out += out_s[w][lane];
+    }
+    if (lane < lanes)
+        store_four(a.out, a.type, a.out_wide, row * a.out_stride + (int64_t)head * dim + 4 * d4, out[0], out[1], out[2],
+                   out[3]);
 }
 
 // Column tiles that a prefill wavefront holds in its registers.
@@ -539,7 +734,8 @@ constexpr int most_tiles(int dim, int mode) {
 template <int FORMAT, int DIM, int NT, int MODE, bool DECODE>
 void launch(hipStream_t s, const Kv8Plan& p, int64_t items, const AttentionArgs& a) {
     const dim3 grid((unsigned)items, (unsigned)a.kv.kv_heads, (unsigned)p.splits);
-    kv8_attention_kernel<FORMAT, DIM, NT, MODE, DECODE><<<grid, 64 * p.waves, 0, s>>>(a);
+    const size_t shared = join_bytes(p.waves, NT, DIM / 16);
+    kv8_attention_kernel<FORMAT, DIM, NT, MODE, DECODE><<<grid, 64 * p.waves, shared, s>>>(a);
 }
 template <int FORMAT, int DIM>
 void launch_decode(hipStream_t s, const Kv8Plan& p, const AttentionArgs& a) {
@@ -620,9 +816,17 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
     else launch_format<MP_KV8_E4M3>(s, p, a, decode);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && p.splits > 1) {
-        const unsigned groups = (unsigned)(((int64_t)rows * heads + 3) / 4);
-        if (decode) kv8_merge_kernel<true><<<groups, 256, 0, s>>>(a, 16);
-        else kv8_merge_kernel<false><<<groups, 256, 0, s>>>(a, 16 * p.column_tiles);
+        const int64_t outputs = (int64_t)rows * heads;
+        const int columns = 16 * p.column_tiles;
+        if (p.splits > 8) {
+            const unsigned groups = (unsigned)outputs;
+            if (decode) kv8_merge_kernel<true, 4><<<groups, 256, 0, s>>>(a, columns);
+            else kv8_merge_kernel<false, 4><<<groups, 256, 0, s>>>(a, columns);
+        } else {
+            const unsigned groups = (unsigned)((outputs + 3) / 4);
+            if (decode) kv8_merge_kernel<true, 1><<<groups, 256, 0, s>>>(a, columns);
+            else kv8_merge_kernel<false, 1><<<groups, 256, 0, s>>>(a, columns);
+        }
         e = hipGetLastError();
     }
     return kv8_done(e, "8-bit attention launch");

@@ -58,8 +58,10 @@ struct Kv8Plan {
 };
 
 constexpr int kKv8Pair = 32;          // tokens of two tiles, a step of a wavefront
-constexpr int kKv8Groups = 1024;      // work-groups that splitting over tokens aims at
+constexpr int kKv8Groups = 512;       // work-groups that splitting over tokens aims at
 constexpr int kKv8LeastChunk = 128;   // tokens
+
+constexpr int kKv8MostWaves = 8;  // of a work-group
 
 constexpr int64_t kv8_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -74,9 +76,12 @@ inline void kv8_split(Kv8Plan* p, int64_t items, int max_length) {
     p->splits = (int)kv8_ceil(length, chunk);
 }
 
+// Up to 4,096 tokens a row's work-group is left alone with it: a second launch
+// to join chunks costs 3 to 4 us.
 inline Kv8Plan kv8_decode_plan(int rows, int kv_heads, int max_length) {
-    Kv8Plan p{1, 4, 0, 0};
-    kv8_split(&p, (int64_t)rows * kv_heads, max_length);
+    Kv8Plan p{1, max_length > 1024 && max_length <= 4096 ? 8 : 4, 0, 0};
+    if (max_length <= 4096) kv8_split(&p, kKv8Groups, max_length);
+    else kv8_split(&p, (int64_t)rows * kv_heads, max_length);
     return p;
 }
 
@@ -88,9 +93,11 @@ inline int64_t kv8_items(int rows, int sequences, int group, int column_tiles) {
 
 // most_tiles: the column tiles a wavefront's registers hold.
 inline Kv8Plan kv8_prefill_plan(int rows, int sequences, int kv_heads, int group, int most_tiles, int max_length) {
-    Kv8Plan p{most_tiles, 8, 0, 0};
-    while (p.column_tiles > 1 && kv8_items(rows, sequences, group, p.column_tiles) * kv_heads < 512) p.column_tiles /= 2;
-    kv8_split(&p, kv8_items(rows, sequences, group, p.column_tiles) * kv_heads, max_length);
+    Kv8Plan p{1, 8, 0, 0};
+    const int64_t items = kv8_items(rows, sequences, group, 1) * kv_heads;
+    if (items >= 1024) p = Kv8Plan{most_tiles < 2 ? most_tiles : 2, max_length > 2048 ? 4 : 1, 0, 0};
+    if (max_length <= 4096) kv8_split(&p, kKv8Groups, max_length);
+    else kv8_split(&p, kv8_items(rows, sequences, group, p.column_tiles) * kv_heads, max_length);
     return p;
 }
 
