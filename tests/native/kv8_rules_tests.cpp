@@ -92,17 +92,18 @@ void plans() {
     for (int trial = 0; trial < 100000; ++trial) {
         const int group = 1 + (int)(rng() % 16), kv_heads = upto(64), dim = 64 << rng() % 3;
         const int rows = upto(1 << 20), sequences = upto(rows), length = (int)(rng() % 8) ? upto(1 << 22) : 0;
-        const int most = 1 << rng() % 3, heads = group * kv_heads;
+        const int heads = group * kv_heads;
         const Kv8Plan d = kv8_decode_plan(rows, kv_heads, length);
-        const Kv8Plan f = kv8_prefill_plan(rows, sequences, kv_heads, group, most, length);
+        const Kv8Plan f = kv8_prefill_plan(rows, sequences, kv_heads, group, dim, length);
         for (const Kv8Plan& p : {d, f}) {
-            REQUIRE(p.column_tiles >= 1 && p.column_tiles <= 4 && (p.column_tiles & (p.column_tiles - 1)) == 0);
+            REQUIRE(p.column_tiles == 1 || (p.column_tiles == 2 && dim <= 128));
             REQUIRE(p.waves >= 1 && p.waves <= 8 && p.splits >= 1 && p.splits <= 65535);
             REQUIRE(p.chunk % kKv8Pair == 0 && (int64_t)p.chunk * p.splits >= length);
         }
-        REQUIRE(f.column_tiles <= most);
+        REQUIRE(d.column_tiles == 1);
         const int64_t items = kv8_items(rows, sequences, group, f.column_tiles);
-        REQUIRE(items * 64 * f.waves < 1ll << 32 && (int64_t)rows * 64 * d.waves < 1ll << 32);
+        if ((int64_t)rows * heads <= kKv8MostColumns)
+            REQUIRE(items * kv_heads * 64 * f.waves < 1ll << 32 && (int64_t)rows * kv_heads * 64 * d.waves < 1ll << 32);
         // Smaller calls on the same workspace.
         const size_t space = kv8_workspace_floats(rows, sequences, heads, kv_heads, dim, length);
         const int fewer = 1 + (int)(rng() % rows), shorter = length ? (int)(rng() % (length + 1)) : 0;
@@ -110,7 +111,7 @@ void plans() {
         for (int r : {rows, fewer})
             for (int n : {length, shorter}) {
                 REQUIRE(kv8_partial_floats(kv8_decode_plan(r, kv_heads, n), r, heads, dim) <= space);
-                REQUIRE(kv8_partial_floats(kv8_prefill_plan(r, some, kv_heads, group, most, n), r, heads, dim) <= space);
+                REQUIRE(kv8_partial_floats(kv8_prefill_plan(r, some, kv_heads, group, dim, n), r, heads, dim) <= space);
             }
     }
 }

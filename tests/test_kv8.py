@@ -91,6 +91,13 @@ APPENDS = [
     (1, 4, 128, 128, 128, False, F32, 0, 0),
     (1, 3, 256, 32, 32, True, F16, 12, 0),
     (2, 4, 256, 16, 0, False, F32, 0, 0),
+    # queries by 16 bytes: every arrangement of turning and passing dims
+    (2, 32, 128, 64, 64, True, BF16, 0, 0),
+    (1, 7, 128, 16, 128, False, F16, 8, 0),
+    (3, 9, 64, 32, 16, False, BF16, 0, 0),
+    (1, 3, 64, 16, 24, True, F32, 0, 0),
+    (1, 5, 256, 16, 256, False, F32, 4, 0),
+    (1, 1, 64, 16, 0, False, F16, 0, 0),
 ]
 
 
@@ -423,14 +430,15 @@ def test_prefill_of_many_rows(torch_cuda):
         device = Device(torch_cuda, cache)
         starts = starts_of(counts)
         q = rounded(rng.standard_normal((int(starts[-1]), heads, dim)) * 0.02, kind)
-        got = run_prefill(device, 0, q, kind, tables, starts, used, max(lengths), 1 / dim ** 0.5)
-        assert np.isfinite(got).all()
-        for s in (0, 1, 2, 33, 63, 64, 65, 69):
-            v_max = np.abs(cache.tokens(0, 1, tables[s], lengths[s])).max()
-            for i in (0, 1, counts[s] // 2, counts[s] - 1):
-                r = starts[s] + i
-                want, err = cache.attention(0, q[r], tables[s], used[s] + i + 1, 1 / dim ** 0.5)
-                check_row(got[r], want, err, kind, v_max, True, f"dim {dim}, sequence {s}, row {i}")
+        for longest in (max(lengths), 20000):
+            got = run_prefill(device, 0, q, kind, tables, starts, used, longest, 1 / dim ** 0.5)
+            assert np.isfinite(got).all()
+            for s in (0, 1, 2, 33, 63, 64, 65, 69):
+                v_max = np.abs(cache.tokens(0, 1, tables[s], lengths[s])).max()
+                for i in (0, 1, counts[s] // 2, counts[s] - 1):
+                    r = starts[s] + i
+                    want, err = cache.attention(0, q[r], tables[s], used[s] + i + 1, 1 / dim ** 0.5)
+                    check_row(got[r], want, err, kind, v_max, True, f"dim {dim}, sequence {s}, row {i} of {longest}")
 
 
 @FORMATS

@@ -13,6 +13,8 @@
 // function of the inputs alone): a' = a cos - b sin, b' = b cos + a sin; code =
 // rint(x * (1/s)), exact but for the rint since s is a power of two; E4M3
 // codes by v_cvt_pk_fp8_f32 (nearest even).
+#include <type_traits>
+
 #include "kernels.h"
 #include "kv8.h"
 
@@ -38,7 +40,8 @@ struct AppendArgs {
     void* q_out;
     int64_t q_stride, q_out_stride;
     int heads, type, format;
-    bool wide[2], q_wide;
+    bool wide[2];
+    bool q_by_16;  // rows, strides and the turning dims are whole 16 bytes
     int kv_groups;  // work-groups before those of the queries
 };
 
@@ -148,7 +151,7 @@ struct Unit {
     int item, head, kind, tile, first_wave, tiles;
 };
 __device__ __forceinline__ Unit unit_of(const Kv8Layer& kv) {
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Unit u;
     u.tiles = 1 << (kv.page_shift - 4);
     const int unit = blockIdx.x * ((blockDim.x >> 6) / u.tiles) + wave / u.tiles;
@@ -160,16 +163,15 @@ __device__ __forceinline__ Unit unit_of(const Kv8Layer& kv) {
     return u;
 }
 
+// `t`: the wavefront's tile of unit `u`.
 template <int DIM>
-__device__ __forceinline__ void append_unit(const AppendArgs& a, uint32_t* amax_s) {
+__device__ __forceinline__ void append_unit(const AppendArgs& a, const Unit& u, const Tile& t, uint32_t* amax_s) {
     constexpr int kLoads = DIM / 64;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const Unit u = unit_of(a.kv);
-    Tile t = find_tile(a.kv, a.rows, u.item, u.tile);
-    if (a.rope.half) t.last = min(t.last, a.rope.positions - t.pos0);
-    const void* const src = u.kind ? a.x[1] : a.x[0];
-    const int64_t stride = u.kind ? a.x_stride[1] : a.x_stride[0];
-    const bool wide = u.kind ? a.wide[1] : a.wide[0];
+    const int head = u.head, kind = u.kind;
+    const void* const src = kind ? a.x[1] : a.x[0];
+    const int64_t stride = kind ? a.x_stride[1] : a.x_stride[0];
+    const bool wide = kind ? a.wide[1] : a.wide[0];
     float x[kLoads][16];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
@@ -179,11 +181,11 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, uint32_t* amax_
     float held = 0.0f;
     size_t index = 0;
     if (t.block >= 0) {
-        index = kv8_head(a.kv, t.block, u.head);
-        if (t.kept) held = reinterpret_cast<const float*>(a.kv.scales + index)[u.kind];
-        if (u.kind == 0) {
+        index = kv8_head(a.kv, t.block, head);
+        if (t.kept) held = reinterpret_cast<const float*>(a.kv.scales + index)[kind];
+        if (kind == 0) {
             if (c >= t.first && c < t.last) {
-                const int64_t at = (t.row0 + c - t.first) * stride + (int64_t)u.head * DIM;
+                const int64_t at = (t.row0 + c - t.first) * stride + (int64_t)head * DIM;
 #pragma unroll
                 for (int j = 0; j < kLoads; ++j)
                     load_rotated(src, a.type, wide, at, 64 * j + 16 * g, t.pos0 + c, a.rope, x[j]);
@@ -193,7 +195,7 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, uint32_t* amax_
             for (int i = 0; i < 4; ++i) {
                 const int slot = 4 * g + i;
                 if (slot < t.first || slot >= t.last) continue;
-                const int64_t at = (t.row0 + slot - t.first) * stride + (int64_t)u.head * DIM + c;
+                const int64_t at = (t.row0 + slot - t.first) * stride + (int64_t)head * DIM + c;
 #pragma unroll
                 for (int j = 0; j < kLoads; ++j)
 #pragma unroll
@@ -217,15 +219,15 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, uint32_t* amax_
     const float scale = held >= wanted || held != held ? held : wanted;
     const bool grew = t.kept && scale != held && scale == scale;  // kept codes move
     const float inverse = 1.0f / scale, ratio = held * inverse;
-    uint8_t* const bytes = (u.kind ? a.kv.values : a.kv.keys) + index * ((size_t)DIM << a.kv.page_shift) +
+    uint8_t* const bytes = (kind ? a.kv.values : a.kv.keys) + index * ((size_t)DIM << a.kv.page_shift) +
                            u.tile * kTile * DIM + 16 * lane;
-    if (u.tile == 0 && lane == 0) reinterpret_cast<float*>(a.kv.scales + index)[u.kind] = scale;
+    if (u.tile == 0 && lane == 0) reinterpret_cast<float*>(a.kv.scales + index)[kind] = scale;
     if (!grew && (t.first >= kTile || t.last <= 0)) return;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
         uint4* const at = reinterpret_cast<uint4*>(bytes + 1024 * j);
         uint32_t w[4];
-        if (u.kind == 0) {
+        if (kind == 0) {
             const bool fresh = c >= t.first && c < t.last;
             if (!fresh && !(grew && c < t.first)) continue;
             if (!fresh) {
@@ -267,74 +269,151 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, uint32_t* amax_
     }
 }
 
-// Row `row`'s queries, rotated, by one wavefront.
-__device__ __forceinline__ void rotate_row(const AppendArgs& a, int row) {
-    const int lane = threadIdx.x & 63, dim = a.kv.dim, half = a.rope.half, turned = 2 * half;
-    // The row's sequence: rows as items, behind those before starts[0].
-    Kv8Item at;
-    if (row >= a.rows.rows || !kv8_find(a.rows, row, [](int count, int) { return count; }, &at)) return;
-    const int64_t r = at.row0 + at.index;
-    const int64_t pos = (int64_t)at.used + at.index;
-    const int64_t from = r * a.q_stride, to = r * a.q_out_stride;
-    const bool bad = half && (at.used < 0 || pos >= a.rope.positions);
-    const float* const cos = a.rope.cos + (bad ? 0 : pos) * half;
-    const float* const sin = a.rope.sin + (bad ? 0 : pos) * half;
-    const float poison = bad ? quiet_nan() : 0.0f;
-    const int step = a.q_wide && half % 4 == 0 ? 4 : 1;
-    // Per head: the pairs, `step` of them at a time (interleaved: two steps'
-    // worth of elements), then the dims that pass.
-    const int pairs = half / step, rest = (dim - turned) / step, per_head = pairs + rest;
-    for (int i = lane; i < a.heads * per_head; i += 64) {
-        const int head = i / per_head, p = i % per_head;
-        const int64_t src = from + (int64_t)head * dim, dst = to + (int64_t)head * dim;
-        if (p >= pairs) {
-            const int d = turned + (p - pairs) * step;
-            if (step == 4) {
-                float x[4];
-                load_row<4>(a.q, a.type, true, src + d, x);
-                store_four(a.q_out, a.type, true, dst + d, bad ? poison : x[0], bad ? poison : x[1],
-                           bad ? poison : x[2], bad ? poison : x[3]);
-            } else {
-                const float x = load_one(a.q, a.type, src + d);
-                store_one(a.q_out, a.type, dst + d, bad ? poison : x);
-            }
-            continue;
-        }
-        const int k = p * step;  // first pair
-        const int d0 = a.rope.interleaved ? 2 * k : k, d1 = a.rope.interleaved ? 2 * k + step : k + half;
-        if (step == 4) {
-            float u[4], v[4], lo[4], hi[4];
-            load_row<4>(a.q, a.type, true, src + d0, u);
-            load_row<4>(a.q, a.type, true, src + d1, v);
+// 16 bytes as E elements (4 FP32, 8 of a 16-bit type), and back.
+template <int E>
+__device__ __forceinline__ void unpack(uint4 v, int type, float (&x)[E]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float c = bad ? poison : cos[k + e], s = bad ? poison : sin[k + e];
-                const float x = a.rope.interleaved ? (e < 2 ? u[2 * (e & 1)] : v[2 * (e & 1)]) : u[e];
-                const float y = a.rope.interleaved ? (e < 2 ? u[2 * (e & 1) + 1] : v[2 * (e & 1) + 1]) : v[e];
-                lo[e] = x * c - y * s;
-                hi[e] = y * c + x * s;
-            }
-            if (a.rope.interleaved) {
-                store_four(a.q_out, a.type, true, dst + d0, lo[0], hi[0], lo[1], hi[1]);
-                store_four(a.q_out, a.type, true, dst + d1, lo[2], hi[2], lo[3], hi[3]);
-            } else {
-                store_four(a.q_out, a.type, true, dst + d0, lo[0], lo[1], lo[2], lo[3]);
-                store_four(a.q_out, a.type, true, dst + d1, hi[0], hi[1], hi[2], hi[3]);
-            }
+    for (int i = 0; i < E; ++i) {
+        const uint32_t two = w[i * 4 / E];
+        if (E == 4) x[i] = __uint_as_float(two);
+        else if (type == MP_TYPE_BF16) x[i] = __uint_as_float(i % 2 ? two & 0xFFFF0000u : two << 16);
+        else x[i] = from_f16(i % 2 ? two >> 16 : two & 0xFFFF);
+    }
+}
+template <int E>
+__device__ __forceinline__ uint4 pack(const float (&x)[E], int type) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (E == 4) {
+            w[i] = __float_as_uint(x[i]);
         } else {
-            const float c = bad ? poison : cos[k], s = bad ? poison : sin[k];
-            const float x = load_one(a.q, a.type, src + d0), y = load_one(a.q, a.type, src + d1);
-            store_one(a.q_out, a.type, dst + d0, x * c - y * s);
-            store_one(a.q_out, a.type, dst + d1, y * c + x * s);
+            const float lo = x[2 * i % E], hi = x[(2 * i + 1) % E];
+            w[i] = type == MP_TYPE_BF16 ? to_bf16(lo) | (uint32_t)to_bf16(hi) << 16
+                                        : to_f16(lo) | (uint32_t)to_f16(hi) << 16;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A row's queries by 16 bytes. A lane has one place in every head it sees:
+// E pairs (i, i + half), or E elements of adjacent pairs, or E dims that pass.
+// It reads its cosines and sines once, and four heads at a time.
+template <int E>
+__device__ __forceinline__ void rotate_wide(const AppendArgs& a, int64_t row, int64_t pos, bool bad) {
+    const int lane = threadIdx.x & 63, dim = a.kv.dim, half = a.rope.half;
+    const bool pairs_apart = !a.rope.interleaved;
+    const int turning = pairs_apart ? half / E : 2 * half / E, places = turning + (dim - 2 * half) / E;
+    const int lanes = places <= 8 ? 8 : places <= 16 ? 16 : places <= 32 ? 32 : 64;  // dim / E is at most 64
+    const int place = lane % lanes, step = 64 / lanes;
+    if (place >= places) return;
+    const bool turns = place < turning, two = turns && pairs_apart;
+    const int d0 = turns || !pairs_apart ? place * E : 2 * half + (place - turning) * E, d1 = two ? d0 + half : d0;
+    const int64_t size = E == 4 ? 4 : 2;
+    const char* const from = static_cast<const char*>(a.q) + row * a.q_stride * size;
+    char* const to = static_cast<char*>(a.q_out) + row * a.q_out_stride * size;
+    // Cosine and sine of the lane's pairs; a row without any is NaN, turned or not.
+    float cos[E], sin[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int pair = two ? d0 + i : (d0 + i) / 2;
+        cos[i] = turns && !bad ? a.rope.cos[pos * half + pair] : bad ? quiet_nan() : 1.0f;
+        sin[i] = turns && !bad ? a.rope.sin[pos * half + pair] : 0.0f;
+    }
+    for (int h0 = lane / lanes; h0 < a.heads; h0 += 4 * step) {
+        uint4 u[4], v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int h = h0 + k * step;
+            if (h < a.heads) {
+                u[k] = *reinterpret_cast<const uint4*>(from + ((int64_t)h * dim + d0) * size);
+                if (two) v[k] = *reinterpret_cast<const uint4*>(from + ((int64_t)h * dim + d1) * size);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int h = h0 + k * step;
+            if (h >= a.heads) continue;
+            float x[E], y[E], lo[E], hi[E];
+            unpack<E>(u[k], a.type, x);
+            if (two) {
+                unpack<E>(v[k], a.type, y);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    lo[i] = x[i] * cos[i] - y[i] * sin[i];
+                    hi[i] = y[i] * cos[i] + x[i] * sin[i];
+                }
+                *reinterpret_cast<uint4*>(to + ((int64_t)h * dim + d1) * size) = pack<E>(hi, a.type);
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; i += 2) {
+                    lo[i] = turns ? x[i] * cos[i] - x[i + 1] * sin[i] : bad ? cos[i] : x[i];
+                    lo[i + 1] = turns ? x[i + 1] * cos[i] + x[i] * sin[i] : bad ? cos[i] : x[i + 1];
+                }
+            }
+            *reinterpret_cast<uint4*>(to + ((int64_t)h * dim + d0) * size) = pack<E>(lo, a.type);
         }
     }
 }
 
-template <int DIM>
+// The queries of row `r` at position `pos`, rotated, by one wavefront.
+__device__ __forceinline__ void rotate_row(const AppendArgs& a, int64_t r, int64_t pos, bool bad) {
+    const int lane = threadIdx.x & 63, dim = a.kv.dim, half = a.rope.half, turned = 2 * half;
+    if (a.q_by_16) {
+        if (a.type == MP_TYPE_F32) rotate_wide<4>(a, r, pos, bad);
+        else rotate_wide<8>(a, r, pos, bad);
+        return;
+    }
+    // One pair, or one dim that passes, at a time.
+    const int64_t from = r * a.q_stride, to = r * a.q_out_stride;
+    const int per_head = half + dim - turned;
+    for (int i = lane; i < a.heads * per_head; i += 64) {
+        const int head = i / per_head, p = i % per_head;
+        const int64_t src = from + (int64_t)head * dim, dst = to + (int64_t)head * dim;
+        if (p >= half) {
+            const int d = turned + p - half;
+            const float x = load_one(a.q, a.type, src + d);
+            store_one(a.q_out, a.type, dst + d, bad ? quiet_nan() : x);
+            continue;
+        }
+        const int d0 = a.rope.interleaved ? 2 * p : p, d1 = a.rope.interleaved ? 2 * p + 1 : p + half;
+        const float c = bad ? quiet_nan() : a.rope.cos[pos * half + p], s = bad ? quiet_nan() : a.rope.sin[pos * half + p];
+        const float x = load_one(a.q, a.type, src + d0), y = load_one(a.q, a.type, src + d1);
+        store_one(a.q_out, a.type, dst + d0, x * c - y * s);
+        store_one(a.q_out, a.type, dst + d1, y * c + x * s);
+    }
+}
+
+// The query row of a wavefront of work-group `group`; rows as items, behind
+// those before starts[0].
+__device__ __forceinline__ void rotate_rows(const AppendArgs& a, int group) {
+    Kv8Item at;
+    const int row = group * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (row >= a.rows.rows || !kv8_find(a.rows, row, [](int count, int) { return count; }, &at)) return;
+    const int64_t pos = (int64_t)at.used + at.index;
+    rotate_row(a, at.row0 + at.index, pos, a.rope.half && (at.used < 0 || pos >= a.rope.positions));
+}
+
+// Type and format are constants of a kernel: loads of elements under a branch
+// on either are each waited for before the next (237 us instead of 67 for the
+// keys and values of 16.8k BF16 rows of 8 heads of 128). The queries' rows go
+// beside the keys and values in one launch: 136 instead of 147 us in two for
+// those rows and their 32 query heads, read back, and 8.0 instead of 10.5 for
+// one row of 9 heads of 64.
+template <int TYPE, int FORMAT, int DIM>
 __global__ __launch_bounds__(512) void kv8_append_kernel(AppendArgs a) {
     __shared__ uint32_t amax_s[8];
-    if ((int)blockIdx.x < a.kv_groups) append_unit<DIM>(a, amax_s);
-    else rotate_row(a, (blockIdx.x - a.kv_groups) * (blockDim.x >> 6) + (threadIdx.x >> 6));
+    a.type = TYPE;
+    a.format = FORMAT;
+    if ((int)blockIdx.x < a.kv_groups) {
+        const Unit u = unit_of(a.kv);
+        Tile t = find_tile(a.kv, a.rows, u.item, u.tile);
+        if (a.rope.half) t.last = min(t.last, a.rope.positions - t.pos0);
+        append_unit<DIM>(a, u, t, amax_s);
+    } else {
+        rotate_rows(a, blockIdx.x - a.kv_groups);
+    }
 }
 
 struct ReadArgs {
@@ -346,28 +425,31 @@ struct ReadArgs {
     bool wide[2];
 };
 
-template <int DIM>
+template <int TYPE, int FORMAT, int DIM>
 __global__ __launch_bounds__(512) void kv8_read_kernel(ReadArgs a) {
+    a.type = TYPE;
+    a.format = FORMAT;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const Unit u = unit_of(a.kv);
     const Tile t = find_tile(a.kv, a.rows, u.item, u.tile);
     if (!t.found || t.first >= kTile || t.last <= 0) return;
     const int first = max(t.first, 0);  // row0 is that of slot t.first
-    void* const dst = u.kind ? a.x[1] : a.x[0];
-    const int64_t stride = u.kind ? a.x_stride[1] : a.x_stride[0];
-    const bool wide = u.kind ? a.wide[1] : a.wide[0];
-    const size_t index = kv8_head(a.kv, max(t.block, 0), u.head);
+    const int head = u.head, kind = u.kind;
+    void* const dst = kind ? a.x[1] : a.x[0];
+    const int64_t stride = kind ? a.x_stride[1] : a.x_stride[0];
+    const bool wide = kind ? a.wide[1] : a.wide[0];
+    const size_t index = kv8_head(a.kv, max(t.block, 0), head);
     const float scale =
-        t.block >= 0 ? reinterpret_cast<const float*>(a.kv.scales + index)[u.kind] : quiet_nan();
-    const uint8_t* const bytes = (u.kind ? a.kv.values : a.kv.keys) + index * ((size_t)DIM << a.kv.page_shift) +
+        t.block >= 0 ? reinterpret_cast<const float*>(a.kv.scales + index)[kind] : quiet_nan();
+    const uint8_t* const bytes = (kind ? a.kv.values : a.kv.keys) + index * ((size_t)DIM << a.kv.page_shift) +
                                  u.tile * kTile * DIM + 16 * lane;
 #pragma unroll
     for (int j = 0; j < DIM / 64; ++j) {
         const uint4 v = *reinterpret_cast<const uint4*>(bytes + 1024 * j);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        if (u.kind == 0) {
+        if (kind == 0) {
             if (c < first || c >= t.last) continue;
-            const int64_t at = (t.row0 + c - t.first) * stride + (int64_t)u.head * DIM + 64 * j + 16 * g;
+            const int64_t at = (t.row0 + c - t.first) * stride + (int64_t)head * DIM + 64 * j + 16 * g;
 #pragma unroll
             for (int n = 0; n < 4; ++n)
                 store_four(dst, a.type, wide, at + 4 * n, decode(byte_of(w[n], 0), a.format) * scale,
@@ -378,13 +460,33 @@ __global__ __launch_bounds__(512) void kv8_read_kernel(ReadArgs a) {
             for (int i = 0; i < 4; ++i) {
                 const int slot = 4 * g + i;
                 if (slot < first || slot >= t.last) continue;
-                const int64_t at = (t.row0 + slot - t.first) * stride + (int64_t)u.head * DIM + 64 * j + c;
+                const int64_t at = (t.row0 + slot - t.first) * stride + (int64_t)head * DIM + 64 * j + c;
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
                     store_one(dst, a.type, at + 16 * n, decode(byte_of(w[n], i), a.format) * scale);
             }
         }
     }
+}
+
+// Calls f(type, format, dim) with the call's as constants.
+template <typename F, int TYPE, int FORMAT>
+hipError_t with_dim(int dim, const F& f) {
+    using Type = std::integral_constant<int, TYPE>;
+    using Format = std::integral_constant<int, FORMAT>;
+    if (dim == 64) return f(Type(), Format(), std::integral_constant<int, 64>());
+    if (dim == 128) return f(Type(), Format(), std::integral_constant<int, 128>());
+    return f(Type(), Format(), std::integral_constant<int, 256>());
+}
+template <typename F, int TYPE>
+hipError_t with_format(int format, int dim, const F& f) {
+    return format == MP_KV8_INT8 ? with_dim<F, TYPE, MP_KV8_INT8>(dim, f) : with_dim<F, TYPE, MP_KV8_E4M3>(dim, f);
+}
+template <typename F>
+hipError_t with_constants(int type, int format, int dim, const F& f) {
+    if (type == MP_TYPE_F32) return with_format<F, MP_TYPE_F32>(format, dim, f);
+    if (type == MP_TYPE_BF16) return with_format<F, MP_TYPE_BF16>(format, dim, f);
+    return with_format<F, MP_TYPE_F16>(format, dim, f);
 }
 
 int threads_for(int bt) { return bt == 128 ? 512 : kThreads; }
@@ -431,7 +533,7 @@ extern "C" int mp_hip_kv8_append(const mp_kv8_cache* cache, int32_t layer, const
         if (rows == 0 || sequences == 0) return MP_OK;
         const int bt = cache->block_tokens, threads = threads_for(bt), waves = threads / 64;
         const int64_t units = kv8_most_pages(rows, sequences, bt) * cache->kv_heads * 2, per_group = waves / (bt / kTile);
-        const int64_t kv_groups = (units + per_group - 1) / per_group, q_groups = q ? (rows + waves - 1) / waves : 0;
+        const int64_t kv_groups = kv8_ceil(units, per_group), q_groups = q ? kv8_ceil(rows, waves) : 0;
         if (kv_groups + q_groups > kMaxGroups) return too_large();
         AppendArgs a{};
         a.kv = kv8_layer(*cache, layer);
@@ -443,16 +545,20 @@ extern "C" int mp_hip_kv8_append(const mp_kv8_cache* cache, int32_t layer, const
         a.q_stride = q_stride, a.q_out_stride = q_out_stride;
         a.heads = heads, a.type = type, a.format = cache->format;
         a.wide[0] = kv8_wide(k, k_stride, type), a.wide[1] = kv8_wide(v, v_stride, type);
-        a.q_wide = q && kv8_wide(q, q_stride, type) && kv8_wide(q_out, q_out_stride, type);
+        const int per16 = 16 / (int)kv8_element(type);
+        a.q_by_16 = q && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0 &&
+                    q_stride % per16 == 0 && q_out_stride % per16 == 0 &&
+                    (view.interleaved ? 2 * view.half : view.half) % per16 == 0;
         a.kv_groups = (int)kv_groups;
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const StreamDevice device(s);
         if (device.status != hipSuccess) return kv8_done(device.status, "8-bit append: device of the stream");
-        const dim3 grid((unsigned)(kv_groups + q_groups));
-        if (cache->dim == 64) kv8_append_kernel<64><<<grid, threads, 0, s>>>(a);
-        else if (cache->dim == 128) kv8_append_kernel<128><<<grid, threads, 0, s>>>(a);
-        else kv8_append_kernel<256><<<grid, threads, 0, s>>>(a);
-        return kv8_done(hipGetLastError(), "8-bit append launch");
+        const hipError_t e = with_constants(type, cache->format, cache->dim, [&](auto t, auto f, auto d) {
+            kv8_append_kernel<decltype(t)::value, decltype(f)::value, decltype(d)::value>
+                <<<(unsigned)(kv_groups + q_groups), threads, 0, s>>>(a);
+            return hipGetLastError();
+        });
+        return kv8_done(e, "8-bit append launch");
     });
 }
 
@@ -473,7 +579,7 @@ extern "C" int mp_hip_kv8_read(const mp_kv8_cache* cache, int32_t layer, const i
         if (rows == 0 || sequences == 0) return MP_OK;
         const int bt = cache->block_tokens, threads = threads_for(bt), waves = threads / 64;
         const int64_t units = kv8_most_pages(rows, sequences, bt) * cache->kv_heads * 2, per_group = waves / (bt / kTile);
-        const int64_t groups = (units + per_group - 1) / per_group;
+        const int64_t groups = kv8_ceil(units, per_group);
         if (groups > kMaxGroups) return too_large();
         ReadArgs a{};
         a.kv = kv8_layer(*cache, layer);
@@ -485,10 +591,11 @@ extern "C" int mp_hip_kv8_read(const mp_kv8_cache* cache, int32_t layer, const i
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const StreamDevice device(s);
         if (device.status != hipSuccess) return kv8_done(device.status, "8-bit read: device of the stream");
-        const dim3 grid((unsigned)groups);
-        if (cache->dim == 64) kv8_read_kernel<64><<<grid, threads, 0, s>>>(a);
-        else if (cache->dim == 128) kv8_read_kernel<128><<<grid, threads, 0, s>>>(a);
-        else kv8_read_kernel<256><<<grid, threads, 0, s>>>(a);
-        return kv8_done(hipGetLastError(), "8-bit read launch");
+        const hipError_t e = with_constants(type, cache->format, cache->dim, [&](auto t, auto f, auto d) {
+            kv8_read_kernel<decltype(t)::value, decltype(f)::value, decltype(d)::value>
+                <<<(unsigned)groups, threads, 0, s>>>(a);
+            return hipGetLastError();
+        });
+        return kv8_done(e, "8-bit read launch");
     });
 }

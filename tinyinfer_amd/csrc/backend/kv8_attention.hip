@@ -29,114 +29,13 @@
 #include <type_traits>
 
 #include "kernels.h"
-#include "kv8.h"
+#include "kv8_mma.h"
 
 // The summation order is the kernels' own: multiply-adds may be fused.
 #pragma clang fp contract(fast)
 
 namespace mphip {
 namespace {
-
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-
-enum Mode { kPacked, kTwo, kOne };
-
-constexpr float kShift = 11.0f;  // probabilities are held times 2^11 ...
-constexpr float kRaise = 15.0f;  // ... and below 2^15: past it the reference is raised
-
-struct AttentionArgs {
-    Kv8Layer kv;
-    Kv8Rows rows;          // decode: starts null, used = lengths
-    const void* q;
-    void* out;
-    int64_t q_stride, out_stride;
-    int heads, group, type, max_length, chunk, splits;
-    float scale;           // times log2(e)
-    bool q_wide, out_wide;
-    float* partial_out;    // [row][head][split][dim]
-    float2* partial_ml;    // [row][head][split]: reference (log2), sum
-};
-
-__device__ __forceinline__ float infinity() { return __builtin_inff(); }
-__device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7FC00000u); }
-
-// Of the four lanes (c, 0..3) of a column.
-__device__ __forceinline__ float column_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
-}
-
-// Four codes times a power of two as FP16. INT8: a byte b under 0x64 is the
-// FP16 number 1024 + b; less 1152 it is the code, exactly. E4M3: the
-// conversion takes the power of two.
-template <int FORMAT>
-struct Convert;
-template <>
-struct Convert<MP_KV8_INT8> {
-    h2 times, less;
-    explicit __device__ __forceinline__ Convert(float power) {
-        const _Float16 p = (_Float16)power;
-        times = h2{p, p};
-        less = h2{(_Float16)-1152, (_Float16)-1152} * times;
-    }
-    __device__ __forceinline__ void operator()(uint32_t w, h2* lo, h2* hi) const {
-        const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u));
-        const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u));
-        *lo = __builtin_elementwise_fma(a, times, less);
-        *hi = __builtin_elementwise_fma(b, times, less);
-    }
-    // Power 1.
-    static __device__ __forceinline__ void plain(uint32_t w, h2* lo, h2* hi) {
-        const h2 less = {(_Float16)-1152, (_Float16)-1152};
-        *lo = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + less;
-        *hi = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + less;
-    }
-};
-template <>
-struct Convert<MP_KV8_E4M3> {
-    float power;
-    explicit __device__ __forceinline__ Convert(float p) : power(p) {}
-    __device__ __forceinline__ void operator()(uint32_t w, h2* lo, h2* hi) const {
-        *lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, false);
-        *hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, true);
-    }
-    static __device__ __forceinline__ void plain(uint32_t w, h2* lo, h2* hi) {
-        *lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
-        *hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
-    }
-};
-
-union Half8 {
-    h8 all;
-    h2 two[4];
-    _Float16 one[8];
-};
-
-// A load through the scalar cache, at byte `offset` of an array that no kernel
-// beside this one writes; uniform over the wavefront.
-__device__ __forceinline__ int scalar_int(const void* p, uint32_t offset) {
-    return *(const __attribute__((address_space(4))) int32_t*)((uintptr_t)p + offset);
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-
-// x - (float)half of the low or high half, times `factor`: factor * half + x.
-__device__ __forceinline__ float mix_low(h2 half, float factor, float x) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(half), "v"(factor), "v"(x));
-    return r;
-}
-__device__ __forceinline__ float mix_high(h2 half, float factor, float x) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(half), "v"(factor), "v"(x));
-    return r;
-}
 
 // 16-dim tiles of every wavefront that meet in LDS at a time, in 32 KB of it
 // where that holds one: 1 KB a tile, wavefront and column tile.
@@ -148,10 +47,16 @@ constexpr size_t join_bytes(int waves, int column_tiles, int dims) {
     return waves == 1 ? 0 : (size_t)waves * column_tiles * join_dims(waves <= 4 ? 4 : kKv8MostWaves, column_tiles, dims) * 1024;
 }
 
+// Wavefronts a SIMD that the registers are kept to.
+constexpr int least_waves(int dim, int column_tiles, bool decode) {
+    return !decode && dim == 64 && column_tiles == 2 ? 3 : 2;
+}
+
 // DECODE: one row a sequence, its columns the KV head's query heads; else
 // columns are those of a sequence's rows, row major.
 template <int FORMAT, int DIM, int NT, int MODE, bool DECODE>
-__global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(64 * kKv8MostWaves) __attribute__((amdgpu_waves_per_eu(least_waves(DIM, NT, DECODE)))) void
+kv8_attention_kernel(Kv8Attention a) {
     constexpr int kDepth = DECODE ? 2 : 1;
     constexpr int kSteps = DIM / 32;             // of the contraction over dims
     constexpr int kDims = DIM / 16;              // 16-dim tiles of the output
@@ -163,13 +68,14 @@ __global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(Atten
     float2(*const ml_s)[NT][16] = reinterpret_cast<float2(*)[NT][16]>(shared_s);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int head = blockIdx.y, split = blockIdx.z;
+    // Neighbouring work-groups, on different XCDs, have different heads.
+    const int head = blockIdx.x % a.kv.kv_heads, item = blockIdx.x / a.kv.kv_heads, split = blockIdx.z;
 
     // The work-group's columns, all of one sequence: rows row0.. and the
     // position of the first, `first` columns into the sequence's.
     int sequence, row0, count, used, first;
     if (DECODE) {
-        sequence = row0 = blockIdx.x;
+        sequence = row0 = item;
         count = 1;
         const int length = scalar_int(a.rows.used, (uint32_t)sequence * 4u);
         used = min(length, a.max_length + 1) - 1;
@@ -183,8 +89,7 @@ __global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(Atten
     } else {
         Kv8Item at;
         const int group = a.group;
-        if (!kv8_find(a.rows, blockIdx.x, [=](int n, int) { return (n * group + 16 * NT - 1) / (16 * NT); }, &at))
-            return;
+        if (!kv8_find(a.rows, item, [=](int n, int) { return (n * group + 16 * NT - 1) / (16 * NT); }, &at)) return;
         sequence = at.sequence;
         row0 = at.row0;
         count = at.count;
@@ -223,177 +128,49 @@ __global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(Atten
 
     // This wavefront's pairs of tiles: pair0, + waves, ... of the chunk's, `n`
     // of them done, `pairs` in all.
-    const int32_t* const table = a.rows.tables + (size_t)sequence * a.rows.table_stride;
     const int tile_end = (end + kTile - 1) / kTile, pair0 = begin / kKv8Pair + wave;
     const int pairs = max((tile_end + 1) / 2 - pair0 + waves - 1, 0) / waves;
 
     // The loop runs on pairs in two strands that do not wait for each other:
     // the scores of pair n+1 are multiplied while the probabilities of pair n
     // are formed and multiplied with its values. Keys are loaded kDepth + 1
-    // and values kDepth pairs ahead, into the registers just used up. Behind
-    // the last pair the loads are of no bytes: their number is the same at
-    // every step, and so is what a step waits for.
-    //
-    // Where tiles lie and their scales are worked out by the lanes: lane l
-    // holds tile l%2 of the pairs whose number is l/2 modulo 32, and a step
-    // reads what it needs from a lane. Every 16 pairs half the lanes go on to
-    // the pairs 32 on, whose scales were fetched 16 pairs and whose table
-    // entries 32 pairs before. A page that is none reads page 0 and has NaN
-    // scales; a tile behind the last (of a row that ends in a pair's first
-    // tile) reads page 0 and has scales 0.
-    const uint32_t block_scales = (uint32_t)a.kv.layers * a.kv.kv_heads;  // heads of a block
-    const uint32_t block_bytes = block_scales * DIM << a.kv.page_shift;
-    const uint32_t head_bytes = (uint32_t)(a.kv.layer * a.kv.kv_heads + head) * DIM << a.kv.page_shift;
-    const float2* const scales = a.kv.scales + (a.kv.layer * a.kv.kv_heads + head);
-    struct Tiles {
-        uint64_t base;
-        float2 bits;
-        uint32_t none, present;  // bits of NaN or 0; all bits or 0
-    };
-    uint32_t at_low, at_high, at_k, at_v;  // this lane's tile: where, and its scales' bits
-    Tiles soon;                            // of the pairs 32 on
-    int found;                             // their successors' table entry
-    const auto tile_of = [&](int n) { return 2 * (pair0 + n * waves) + (lane & 1); };
-    const auto find_block = [&](int n) {
-        return table[min(tile_of(n) >> (a.kv.page_shift - 4), a.rows.table_stride - 1)];
-    };
-    const auto find_tile = [&](int n, int block) {
-        const int tile = tile_of(n);
-        const bool is = (unsigned)block < (unsigned)a.kv.blocks;
-        const uint32_t at = is && tile < tile_end ? block : 0;
-        Tiles t;
-        t.none = is ? 0u : 0x7FC00000u;
-        t.present = tile < tile_end ? ~0u : 0u;
-        t.base = (uint64_t)at * block_bytes + (head_bytes + (tile & ((1 << (a.kv.page_shift - 4)) - 1)) * (kTile * DIM));
-        t.bits = scales[(size_t)at * block_scales];
-        return t;
-    };
-    const auto take_tile = [&](const Tiles& t) {
-        at_low = (uint32_t)t.base;
-        at_high = (uint32_t)(t.base >> 32);
-        at_k = (__float_as_uint(t.bits.x) | t.none) & t.present;
-        at_v = (__float_as_uint(t.bits.y) | t.none) & t.present;
-    };
-    // Before pair n's keys are looked for.
-    const auto go_on = [&](int n) {
-        if (n & 15 || n < 32 || n >= pairs) return;
-        if ((lane >> 5) == ((n >> 4) & 1)) take_tile(soon);
-        soon = find_tile(n + 16 + (lane >> 1 & 15), found);
-        found = find_block(n + 32 + (lane >> 1 & 15));
-    };
+    // and values kDepth pairs ahead, into the registers just used up; the
+    // number of loads is the same at every step, and so is what a step waits for.
+    // Behind the last pair the loads are of no bytes.
+    Kv8Tiles<DIM, 2> tiles;
+    const int first_block = tiles.begin(a, sequence, head, 2 * pair0, 2 * waves, tile_end, pairs, lane);
     u4 raw_k[kDepth][2][DIM / 64], raw_v[kDepth][2][DIM / 64];
     uint64_t base[2], base_v[2];  // of the newest pair; of the one before
     int size, size_v;
     const auto find_pair = [&](int n) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int from = 2 * (n & 31) + h;
-            base[h] = (uint32_t)__builtin_amdgcn_readlane(at_low, from) |
-                      (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_high, from) << 32;
-        }
+        base[0] = tiles.base(n, 0);
+        base[1] = tiles.base(n, 1);
         size = n < pairs ? kTile * DIM : 0;
     };
     const auto load = [&](uint8_t* pool, const uint64_t (&at)[2], int bytes, u4 (&raw)[2][DIM / 64]) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const auto tile = __builtin_amdgcn_make_buffer_rsrc(pool + at[h], 0, bytes, 0x27000);
-#pragma unroll
-            for (int j = 0; j < DIM / 64; ++j)
-                raw[h][j] = __builtin_amdgcn_raw_buffer_load_b128(tile, 16 * lane + 1024 * j, 0, 0);
-        }
+        load_tile<DIM>(pool, at[0], bytes, lane, raw[0]);
+        load_tile<DIM>(pool, at[1], bytes, lane, raw[1]);
     };
-    const int first_block = find_block(lane >> 1);
-    // The queries' bytes: all loads before any use, and before those of keys
-    // and values, which wait for the table.
+    // The queries' loads come before those of keys and values, which wait for
+    // the table.
     const bool f32 = DECODE ? a.type == MP_TYPE_F32 : MODE == kTwo;
-    u4 raw_q[NT][DIM / 64][4];  // 16 elements; the last two unused for 16-bit types
-    const auto raw_queries = [&](auto get) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int j = 0; j < DIM / 64; ++j) get(raw_q[t][j], q_at[t] + 64 * j + 16 * g);
-    };
-    if (f32) {
-        const float* const from = static_cast<const float*>(a.q);
-        if (a.q_wide)
-            raw_queries([&](u4 (&to)[4], int64_t i) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) to[k] = *reinterpret_cast<const u4*>(from + i + 4 * k);
-            });
-        else
-            raw_queries([&](u4 (&to)[4], int64_t i) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) to[k / 4][k % 4] = __float_as_uint(from[i + k]);
-            });
-    } else {
-        typedef u4 u4_by_8 __attribute__((aligned(8)));
-        const uint16_t* const from = static_cast<const uint16_t*>(a.q);
-        if (a.q_wide)
-            raw_queries([&](u4 (&to)[4], int64_t i) {
-                to[0] = *reinterpret_cast<const u4_by_8*>(from + i);
-                to[1] = *reinterpret_cast<const u4_by_8*>(from + i + 8);
-            });
-        else
-            raw_queries([&](u4 (&to)[4], int64_t i) {
-#pragma unroll
-                for (int k = 0; k < 16; k += 2)
-                    to[k / 8][k / 2 % 4] = from[i + k] | (uint32_t)from[i + k + 1] << 16;
-            });
-    }
+    u4 raw_q[NT][DIM / 64][4];
+    load_queries<DIM, NT>(a, f32, q_at, g, raw_q);
     {
-        const Tiles t = find_tile(lane >> 1, first_block);
-        at_low = (uint32_t)t.base;
-        at_high = (uint32_t)(t.base >> 32);
+        const auto t = tiles.find(lane / 2, first_block);
+        tiles.take_places(t);
 #pragma unroll
         for (int d = 0; d < kDepth; ++d) {
             find_pair(d);
             load(a.kv.keys, base, size, raw_k[d]);
             load(a.kv.values, base, size, raw_v[d]);
         }
-        take_tile(t);
+        tiles.take_scales(t);
     }
-    if (pairs > 32) {
-        soon = find_tile(32 + (lane >> 1 & 15), find_block(32 + (lane >> 1 & 15)));
-        found = find_block(48 + (lane >> 1 & 15));
-    }
-
-    // Queries: part, column tile, step (j, h): dims 64j + 16g + 8h .. +7.
+    tiles.look_ahead();
     Half8 q[kParts][NT][kSteps];
-    float factor[NT];  // of a score: softmax scale / the query's power of two
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        float x[DIM / 64][16];
-        uint32_t amax = 0;
-#pragma unroll
-        for (int j = 0; j < DIM / 64; ++j)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t two = raw_q[t][j][i / 8][i / 2 % 4];
-                x[j][i] = f32                          ? __uint_as_float(raw_q[t][j][i / 4][i % 4])
-                          : a.type == MP_TYPE_BF16     ? __uint_as_float(i % 2 ? two & 0xFFFF0000u : two << 16)
-                                                       : from_f16(i % 2 ? two >> 16 : two & 0xFFFF);
-                amax = max(amax, __float_as_uint(x[j][i]) & 0x7FFFFFFFu);
-            }
-        amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
-        amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-        const int power = min(127 + 14 - (int)(amax >> 23), 126);  // at least -113
-        const float up = __uint_as_float((uint32_t)(127 + power) << 23);
-        // NaN for a row that is not finite or whose pages the table has not.
-        const bool lost = amax >= 0x7F800000u || qpos[t] >> a.kv.page_shift >= a.rows.table_stride;
-        factor[t] = lost ? quiet_nan() : a.scale * __uint_as_float((uint32_t)(127 - power) << 23);
-#pragma unroll
-        for (int j = 0; j < DIM / 64; ++j)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float u = x[j][i] * up, v = x[j][i + 1] * up;
-                const h2 high = {(_Float16)u, (_Float16)v};
-                const h2 low = {(_Float16)(u - (float)high[0]), (_Float16)(v - (float)high[1])};
-                h2& first = q[0][t][2 * j + i / 8].two[i % 8 / 2];
-                if (MODE == kPacked) first = c & 8 ? low : high;
-                else first = high;
-                if (MODE == kTwo) q[kParts - 1][t][2 * j + i / 8].two[i % 8 / 2] = low;
-            }
-    }
+    float factor[NT];
+    split_queries<DIM, NT, MODE, kParts>(a, f32, raw_q, qpos, c, q, factor);
 
     // o, and the sum of the probabilities as one more row of the product with
     // the values (a matrix of ones), whose four registers are the same.
@@ -436,10 +213,8 @@ __global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(Atten
 
     // `k_next`: the next pair's keys, `v`: this one's values.
     const auto step = [&](int n, u4 (&k_next)[2][DIM / 64], u4 (&v)[2][DIM / 64]) {
-        const uint32_t k_bits[2] = {(uint32_t)__builtin_amdgcn_readlane(at_k, 2 * (n & 31)),
-                                    (uint32_t)__builtin_amdgcn_readlane(at_k, 2 * (n & 31) + 1)};
-        const uint32_t v_bits[2] = {(uint32_t)__builtin_amdgcn_readlane(at_v, 2 * (n & 31)),
-                                    (uint32_t)__builtin_amdgcn_readlane(at_v, 2 * (n & 31) + 1)};
+        const uint32_t k_bits[2] = {tiles.k_bits(n, 0), tiles.k_bits(n, 1)};
+        const uint32_t v_bits[2] = {tiles.v_bits(n, 0), tiles.v_bits(n, 1)};
         if (MODE == kPacked) {  // the low parts' scores are 8 columns on
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -466,17 +241,9 @@ __global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(Atten
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (token0 + kTile * h + 4 * g + i > qpos[t]) s[t][h][i] = -infinity();
-            // Slots past the last row's position may hold anything: as bytes
-            // they are made 0 where an E4M3 NaN could be (INT8 codes are
-            // finite, and their probability is 0).
             if (FORMAT == MP_KV8_E4M3 && token0 + kKv8Pair - 1 > last) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int left = last + 1 - token0 - kTile * h - 4 * g;
-                    const uint32_t keep = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
-#pragma unroll
-                    for (int j = 0; j < DIM / 64; ++j) v[h][j] &= keep;
-                }
+                clear_past<DIM>(last + 1 - token0 - 4 * g, v[0]);
+                clear_past<DIM>(last + 1 - token0 - kTile - 4 * g, v[1]);
             }
         }
         // The reference is raised only where a score is past the limit.
@@ -519,11 +286,7 @@ __global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(Atten
             }
             v_top = v_now;
         }
-        // Powers of two of the tiles' values; 2^-40 of the top one is nothing.
-        const auto power = [&](uint32_t bits) {
-            return __uint_as_float((uint32_t)max((int)(bits - v_top) + (127 << 23), (127 - 40) << 23));
-        };
-        const Convert<FORMAT> convert0(power(v_bits[0])), convert1(power(v_bits[1]));
+        const Convert<FORMAT> convert0(value_power(v_bits[0], v_top)), convert1(value_power(v_bits[1], v_top));
         base_v[0] = base[0], base_v[1] = base[1], size_v = size;
         find_pair(n + kDepth + 1);
         f4 s_next[NT][2];
@@ -566,7 +329,7 @@ __global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(Atten
     for (int n = 0; n < pairs;) {
 #pragma unroll
         for (int d = 0; d < kDepth; ++d) {
-            go_on(n + kDepth + 1);
+            tiles.go_on(n + kDepth + 1);
             step(n, raw_k[(d + 1) % kDepth], raw_v[d]);
             if (++n >= pairs && d + 1 < kDepth) break;
         }
@@ -665,7 +428,7 @@ __global__ __launch_bounds__(64 * kKv8MostWaves) void kv8_attention_kernel(Atten
 // four (row, head) or one a work-group. `columns_tile`: columns of an
 // attention work-group.
 template <bool DECODE, int WAVES>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(AttentionArgs a, int columns_tile) {
+__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Attention a, int columns_tile) {
     __shared__ f4 out_s[WAVES][64];
     const int lane = threadIdx.x & 63, dim = a.kv.dim;
     const int in_group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -726,42 +489,33 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(AttentionArgs a, int col
                    out[3]);
 }
 
-// Column tiles that a prefill wavefront holds in its registers.
-constexpr int most_tiles(int dim, int mode) {
-    return dim == 64 ? 4 : dim == 128 ? (mode == kTwo ? 2 : 4) : (mode == kTwo ? 1 : 2);
-}
-
 template <int FORMAT, int DIM, int NT, int MODE, bool DECODE>
-void launch(hipStream_t s, const Kv8Plan& p, int64_t items, const AttentionArgs& a) {
-    const dim3 grid((unsigned)items, (unsigned)a.kv.kv_heads, (unsigned)p.splits);
+void launch(hipStream_t s, const Kv8Plan& p, int64_t items, const Kv8Attention& a) {
+    const dim3 grid((unsigned)(items * a.kv.kv_heads), 1, (unsigned)p.splits);
     const size_t shared = join_bytes(p.waves, NT, DIM / 16);
     kv8_attention_kernel<FORMAT, DIM, NT, MODE, DECODE><<<grid, 64 * p.waves, shared, s>>>(a);
 }
 template <int FORMAT, int DIM>
-void launch_decode(hipStream_t s, const Kv8Plan& p, const AttentionArgs& a) {
+void launch_decode(hipStream_t s, const Kv8Plan& p, const Kv8Attention& a) {
     if (a.group <= 8) launch<FORMAT, DIM, 1, kPacked, true>(s, p, a.rows.rows, a);
     else launch<FORMAT, DIM, 1, kTwo, true>(s, p, a.rows.rows, a);
 }
 template <int FORMAT, int DIM, int MODE>
-void launch_prefill(hipStream_t s, const Kv8Plan& p, const AttentionArgs& a) {
+void launch_prefill(hipStream_t s, const Kv8Plan& p, const Kv8Attention& a) {
     const int64_t items = kv8_items(a.rows.rows, a.rows.sequences, a.group, p.column_tiles);
-    constexpr int kMost = most_tiles(DIM, MODE);
-    if (p.column_tiles == 4) {
-        if constexpr (kMost >= 4) launch<FORMAT, DIM, 4, MODE, false>(s, p, items, a);
-    } else if (p.column_tiles == 2) {
-        if constexpr (kMost >= 2) launch<FORMAT, DIM, 2, MODE, false>(s, p, items, a);
-    } else {
-        launch<FORMAT, DIM, 1, MODE, false>(s, p, items, a);
+    if constexpr (DIM <= 128) {
+        if (p.column_tiles == 2) return launch<FORMAT, DIM, 2, MODE, false>(s, p, items, a);
     }
+    launch<FORMAT, DIM, 1, MODE, false>(s, p, items, a);
 }
 template <int FORMAT, int DIM>
-void launch_attention(hipStream_t s, const Kv8Plan& p, const AttentionArgs& a, bool decode) {
+void launch_attention(hipStream_t s, const Kv8Plan& p, const Kv8Attention& a, bool decode) {
     if (decode) launch_decode<FORMAT, DIM>(s, p, a);
     else if (a.type == MP_TYPE_F32) launch_prefill<FORMAT, DIM, kTwo>(s, p, a);
     else launch_prefill<FORMAT, DIM, kOne>(s, p, a);
 }
 template <int FORMAT>
-void launch_format(hipStream_t s, const Kv8Plan& p, const AttentionArgs& a, bool decode) {
+void launch_format(hipStream_t s, const Kv8Plan& p, const Kv8Attention& a, bool decode) {
     if (a.kv.dim == 64) launch_attention<FORMAT, 64>(s, p, a, decode);
     else if (a.kv.dim == 128) launch_attention<FORMAT, 128>(s, p, a, decode);
     else launch_attention<FORMAT, 256>(s, p, a, decode);
@@ -788,17 +542,19 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
     if (kv8_bad_ints(used) || (!decode && kv8_bad_ints(starts)))
         return kv8_refuse("8-bit attention: lengths, starts or used are missing or misaligned");
     if (!isfinite(scale) || scale < 0) return kv8_refuse("8-bit attention: scale must be finite and not negative");
+    if ((int64_t)rows * heads > kKv8MostColumns)
+        return kv8_refuse("8-bit attention: rows times heads are too many for one call");
     if (rows == 0 || sequences == 0) return MP_OK;
     const int group = heads / cache->kv_heads;
     const Kv8Plan p = decode ? kv8_decode_plan(rows, cache->kv_heads, max_length)
-                             : kv8_prefill_plan(rows, sequences, cache->kv_heads, group,
-                                                most_tiles(cache->dim, type == MP_TYPE_F32 ? kTwo : kOne), max_length);
+                             : kv8_prefill_plan(rows, sequences, cache->kv_heads, group, cache->dim,
+                                                max_length);
     const size_t need = kv8_partial_floats(p, rows, heads, cache->dim) * sizeof(float);
     if (need > workspace_bytes || (need && !workspace))
         return kv8_refuse("8-bit attention: the workspace is smaller than mp_hip_kv8_attention_workspace says");
     if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
         return kv8_refuse("8-bit attention: the workspace must be 16-byte aligned");
-    AttentionArgs a{};
+    Kv8Attention a{};
     a.kv = kv8_layer(*cache, layer);
     a.rows = Kv8Rows{tables, starts, used, table_stride, sequences, rows};
     a.q = q, a.out = out;

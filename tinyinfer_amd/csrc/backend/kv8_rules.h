@@ -10,6 +10,9 @@ namespace mphip {
 constexpr int kTile = 16;  // tokens of a tile
 constexpr int kKv8MaxRows = 1 << 20, kKv8MaxHeads = 1024, kKv8MaxGroup = 16, kKv8MaxLength = 1 << 30;
 
+// Rows times query heads of an attention call: 2^31 threads at most.
+constexpr int64_t kKv8MostColumns = 1 << 22;
+
 // Rows start .. next-1 of a sequence inside 0 .. rows-1, whatever the two are.
 struct Kv8Span {
     int row0, count;
@@ -42,6 +45,8 @@ constexpr int64_t kv8_most_pages(int rows, int sequences, int bt) {
     const int64_t by_pages = ((int64_t)rows + (int64_t)sequences * (2 * bt - 2)) / bt;
     return by_pages < rows ? by_pages : rows;
 }
+constexpr int64_t kv8_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 // A table's page `page` if it is one of the pool's, else -1.
 constexpr int kv8_block(const int32_t* table, int stride, int page, int blocks) {
     if (page < 0 || page >= stride) return -1;
@@ -63,8 +68,6 @@ constexpr int kKv8LeastChunk = 128;   // tokens
 
 constexpr int kKv8MostWaves = 8;  // of a work-group
 
-constexpr int64_t kv8_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // Tokens a chunk and how many chunks, for `items` work-groups a chunk.
 inline void kv8_split(Kv8Plan* p, int64_t items, int max_length) {
     const int64_t step = (int64_t)kKv8Pair * p->waves;
@@ -79,23 +82,28 @@ inline void kv8_split(Kv8Plan* p, int64_t items, int max_length) {
 // Up to 4,096 tokens a row's work-group is left alone with it: a second launch
 // to join chunks costs 3 to 4 us.
 inline Kv8Plan kv8_decode_plan(int rows, int kv_heads, int max_length) {
-    Kv8Plan p{1, max_length > 1024 && max_length <= 4096 ? 8 : 4, 0, 0};
-    if (max_length <= 4096) kv8_split(&p, kKv8Groups, max_length);
-    else kv8_split(&p, (int64_t)rows * kv_heads, max_length);
+    const int64_t items = (int64_t)rows * kv_heads;
+    Kv8Plan p{1, 4, 0, 0};
+    if (max_length > 4096) {
+        kv8_split(&p, items, max_length);
+    } else {
+        if (max_length > 1024 && items < 512) p.waves = 8;
+        kv8_split(&p, kKv8Groups, max_length);
+    }
     return p;
 }
 
-// Column tiles of all sequences: every sequence's last one may be part empty.
+// Work-groups of `column_tiles` that the sequences' columns take: every
+// sequence's last one may be part empty.
 inline int64_t kv8_items(int rows, int sequences, int group, int column_tiles) {
     const int64_t columns = 16 * column_tiles, by_tiles = (int64_t)rows * group / columns + sequences;
     return by_tiles < rows * (int64_t)group ? by_tiles : rows * (int64_t)group;
 }
 
-// most_tiles: the column tiles a wavefront's registers hold.
-inline Kv8Plan kv8_prefill_plan(int rows, int sequences, int kv_heads, int group, int most_tiles, int max_length) {
+inline Kv8Plan kv8_prefill_plan(int rows, int sequences, int kv_heads, int group, int dim, int max_length) {
     Kv8Plan p{1, 8, 0, 0};
     const int64_t items = kv8_items(rows, sequences, group, 1) * kv_heads;
-    if (items >= 1024) p = Kv8Plan{most_tiles < 2 ? most_tiles : 2, max_length > 2048 ? 4 : 1, 0, 0};
+    if (items >= 1024) p = Kv8Plan{dim <= 128 ? 2 : 1, max_length > 2048 ? 4 : 1, 0, 0};
     if (max_length <= 4096) kv8_split(&p, kKv8Groups, max_length);
     else kv8_split(&p, kv8_items(rows, sequences, group, p.column_tiles) * kv_heads, max_length);
     return p;
@@ -112,7 +120,7 @@ inline size_t kv8_workspace_floats(int rows, int sequences, int heads, int kv_he
     (void)sequences;
     const int64_t splits = kv8_ceil(max_length > 0 ? max_length : 1, kKv8LeastChunk);
     if (splits <= 1) return 0;
-    const int64_t columns = 16 * 4;  // of the largest work-group
+    const int64_t columns = 16 * 2;  // of the largest work-group
     const int64_t by_rows = (int64_t)rows * heads * splits, by_groups = 2ll * kKv8Groups * columns;
     return (size_t)(by_rows < by_groups ? by_rows : by_groups) * (dim + 2);
 }
