@@ -238,9 +238,9 @@ int mp_hip_paged_attention_decode_noalloc(const float* q, const float* keys, con
  * append or read with used[s] outside 0 .. 2^30.
  *
  * What the device finds: a token whose page id is not in 0 .. blocks-1 or
- * whose page lies past table_stride is not written; an attention that needs
- * such a page gives NaN, as it does for a row longer than max_length and for
- * a NaN in the cache or in q. */
+ * whose page lies past table_stride is not written; an attention row that
+ * needs such a page is NaN, as is one longer than max_length and one that
+ * meets a NaN or an infinity in q or a NaN in the pages it sees. */
 enum { MP_TYPE_F32 = 0, MP_TYPE_BF16 = 1, MP_TYPE_F16 = 2 };
 enum { MP_KV8_INT8 = 0, MP_KV8_E4M3 = 1 };
 
@@ -302,8 +302,8 @@ int mp_hip_kv8_attention_workspace(const mp_kv8_cache* cache, int32_t rows, int3
  * lengths[r] tokens of its page table tables + r*table_stride (device int32,
  * at most max_length): out = sum_t softmax_t(scale * q.k_t) v_t, query head h
  * on KV head h / (heads / kv_heads), at most 16 query heads per KV head. A
- * row of no tokens (length 0 or less) gives zeros. `scale` is finite and not
- * negative. Sums are FP32 (about 1e-6 of the 64-bit result for FP32 rows). */
+ * row of no tokens (length 0 or less) gives zeros. `scale` is finite (to
+ * 2.3e38) and not negative. out may be q, with its stride. Sums are FP32 (about 1e-6 of the 64-bit result for FP32 rows). */
 int mp_hip_kv8_attention_decode(const mp_kv8_cache* cache, int32_t layer, const void* q, int64_t q_stride,
                                 int32_t type, const int32_t* tables, int32_t table_stride, const int32_t* lengths,
                                 int32_t rows, int32_t heads, int32_t max_length, float scale, void* out,
@@ -313,7 +313,8 @@ int mp_hip_kv8_attention_decode(const mp_kv8_cache* cache, int32_t layer, const 
  * tokens 0 .. p of its sequence, all of them in the pages already (append
  * first); used[s] + the rows of s is at most max_length. Any mix of counts,
  * single tokens among them. FP32 rows keep FP32 accuracy; for BF16 and FP16
- * rows the probabilities are rounded to FP16 for the product with the values. */
+ * rows the probabilities are rounded to FP16 for the product with the values.
+ * out may be q, with its stride. */
 int mp_hip_kv8_attention_prefill(const mp_kv8_cache* cache, int32_t layer, const void* q, int64_t q_stride,
                                  int32_t type, const int32_t* tables, int32_t table_stride, const int32_t* starts,
                                  const int32_t* used, int32_t sequences, int32_t rows, int32_t heads,

@@ -93,7 +93,7 @@ void plans() {
         const int group = 1 + (int)(rng() % 16), kv_heads = upto(64), dim = 64 << rng() % 3;
         const int rows = upto(1 << 20), sequences = upto(rows), length = (int)(rng() % 8) ? upto(1 << 22) : 0;
         const int heads = group * kv_heads;
-        const Kv8Plan d = kv8_decode_plan(rows, kv_heads, length);
+        const Kv8Plan d = kv8_decode_plan(rows, kv_heads, dim, length);
         const Kv8Plan f = kv8_prefill_plan(rows, sequences, kv_heads, group, dim, length);
         for (const Kv8Plan& p : {d, f}) {
             REQUIRE(p.column_tiles == 1 || (p.column_tiles == 2 && dim <= 128));
@@ -110,7 +110,7 @@ void plans() {
         const int some = 1 + (int)(rng() % (fewer < sequences ? fewer : sequences));
         for (int r : {rows, fewer})
             for (int n : {length, shorter}) {
-                REQUIRE(kv8_partial_floats(kv8_decode_plan(r, kv_heads, n), r, heads, dim) <= space);
+                REQUIRE(kv8_partial_floats(kv8_decode_plan(r, kv_heads, dim, n), r, heads, dim) <= space);
                 REQUIRE(kv8_partial_floats(kv8_prefill_plan(r, some, kv_heads, group, dim, n), r, heads, dim) <= space);
             }
     }

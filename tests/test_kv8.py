@@ -503,6 +503,66 @@ def test_attention_beyond_what_is_there(torch_cuda):
     assert np.array_equal(np.isnan(got).all(2), lost)
 
 
+@FORMATS
+@pytest.mark.parametrize("dim, heads, kind", [(64, 3, F32), (128, 5, BF16), (256, 2, F32), (64, 2, F16)])
+def test_prefill_rows_before_a_nan(torch_cuda, fmt, dim, heads, kind):
+    """Rows of one work-group on both sides of a page of NaN keys, of NaN values, of no page at all, of the table's
+    end and of max_length: those before are as without it, those after are NaN."""
+    for case in ("keys", "values", "page", "table", "length"):
+        rng = np.random.default_rng(15)
+        cache = Cache(9, 1, 1, 16, dim, fmt, rng)
+        tables = np.array([[3, 1, 4, 0, 5, 8]], dtype=np.int32)
+        total, bad = 90, 48
+        fill(cache, rng, tables, [total])
+        q = rounded(rng.standard_normal((total, heads, dim)), kind)
+        scale = 1 / dim ** 0.5
+        clean = [cache.attention(0, q[i], tables[0], i + 1, scale) for i in range(total)]
+        v_max = np.abs(cache.tokens(0, 1, tables[0], total)).max()
+        longest, given = total, tables
+        if case in ("keys", "values"):
+            which = int(case == "values")
+            cache.scales[0, 0, 0, which] = np.nan
+            if fmt == E4M3:
+                cache.bytes[which][0, 0, 0] = 0x7F  # what appending NaN leaves there
+        elif case == "page":
+            given = tables.copy()
+            given[0, 3] = 9
+        elif case == "table":
+            given = np.ascontiguousarray(tables[:, :3])
+        else:
+            longest = bad
+        device = Device(torch_cuda, cache)
+        for many in (longest, 5000) if case != "length" else (longest,):
+            got = run_prefill(device, 0, q, kind, given, [0, total], [0], many, scale)
+            assert np.isnan(got[bad:]).all(), case
+            for i in (0, 15, 16, 31, 40, 46, 47):
+                check_row(got[i], *clean[i], kind, v_max, True, f"{case}, row {i}")
+
+
+def test_out_over_q(torch_cuda):
+    """The result in place of the queries, of one chunk and of several."""
+    rng = np.random.default_rng(16)
+    torch = torch_cuda
+    cache = Cache(64, 1, 2, 16, 64, INT8, rng)
+    tables = rng.integers(0, 64, (3, 300)).astype(np.int32)
+    device = Device(torch, cache)
+    q = (rng.standard_normal((3, 6, 64)) * 0.05).astype(np.float32)
+    d_tables, d_lengths = device.ints(tables), device.ints([4800, 700, 33])
+    starts, used = device.ints([0, 1, 2, 3]), device.ints([4799, 699, 32])
+    for longest in (4800, 6000):
+        want = run_decode(device, 0, q, F32, tables, [4800, 700, 33], longest, 0.125)
+        space, size = workspace_for(device, 3, 3, 6, longest)
+        x = torch.from_numpy(q.reshape(3, -1)).cuda()
+        mp.kv8_attention_decode(device.view, 0, x.data_ptr(), 384, F32, d_tables.data_ptr(), 300, d_lengths.data_ptr(),
+                                3, 6, longest, 0.125, x.data_ptr(), 384, space.data_ptr(), size)
+        assert np.array_equal(device.back(x, 384).reshape(3, 6, 64), want)
+        want = run_prefill(device, 0, q, F32, tables, [0, 1, 2, 3], [4799, 699, 32], longest, 0.125)
+        x = torch.from_numpy(q.reshape(3, -1)).cuda()
+        mp.kv8_attention_prefill(device.view, 0, x.data_ptr(), 384, F32, d_tables.data_ptr(), 300, starts.data_ptr(),
+                                 used.data_ptr(), 3, 3, 6, longest, 0.125, x.data_ptr(), 384, space.data_ptr(), size)
+        assert np.array_equal(device.back(x, 384).reshape(3, 6, 64), want)
+
+
 def test_long_context(torch_cuda):
     """70,000 tokens of which the pool holds 128 pages again and again: splits of more than one batch, positions past
     16 bits; decode and a chunk of the last rows."""

@@ -107,7 +107,8 @@ def test_bad_layers_are_refused():
     (decode, dict(heads=51, q_stride=51 * 64, out_stride=51 * 64), "at most 16"), (decode, dict(heads=0), "heads"),
     (decode, dict(max_length=-1), "max_length"), (decode, dict(max_length=(1 << 30) + 1), "max_length"),
     (decode, dict(scale=float("nan")), "scale"), (decode, dict(scale=float("inf")), "scale"),
-    (decode, dict(scale=-1.0), "scale"), (decode, dict(max_length=10000), "workspace"),
+    (decode, dict(scale=-1.0), "scale"), (decode, dict(scale=3e38), "scale"),
+    (decode, dict(rows=1 << 19), "too many"), (prefill, dict(rows=1 << 19), "too many"), (decode, dict(max_length=10000), "workspace"),
     (decode, dict(max_length=10000, workspace=P + 4, workspace_bytes=1 << 30), "aligned"),
     (decode, dict(max_length=10000, workspace=None, workspace_bytes=1 << 30), "workspace"),
     (prefill, dict(starts=None), "starts"), (prefill, dict(used=None), "used"), (prefill, dict(scale=float("nan")), "scale"),

@@ -57,7 +57,7 @@ constexpr int least_waves(int dim, int column_tiles, bool decode) {
 template <int FORMAT, int DIM, int NT, int MODE, bool DECODE>
 __global__ __launch_bounds__(64 * kKv8MostWaves) __attribute__((amdgpu_waves_per_eu(least_waves(DIM, NT, DECODE)))) void
 kv8_attention_kernel(Kv8Attention a) {
-    constexpr int kDepth = DECODE ? 2 : 1;
+    constexpr int kDepth = DECODE && DIM < 256 ? 2 : 1;
     constexpr int kSteps = DIM / 32;             // of the contraction over dims
     constexpr int kDims = DIM / 16;              // 16-dim tiles of the output
     constexpr int kParts = MODE == kTwo ? 2 : 1;  // operands of a query or probability
@@ -98,8 +98,9 @@ kv8_attention_kernel(Kv8Attention a) {
         first = ((count * group - 1) / (16 * NT) - at.index) * (16 * NT);
     }
     const int columns = count * a.group;
-    const int last = used + (min(first + kColumns * NT, columns) - 1) / a.group;  // position of the last row
-    if (used < 0 || used >= a.max_length || last >= a.max_length) {  // more than the caller allowed for
+    // Position of the last row, of those within what the caller allowed for.
+    const int last = min(used + (min(first + kColumns * NT, columns) - 1) / a.group, a.max_length - 1);
+    if (used < 0 || used >= a.max_length) {  // none is
         if (split) return;
         for (int i = threadIdx.x; i < kColumns * NT * DIM; i += blockDim.x) {
             const int column = first + i / DIM;
@@ -214,7 +215,7 @@ kv8_attention_kernel(Kv8Attention a) {
     // `k_next`: the next pair's keys, `v`: this one's values.
     const auto step = [&](int n, u4 (&k_next)[2][DIM / 64], u4 (&v)[2][DIM / 64]) {
         const uint32_t k_bits[2] = {tiles.k_bits(n, 0), tiles.k_bits(n, 1)};
-        const uint32_t v_bits[2] = {tiles.v_bits(n, 0), tiles.v_bits(n, 1)};
+        uint32_t v_bits[2] = {tiles.v_bits(n, 0), tiles.v_bits(n, 1)};
         if (MODE == kPacked) {  // the low parts' scores are 8 columns on
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -273,6 +274,20 @@ kv8_attention_kernel(Kv8Attention a) {
                         for (int i = 0; i < 4; ++i) s[t][h][i] -= by;
                 }
             }
+        }
+        // Values that are NaN: so are the columns that see the tile, and only
+        // they, since the tile's place is taken by zeros.
+        if (max(v_bits[0], v_bits[1]) >= 0x7F800000u) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (v_bits[h] >= 0x7F800000u) {
+                    v_bits[h] = 0;
+#pragma unroll
+                    for (int j = 0; j < DIM / 64; ++j) v[h][j] = u4{0, 0, 0, 0};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        if (token0 + kTile * h <= qpos[t]) l[t] = f4{1.f, 1.f, 1.f, 1.f} * quiet_nan();
+                }
         }
         // The value scale: o is held in the largest met so far.
         const uint32_t v_now = max(v_bits[0], v_bits[1]);
@@ -437,7 +452,9 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Attention a, int colu
     int row = index / a.heads, last;
     if (row >= a.rows.rows) return;
     if (DECODE) {
-        last = a.rows.used[row] - 1;
+        const int length = a.rows.used[row];
+        if (length <= a.chunk || length > a.max_length) return;
+        last = length - 1;
     } else {
         Kv8Item at;
         if (!kv8_find(a.rows, row, [](int n, int) { return n; }, &at)) return;
@@ -445,10 +462,10 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Attention a, int colu
         if (at.used < 0 || at.used >= a.max_length) return;
         const int column = at.index * a.group + head % a.group;
         const int end = min((column / columns_tile + 1) * columns_tile, at.count * a.group);
-        last = at.used + (end - 1) / a.group;  // of the work-group that had this column
+        last = min(at.used + (end - 1) / a.group, a.max_length - 1);  // of the work-group that had this column
     }
     // One chunk (or none) was stored by its work-group, as were NaN rows.
-    if (last < a.chunk || last >= a.max_length) return;
+    if (last < a.chunk) return;
     const int chunks = last / a.chunk + 1;
     const size_t at = ((size_t)row * a.heads + head) * a.splits;
     // Every wavefront finds the reference and the weights' sum, and joins its
@@ -541,12 +558,13 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
     if (wrong) return kv8_refuse(wrong);
     if (kv8_bad_ints(used) || (!decode && kv8_bad_ints(starts)))
         return kv8_refuse("8-bit attention: lengths, starts or used are missing or misaligned");
-    if (!isfinite(scale) || scale < 0) return kv8_refuse("8-bit attention: scale must be finite and not negative");
+    if (!(scale >= 0) || !isfinite((float)(scale * 1.4426950408889634074)))
+        return kv8_refuse("8-bit attention: scale must be finite (to 2.3e38) and not negative");
     if ((int64_t)rows * heads > kKv8MostColumns)
         return kv8_refuse("8-bit attention: rows times heads are too many for one call");
     if (rows == 0 || sequences == 0) return MP_OK;
     const int group = heads / cache->kv_heads;
-    const Kv8Plan p = decode ? kv8_decode_plan(rows, cache->kv_heads, max_length)
+    const Kv8Plan p = decode ? kv8_decode_plan(rows, cache->kv_heads, cache->dim, max_length)
                              : kv8_prefill_plan(rows, sequences, cache->kv_heads, group, cache->dim,
                                                 max_length);
     const size_t need = kv8_partial_floats(p, rows, heads, cache->dim) * sizeof(float);

@@ -151,8 +151,8 @@ __device__ __forceinline__ void load_queries(const Kv8Attention& a, bool f32, co
 
 // Those queries as operands: part, column tile, step 2j + h of dims 64j + 16g
 // + 8h .. +7; and the factor of a column's scores, the softmax scale over the
-// query's power of two (NaN for a row that is not finite or whose pages the
-// table has not).
+// query's power of two (NaN for a row that is not finite, longer than the
+// caller allowed for or with pages that the table has not).
 template <int DIM, int NT, int MODE, int PARTS>
 __device__ __forceinline__ void split_queries(const Kv8Attention& a, bool f32, const u4 (&raw)[NT][DIM / 64][4],
                                               const int (&qpos)[NT], int c, Half8 (&q)[PARTS][NT][DIM / 32],
@@ -175,7 +175,8 @@ __device__ __forceinline__ void split_queries(const Kv8Attention& a, bool f32, c
         amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
         const int power = min(127 + 14 - (int)(amax >> 23), 126);  // at least -113
         const float up = __uint_as_float((uint32_t)(127 + power) << 23);
-        const bool lost = amax >= 0x7F800000u || qpos[t] >> a.kv.page_shift >= a.rows.table_stride;
+        const bool lost = amax >= 0x7F800000u || qpos[t] >= a.max_length ||
+                          qpos[t] >> a.kv.page_shift >= a.rows.table_stride;
         factor[t] = lost ? quiet_nan() : a.scale * __uint_as_float((uint32_t)(127 - power) << 23);
 #pragma unroll
         for (int j = 0; j < DIM / 64; ++j)

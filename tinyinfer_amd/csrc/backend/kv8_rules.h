@@ -62,34 +62,45 @@ struct Kv8Plan {
     int column_tiles, waves, chunk, splits;
 };
 
-constexpr int kKv8Pair = 32;          // tokens of two tiles, a step of a wavefront
-constexpr int kKv8Groups = 512;       // work-groups that splitting over tokens aims at
-constexpr int kKv8LeastChunk = 128;   // tokens
+constexpr int kKv8Pair = 32;         // tokens of two tiles, a step of a wavefront
+constexpr int kKv8MostWaves = 8;     // of a work-group
+constexpr int kKv8MostGroups = 512;  // work-groups that splitting over tokens aims at
+constexpr int kKv8LeastChunk = 128;  // tokens
 
-constexpr int kKv8MostWaves = 8;  // of a work-group
-
-// Tokens a chunk and how many chunks, for `items` work-groups a chunk.
-inline void kv8_split(Kv8Plan* p, int64_t items, int max_length) {
-    const int64_t step = (int64_t)kKv8Pair * p->waves;
+// Divides `items` work-groups of up to max_length tokens.
+//
+// Alone with its columns, a work-group takes about 5.5 us and 3.9 for every
+// 1,000 tokens; splitting the tokens takes a second launch (3 to 4 us) and the
+// chip's memory rate. One row of 3 KV heads of 64, alone and split: 7.6 and
+// 9.6 us at 500 tokens, 11 and 9.9 at 1,500, 17 and 10.3 at 3,000, 119 and 13
+// at 30,000; 48 heads of rows 10.8 and 11.7 at 1,500, 15 and 12.8 at 3,000; 192
+// 17 and 20.5 at 3,000, 32 and 35 at 8,000. Half as many chunks for very few
+// work-groups: 13 instead of 16 us for the row of 30,000, but 39 instead of 32
+// for 16 of them.
+// Eight wavefronts where the work-groups leave the chip idle and each has
+// enough to join for: 17.0 instead of 18.7 us for 192 heads of 3,000 tokens,
+// 8.4 instead of 7.9 at 500; 27 instead of 25.6 for 384 heads of 3,000; dims of
+// 128 take four up to 2,048 tokens (13.9 and 13.5 at 1,500, 21.6 and 23.6 at
+// 4,096).
+inline void kv8_split(Kv8Plan* p, int64_t items, int dim, int max_length) {
     const int64_t length = max_length > 0 ? max_length : 1;
-    int64_t splits = kv8_ceil(kKv8Groups, items > 0 ? items : 1);
+    int64_t splits = 1;
+    if (items < kKv8MostGroups && length > 1024 + 40 * items) {
+        p->waves = 4;
+        splits = kv8_ceil(items < 16 ? kKv8MostGroups / 2 : kKv8MostGroups, items);
+    } else if (p->waves == 4 && items < 256 && length > (dim == 64 ? 1024 : 2048)) {
+        p->waves = 8;
+    }
+    const int64_t step = (int64_t)kKv8Pair * p->waves;
     int64_t chunk = kv8_ceil(kv8_ceil(length, splits), step) * step;
     if (chunk < kKv8LeastChunk) chunk = kKv8LeastChunk;
     p->chunk = (int)chunk;
     p->splits = (int)kv8_ceil(length, chunk);
 }
 
-// Up to 4,096 tokens a row's work-group is left alone with it: a second launch
-// to join chunks costs 3 to 4 us.
-inline Kv8Plan kv8_decode_plan(int rows, int kv_heads, int max_length) {
-    const int64_t items = (int64_t)rows * kv_heads;
+inline Kv8Plan kv8_decode_plan(int rows, int kv_heads, int dim, int max_length) {
     Kv8Plan p{1, 4, 0, 0};
-    if (max_length > 4096) {
-        kv8_split(&p, items, max_length);
-    } else {
-        if (max_length > 1024 && items < 512) p.waves = 8;
-        kv8_split(&p, kKv8Groups, max_length);
-    }
+    kv8_split(&p, (int64_t)rows * kv_heads, dim, max_length);
     return p;
 }
 
@@ -100,12 +111,23 @@ inline int64_t kv8_items(int rows, int sequences, int group, int column_tiles) {
     return by_tiles < rows * (int64_t)group ? by_tiles : rows * (int64_t)group;
 }
 
+// Two column tiles share a conversion of the codes, where that leaves
+// work-groups enough (1 and 2 tiles, us; 3 heads of 64, then 8 of 128): 18.6
+// and 20.2 for 512 rows at 1,500 tokens, 57 and 52 for 16 x 256, 445 and 365
+// at 16,000; 34 and 30 for 512 rows at 1,500, 176 and 137 for 16 x 256, 35.5
+// and 36.4 for prompts of 256. dims of 256 have no registers for two.
+// One wavefront a work-group saves the joining where there is work for the
+// chip without dealing tokens (1 and 4 wavefronts, us): 15 and 20 for 16 x 256
+// rows of prompts, 36 and 79 for the wide heads, 272 and 483 for 16.8k rows of
+// prompts of up to 2,000, but 152 and 109 for 16 x 256 rows at 4,000.
 inline Kv8Plan kv8_prefill_plan(int rows, int sequences, int kv_heads, int group, int dim, int max_length) {
-    Kv8Plan p{1, 8, 0, 0};
-    const int64_t items = kv8_items(rows, sequences, group, 1) * kv_heads;
-    if (items >= 1024) p = Kv8Plan{dim <= 128 ? 2 : 1, max_length > 2048 ? 4 : 1, 0, 0};
-    if (max_length <= 4096) kv8_split(&p, kKv8Groups, max_length);
-    else kv8_split(&p, kv8_items(rows, sequences, group, p.column_tiles) * kv_heads, max_length);
+    Kv8Plan p{1, 4, 0, 0};
+    if (dim <= 128 && max_length > 512 &&
+        kv8_items(rows, sequences, group, 1) * kv_heads * (int64_t)max_length >= 3 << 19)
+        p.column_tiles = 2;
+    const int64_t items = kv8_items(rows, sequences, group, p.column_tiles) * kv_heads;
+    if (items >= 4096 || max_length <= 64 || (max_length <= 512 && items >= kKv8MostGroups)) p.waves = 1;
+    kv8_split(&p, items, dim, max_length);
     return p;
 }
 
@@ -115,13 +137,13 @@ inline size_t kv8_partial_floats(const Kv8Plan& p, int rows, int heads, int dim)
 }
 
 // Floats that hold the partial results of any call of up to these sizes:
-// items * splits < 2 * kKv8Groups while there is more than one split.
+// items * splits < 2 * kKv8MostGroups while there is more than one split.
 inline size_t kv8_workspace_floats(int rows, int sequences, int heads, int kv_heads, int dim, int max_length) {
     (void)sequences;
     const int64_t splits = kv8_ceil(max_length > 0 ? max_length : 1, kKv8LeastChunk);
     if (splits <= 1) return 0;
     const int64_t columns = 16 * 2;  // of the largest work-group
-    const int64_t by_rows = (int64_t)rows * heads * splits, by_groups = 2ll * kKv8Groups * columns;
+    const int64_t by_rows = (int64_t)rows * heads * splits, by_groups = 2ll * kKv8MostGroups * columns;
     return (size_t)(by_rows < by_groups ? by_rows : by_groups) * (dim + 2);
 }
 
