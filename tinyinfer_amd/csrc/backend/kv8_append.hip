@@ -7,7 +7,15 @@
 // (c, g) = (l%16, l/16) owning the 16 bytes at 16 l of each 1 KB of the tile
 // (kv8.h): for keys 16 dims of slot c, for values 4 slots of dims 16 apart.
 // The maximum of a unit meets in LDS where its page has several tiles.
-// Queries are rotated by wavefronts of their own, one row each.
+// Queries are rotated by wavefronts of their own, one row each. Every
+// wavefront finds its rows from the device's metadata by itself (kv8_find).
+//
+// Bound by memory: bytes in and out (378 MB in 97 us for 16.8k BF16 rows of 32
+// query and 8 KV heads of 128, 3.9 TB/s, where a large copy reaches 4.7), and
+// for few rows by the launch and one chain of loads: metadata, table, rows
+// (4.4 us for one row of 9 and 3 heads of 64). The values' elements are read
+// one by one, 16 lanes a run, since a lane's bytes are of dims 16 apart: the
+// page's order suits the attention that reads it a thousand times.
 //
 // Arithmetic (every operation rounded on its own, so that the codes are a
 // function of the inputs alone): a' = a cos - b sin, b' = b cos + a sin; code =
@@ -400,9 +408,12 @@ __device__ __forceinline__ void rotate_rows(const AppendArgs& a, int group) {
 // keys and values of 16.8k BF16 rows of 8 heads of 128). The queries' rows go
 // beside the keys and values in one launch: 136 instead of 147 us in two for
 // those rows and their 32 query heads, read back, and 8.0 instead of 10.5 for
-// one row of 9 heads of 64.
+// one row of 9 heads of 64. What it waits for is memory: with registers for six
+// wavefronts a SIMD instead of four 127 us instead of 136, for eight (spilled)
+// 160.
 template <int TYPE, int FORMAT, int DIM>
-__global__ __launch_bounds__(512) void kv8_append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DIM <= 128 ? 6 : 4))) void kv8_append_kernel(
+    AppendArgs a) {
     __shared__ uint32_t amax_s[8];
     a.type = TYPE;
     a.format = FORMAT;
