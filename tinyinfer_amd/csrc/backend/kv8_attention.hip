@@ -26,6 +26,20 @@
 // The key scale multiplies the score with the softmax scale; the value scale,
 // as a power of two relative to the largest met so far, is applied with the
 // conversion of the value codes, where it is exact.
+//
+// What bounds it. Decode: memory, 5.3 TB/s over 256 rows of about 1,050 tokens,
+// 8 heads of 128 in E4M3 (558 MB in 106 us); rows of a few hundred tokens the
+// chain of launch, table, first tiles and joining (7.5 us for one of 503).
+// Prefill: the vector unit beside the matrix cores, 0.75 and 0.46 of a SIMD's
+// cycles for 8 x 512 FP32 rows at 8,192 (185-208 us, 0.8 PFLOP/s of products
+// counting both parts; a large FP16 matrix product reaches 1.15 here), 0.66 and
+// 0.35 for 16.8k BF16 rows of prompts (272 us, 0.7 PFLOP/s). Of about 150 vector
+// instructions a step of 32 tokens and 32 columns, 64 convert codes, 16 scale
+// scores, 16 are exponentials (four cycles each) and 32 split probabilities.
+// Hence: sums of probabilities by a matrix instruction (an operand of ones), the
+// reference raised only past 2^15, masks under a branch, one test a pair of
+// tiles, tile lookups by the lanes for 32 pairs at once instead of 90 scalar
+// instructions a pair (decode of 64 rows 14.7 -> 13.2 us).
 #include <type_traits>
 
 #include "kernels.h"
@@ -73,20 +87,8 @@ kv8_attention_kernel(Kv8Attention a) {
 
     // The work-group's columns, all of one sequence: rows row0.. and the
     // position of the first, `first` columns into the sequence's.
-    int sequence, row0, count, used, first;
-    if (DECODE) {
-        sequence = row0 = item;
-        count = 1;
-        const int length = scalar_int(a.rows.used, (uint32_t)sequence * 4u);
-        used = min(length, a.max_length + 1) - 1;
-        first = 0;
-        if (length <= 0) {  // nothing to see: zeros
-            if (split) return;
-            for (int i = threadIdx.x; i < a.group * DIM; i += blockDim.x)
-                store_one(a.out, a.type, row0 * a.out_stride + (int64_t)head * a.group * DIM + i, 0.0f);
-            return;
-        }
-    } else {
+    int sequence = item, row0 = item, count = 1, used = 0, first = 0;
+    if (!DECODE) {
         Kv8Item at;
         const int group = a.group;
         if (!kv8_find(a.rows, item, [=](int n, int) { return (n * group + 16 * NT - 1) / (16 * NT); }, &at)) return;
@@ -97,7 +99,38 @@ kv8_attention_kernel(Kv8Attention a) {
         // The last columns see the most tokens: they start first.
         first = ((count * group - 1) / (16 * NT) - at.index) * (16 * NT);
     }
-    const int columns = count * a.group;
+    const int columns = count * a.group, begin = split * a.chunk;
+    // This wavefront's pairs of tiles: pair0, + waves, ... of the chunk's.
+    const int pair0 = begin / kKv8Pair + wave;
+    int row_of[NT];  // of this lane's column in each column tile
+    int64_t q_at[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int column = min(first + 16 * t + (MODE == kPacked ? c & 7 : c), columns - 1);
+        row_of[t] = column / a.group;
+        q_at[t] = (row0 + row_of[t]) * a.q_stride + ((int64_t)head * a.group + column % a.group) * DIM;
+    }
+    // The table's first entries and the queries. A decode row's are on their
+    // way while its length is (13.2 instead of 13.5 us for 64 ragged rows).
+    const bool f32 = DECODE ? a.type == MP_TYPE_F32 : MODE == kTwo;
+    Kv8Tiles<DIM, 2> tiles;
+    int first_block;
+    u4 raw_q[NT][DIM / 64][4];
+    const auto first_loads = [&]() {
+        first_block = tiles.begin(a, sequence, head, 2 * pair0, 2 * waves, lane);
+        load_queries<DIM, NT>(a, f32, q_at, g, raw_q);
+    };
+    if (DECODE) {
+        first_loads();
+        const int length = scalar_int(a.rows.used, (uint32_t)sequence * 4u);
+        used = min(length, a.max_length + 1) - 1;
+        if (length <= 0) {  // nothing to see: zeros
+            if (split) return;
+            for (int i = threadIdx.x; i < a.group * DIM; i += blockDim.x)
+                store_one(a.out, a.type, row0 * a.out_stride + (int64_t)head * a.group * DIM + i, 0.0f);
+            return;
+        }
+    }
     // Position of the last row, of those within what the caller allowed for.
     const int last = min(used + (min(first + kColumns * NT, columns) - 1) / a.group, a.max_length - 1);
     if (used < 0 || used >= a.max_length) {  // none is
@@ -112,25 +145,16 @@ kv8_attention_kernel(Kv8Attention a) {
         }
         return;
     }
-    const int begin = split * a.chunk, end = min(begin + a.chunk, last + 1);  // tokens of this work-group
+    const int end = min(begin + a.chunk, last + 1);  // of the tokens of this work-group
     if (begin >= end) return;
     const bool alone = last < a.chunk;  // the columns' tokens are one chunk
-
-    // This lane's column in each column tile.
+    if (!DECODE) first_loads();
     int qpos[NT];
-    int64_t q_at[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int column = min(first + 16 * t + (MODE == kPacked ? c & 7 : c), columns - 1);
-        const int row = column / a.group;
-        qpos[t] = used + row;
-        q_at[t] = (row0 + row) * a.q_stride + ((int64_t)head * a.group + column % a.group) * DIM;
-    }
-
-    // This wavefront's pairs of tiles: pair0, + waves, ... of the chunk's, `n`
-    // of them done, `pairs` in all.
-    const int tile_end = (end + kTile - 1) / kTile, pair0 = begin / kKv8Pair + wave;
+    for (int t = 0; t < NT; ++t) qpos[t] = used + row_of[t];
+    const int tile_end = (end + kTile - 1) / kTile;
     const int pairs = max((tile_end + 1) / 2 - pair0 + waves - 1, 0) / waves;
+    tiles.until(tile_end, pairs);
 
     // The loop runs on pairs in two strands that do not wait for each other:
     // the scores of pair n+1 are multiplied while the probabilities of pair n
@@ -138,8 +162,6 @@ kv8_attention_kernel(Kv8Attention a) {
     // and values kDepth pairs ahead, into the registers just used up; the
     // number of loads is the same at every step, and so is what a step waits for.
     // Behind the last pair the loads are of no bytes.
-    Kv8Tiles<DIM, 2> tiles;
-    const int first_block = tiles.begin(a, sequence, head, 2 * pair0, 2 * waves, tile_end, pairs, lane);
     u4 raw_k[kDepth][2][DIM / 64], raw_v[kDepth][2][DIM / 64];
     uint64_t base[2], base_v[2];  // of the newest pair; of the one before
     int size, size_v;
@@ -152,11 +174,6 @@ kv8_attention_kernel(Kv8Attention a) {
         load_tile<DIM>(pool, at[0], bytes, lane, raw[0]);
         load_tile<DIM>(pool, at[1], bytes, lane, raw[1]);
     };
-    // The queries' loads come before those of keys and values, which wait for
-    // the table.
-    const bool f32 = DECODE ? a.type == MP_TYPE_F32 : MODE == kTwo;
-    u4 raw_q[NT][DIM / 64][4];
-    load_queries<DIM, NT>(a, f32, q_at, g, raw_q);
     {
         const auto t = tiles.find(lane / 2, first_block);
         tiles.take_places(t);

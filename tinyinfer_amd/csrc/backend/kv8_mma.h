@@ -239,10 +239,9 @@ struct Kv8Tiles {
         at_k = (__float_as_uint(t.bits.x) | t.none) & t.present;
         at_v = (__float_as_uint(t.bits.y) | t.none) & t.present;
     }
-    // The table's entries of the first steps, of a sequence whose tiles end
-    // at `end`, `count` steps of which are this wavefront's.
+    // The table's entries of the first steps.
     __device__ __forceinline__ int begin(const Kv8Attention& a, int sequence, int head, int first_tile, int tiles_on,
-                                         int end, int count, int l) {
+                                         int l) {
         table = a.rows.tables + (size_t)sequence * a.rows.table_stride;
         stride = a.rows.table_stride;
         blocks = a.kv.blocks;
@@ -253,10 +252,13 @@ struct Kv8Tiles {
         scales = a.kv.scales + (a.kv.layer * a.kv.kv_heads + head);
         tile0 = first_tile;
         step = tiles_on;
-        tile_end = end;
-        steps = count;
         lane = l;
         return find_block(lane / EACH);
+    }
+    // The tiles end at `end`, and this wavefront has `count` steps.
+    __device__ __forceinline__ void until(int end, int count) {
+        tile_end = end;
+        steps = count;
     }
     // After the first steps' tiles have been taken.
     __device__ __forceinline__ void look_ahead() {
