@@ -10,8 +10,8 @@
 // Queries are rotated by wavefronts of their own, one row each. Every
 // wavefront finds its rows from the device's metadata by itself (kv8_find).
 //
-// Bound by memory: bytes in and out (378 MB in 97 us for 16.8k BF16 rows of 32
-// query and 8 KV heads of 128, 3.9 TB/s, where a large copy reaches 4.7), and
+// Bound by memory: bytes in and out (378 MB in 101 us for 16.8k BF16 rows of 32
+// query and 8 KV heads of 128, 3.7 TB/s, where a large copy reaches 4.7), and
 // for few rows by the launch and one chain of loads: metadata, table, rows
 // (4.4 us for one row of 9 and 3 heads of 64). The values' elements are read
 // one by one, 16 lanes a run, since a lane's bytes are of dims 16 apart: the
