@@ -97,7 +97,7 @@ void plans() {
         const Kv8Plan f = kv8_prefill_plan(rows, sequences, kv_heads, group, dim, length);
         for (const Kv8Plan& p : {d, f}) {
             REQUIRE(p.column_tiles == 1 || (p.column_tiles == 2 && dim <= 128));
-            REQUIRE(p.waves >= 1 && p.waves <= 8 && p.splits >= 1 && p.splits <= 65535);
+            REQUIRE((p.waves == 1 || p.waves == 4 || p.waves == kKv8MostWaves) && p.splits >= 1 && p.splits <= 65535);
             REQUIRE(p.chunk % kKv8Pair == 0 && (int64_t)p.chunk * p.splits >= length);
         }
         REQUIRE(d.column_tiles == 1);

@@ -58,7 +58,7 @@ constexpr int join_dims(int waves, int column_tiles, int dims) {
     return fit < 1 ? 1 : fit < dims ? fit : dims;
 }
 constexpr size_t join_bytes(int waves, int column_tiles, int dims) {
-    return waves == 1 ? 0 : (size_t)waves * column_tiles * join_dims(waves <= 4 ? 4 : kKv8MostWaves, column_tiles, dims) * 1024;
+    return waves == 1 ? 0 : (size_t)waves * column_tiles * join_dims(waves, column_tiles, dims) * 1024;
 }
 
 // Wavefronts a SIMD that the registers are kept to.
@@ -237,9 +237,7 @@ kv8_attention_kernel(Kv8Attention a) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[0][h][i] += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
-                        0, __float_as_int(s[0][h][i]), 0x128, 0xF, 0xF, true));
+                for (int i = 0; i < 4; ++i) s[0][h][i] = add_across(s[0][h][i]);
         }
         const int token0 = (pair0 + n * waves) * kKv8Pair;
         // Scores in powers of two less the reference.
@@ -374,40 +372,19 @@ kv8_attention_kernel(Kv8Attention a) {
         sum[t] = l[t][0];
         if (limit[t] == -infinity() && sum[t] == sum[t]) ref[t] = -infinity();
         if (MODE == kPacked) {
-            sum[t] += __shfl_xor(sum[t], 8);
+            sum[t] = add_across(sum[t]);
 #pragma unroll
             for (int n = 0; n < kDims; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[t][n][i] += __shfl_xor(o[t][n][i], 8);
+                for (int i = 0; i < 4; ++i) o[t][n][i] = add_across(o[t][n][i]);
         }
-    }
-    float best[NT], total[NT];
-    if (waves > 1) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-            if (g == 0) ml_s[wave][t][c] = make_float2(ref[t], sum[t]);
-        __syncthreads();
     }
     // Reference and sum over the wavefronts; what turns this one's o into its
     // share of the result, as values.
-    float weight[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        best[t] = ref[t];
-        total[t] = sum[t];
-        float scaled = 1.0f;
-        if (waves > 1) {
-            best[t] = -infinity();
-            for (int w = 0; w < waves; ++w) best[t] = fmaxf(best[t], ml_s[w][t][c].x);
-            total[t] = 0.0f;
-            for (int w = 0; w < waves; ++w) {
-                const float2 ml = ml_s[w][t][c];
-                if (ml.y != 0.0f) total[t] += ml.y * __builtin_amdgcn_exp2f(ml.x - best[t]);
-            }
-            scaled = __builtin_amdgcn_exp2f(ref[t] - best[t]);
-        }
+    float best[NT], total[NT], weight[NT];
+    const auto weigh = [&](int t, float scaled) {
         weight[t] = sum[t] == 0.0f ? 0.0f : scaled / total[t] * __uint_as_float(v_top);
-    }
+    };
     const auto store = [&](int t, int n, f4 x) {
         const int column = first + 16 * t + c;
         if ((MODE == kPacked && c >= a.group) || column >= columns) return;
@@ -425,15 +402,39 @@ kv8_attention_kernel(Kv8Attention a) {
     };
     if (waves == 1) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) {
+            best[t] = ref[t];
+            total[t] = sum[t];
+            weigh(t, 1.0f);
 #pragma unroll
             for (int n = 0; n < kDims; ++n) store(t, n, o[t][n] * weight[t]);
+        }
         return;
     }
-    // The shares meet in LDS, `kAt` tiles of 16 dims at a time, the fewer the
-    // more wavefronts there are; output tiles are dealt to the wavefronts.
-    const auto join = [&](auto at_a_time) {
-        constexpr int kAt = decltype(at_a_time)::value;
+    // Four or eight wavefronts meet in LDS: first their references and sums,
+    // then their shares, join_dims tiles of 16 dims at a time; output tiles are
+    // dealt to the wavefronts. As many reads in flight as there are wavefronts.
+    const auto join = [&](auto count) {
+        constexpr int kCount = decltype(count)::value, kAt = join_dims(kCount, NT, kDims);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (g == 0) ml_s[wave][t][c] = make_float2(ref[t], sum[t]);
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float2 ml[kCount];
+#pragma unroll
+            for (int w = 0; w < kCount; ++w) ml[w] = ml_s[w][t][c];
+            best[t] = ml[0].x;
+#pragma unroll
+            for (int w = 1; w < kCount; ++w) best[t] = fmaxf(best[t], ml[w].x);
+            total[t] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kCount; ++w)
+                total[t] += ml[w].y != 0.0f ? ml[w].y * __builtin_amdgcn_exp2f(ml[w].x - best[t]) : 0.0f;
+            weigh(t, __builtin_amdgcn_exp2f(ref[t] - best[t]));
+        }
+        __syncthreads();  // the shares lie where the references did
 #pragma unroll
         for (int n0 = 0; n0 < kDims; n0 += kAt) {
             if (n0) __syncthreads();
@@ -442,18 +443,20 @@ kv8_attention_kernel(Kv8Attention a) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) o_s[(wave * kAt + n) * NT + t][lane] = o[t][n0 + n] * weight[t];
             __syncthreads();
-            for (int i = wave; i < kAt * NT; i += waves) {
-                f4 x = o_s[i][lane];
-                for (int w = 1; w < waves; ++w) x += o_s[w * kAt * NT + i][lane];
+            for (int i = wave; i < kAt * NT; i += kCount) {
+                f4 x[kCount];
+#pragma unroll
+                for (int w = 0; w < kCount; ++w) x[w] = o_s[w * kAt * NT + i][lane];
+#pragma unroll
+                for (int w = 1; w < kCount; ++w) x[0] += x[w];
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
-                    if (u == i % NT) store(u, n0 + i / NT, x);
+                    if (u == i % NT) store(u, n0 + i / NT, x[0]);
             }
         }
     };
-    __syncthreads();  // the references and sums lie where the shares will
-    if (waves <= 4) join(std::integral_constant<int, join_dims(4, NT, kDims)>());
-    else join(std::integral_constant<int, join_dims(kKv8MostWaves, NT, kDims)>());
+    if (waves == 4) join(std::integral_constant<int, 4>());
+    else join(std::integral_constant<int, kKv8MostWaves>());
 }
 
 // Joins the chunks of rows that have several: WAVES wavefronts a (row, head),

@@ -55,7 +55,7 @@ constexpr int kv8_block(const int32_t* table, int stride, int page, int blocks) 
 }
 
 // A work-group takes 16 * column_tiles columns (a column is one row's query
-// head) of a KV head and `chunk` of their tokens; its `waves` wavefronts deal
+// head) of a KV head and `chunk` of their tokens; its 1, 4 or 8 `waves` deal
 // the chunk's pairs of 16-token tiles among themselves. With more than one
 // chunk the results meet in a second launch.
 struct Kv8Plan {
