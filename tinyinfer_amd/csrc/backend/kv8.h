@@ -26,6 +26,7 @@
 
 #include "../../../include/mp_hip.h"
 #include "kv8_rules.h"
+#include "lanes.h"
 
 namespace mphip {
 
@@ -43,6 +44,50 @@ struct Kv8Layer {
 // Index of (block, head) in `scales`; its bytes follow from there.
 __device__ __forceinline__ size_t kv8_head(const Kv8Layer& kv, int block, int head) {
     return ((size_t)block * kv.layers + kv.layer) * kv.kv_heads + head;
+}
+
+// ---- across a wavefront, without a way through LDS -----------------------------
+
+// Of the four lanes (c, 0..3) of a column, by swapping rows of 16 lanes and
+// halves of the wavefront between two copies: no way through LDS.
+__device__ __forceinline__ float column_max(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ uint32_t column_max(uint32_t v) {
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)r[0], (uint32_t)r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+__device__ __forceinline__ float column_sum(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp<kDppQuadXor1>(v));
+    return column_max(row_quads_max(fmaxf(v, dpp<kDppQuadXor2>(v))));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, dpp_u<kDppQuadXor1>(v));
+    v = max(v, dpp_u<kDppQuadXor2>(v));
+    v = max(v, dpp_u<kDppRowRor4>(v));
+    return column_max(max(v, dpp_u<kDppRowRor8>(v)));
+}
+__device__ __forceinline__ float wave_sum(float v) { return column_sum(row_sum(v)); }
+// The sum over the lanes up to this one: within rows of 16, then the rows'
+// totals (row_shr 1, 2, 4, 8; row_bcast 15 and 31).
+__device__ __forceinline__ int wave_prefix(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
 }
 
 // Packed rows of sequences (mp_hip.h).
@@ -76,12 +121,7 @@ __device__ __forceinline__ bool kv8_find(const Kv8Rows& r, int item, Items items
             used = r.used[s];
             if (count > 0) n = items(count, used);
         }
-        int sum = n;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int other = __shfl_up(sum, d);
-            if (lane >= d) sum += other;
-        }
+        const int sum = wave_prefix(n);
         const uint64_t past = __builtin_amdgcn_ballot_w64(sum > item - before);
         if (past) {
             const int l = __builtin_ctzll(past);

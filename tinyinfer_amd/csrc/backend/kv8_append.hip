@@ -215,8 +215,7 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const Unit& u, 
 #pragma unroll
             for (int k = 0; k < 16; ++k) amax = max(amax, __float_as_uint(x[j][k]) & 0x7FFFFFFFu);
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
+    amax = wave_max(amax);
     if (u.tiles > 1) {  // the same in the whole launch
         if (lane == 0) amax_s[threadIdx.x >> 6] = amax;
         __syncthreads();  // also: every tile has read `held` before one changes it

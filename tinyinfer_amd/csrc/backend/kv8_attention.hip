@@ -492,15 +492,13 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Attention a, int colu
     // share of the chunks: dim/4 lanes a chunk.
     float best = -infinity();
     for (int b = lane; b < chunks; b += 64) best = fmaxf(best, a.partial_ml[at + b].x);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) best = fmaxf(best, __shfl_xor(best, d));
+    best = wave_max(best);
     float total = 0.0f;
     for (int b = lane; b < chunks; b += 64) {
         const float2 ml = a.partial_ml[at + b];
         if (ml.y != 0.0f) total += ml.y * __builtin_amdgcn_exp2f(ml.x - best);
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+    total = wave_sum(total);
     const int lanes = dim / 4, each = 64 / lanes, d4 = lane % lanes;
     f4 out = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4

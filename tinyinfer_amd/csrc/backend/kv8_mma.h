@@ -33,20 +33,6 @@ struct Kv8Attention {
 __device__ __forceinline__ float infinity() { return __builtin_inff(); }
 __device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7FC00000u); }
 
-// Of the four lanes (c, 0..3) of a column, by swapping rows of 16 lanes and
-// halves of the wavefront between two copies: no way through LDS.
-__device__ __forceinline__ float column_max(float v) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ uint32_t column_max(uint32_t v) {
-    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max((uint32_t)r[0], (uint32_t)r[1]);
-    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max((uint32_t)r[0], (uint32_t)r[1]);
-}
 // v plus its value 8 columns on.
 __device__ __forceinline__ float add_across(float v) {
     return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true));
