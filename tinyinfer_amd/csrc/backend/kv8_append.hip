@@ -185,36 +185,33 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const Unit& u, 
     for (int j = 0; j < kLoads; ++j)
 #pragma unroll
         for (int k = 0; k < 16; ++k) x[j][k] = 0.0f;
-    uint32_t amax = 0;
-    float held = 0.0f;
-    size_t index = 0;
-    if (t.block >= 0) {
-        index = kv8_head(a.kv, t.block, head);
-        if (t.kept) held = reinterpret_cast<const float*>(a.kv.scales + index)[kind];
-        if (kind == 0) {
-            if (c >= t.first && c < t.last) {
-                const int64_t at = (t.row0 + c - t.first) * stride + (int64_t)head * DIM;
+    // The rows do not wait for the table, only the held scale does.
+    if (t.found && kind == 0) {
+        if (c >= t.first && c < t.last) {
+            const int64_t at = (t.row0 + c - t.first) * stride + (int64_t)head * DIM;
 #pragma unroll
-                for (int j = 0; j < kLoads; ++j)
-                    load_rotated(src, a.type, wide, at, 64 * j + 16 * g, t.pos0 + c, a.rope, x[j]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int slot = 4 * g + i;
-                if (slot < t.first || slot >= t.last) continue;
-                const int64_t at = (t.row0 + slot - t.first) * stride + (int64_t)head * DIM + c;
-#pragma unroll
-                for (int j = 0; j < kLoads; ++j)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) x[j][4 * n + i] = load_one(src, a.type, at + 64 * j + 16 * n);
-            }
+            for (int j = 0; j < kLoads; ++j)
+                load_rotated(src, a.type, wide, at, 64 * j + 16 * g, t.pos0 + c, a.rope, x[j]);
         }
+    } else if (t.found) {
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j)
+        for (int i = 0; i < 4; ++i) {
+            const int slot = 4 * g + i;
+            if (slot < t.first || slot >= t.last) continue;
+            const int64_t at = (t.row0 + slot - t.first) * stride + (int64_t)head * DIM + c;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) amax = max(amax, __float_as_uint(x[j][k]) & 0x7FFFFFFFu);
+            for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[j][4 * n + i] = load_one(src, a.type, at + 64 * j + 16 * n);
+        }
     }
+    const size_t index = kv8_head(a.kv, max(t.block, 0), head);
+    const float held = t.kept && t.block >= 0 ? reinterpret_cast<const float*>(a.kv.scales + index)[kind] : 0.0f;
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) amax = max(amax, __float_as_uint(x[j][k]) & 0x7FFFFFFFu);
     amax = wave_max(amax);
     if (u.tiles > 1) {  // the same in the whole launch
         if (lane == 0) amax_s[threadIdx.x >> 6] = amax;
