@@ -106,8 +106,14 @@ def _bind(lib):
     return lib
 
 
+_bound = None
+
+
 def lib():
-    return _bind(library())
+    global _bound
+    if _bound is None:
+        _bound = _bind(library())
+    return _bound
 
 
 class HipBackend:

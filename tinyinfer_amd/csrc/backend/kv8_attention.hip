@@ -28,12 +28,12 @@
 // conversion of the value codes, where it is exact.
 //
 // What bounds it. Decode: memory, 5.3 TB/s over 256 rows of about 1,050 tokens,
-// 8 heads of 128 in E4M3 (558 MB in 106 us); rows of a few hundred tokens the
-// chain of launch, table, first tiles and joining (7.5 us for one of 503).
+// 8 heads of 128 in E4M3 (558 MB in 105 us); rows of a few hundred tokens the
+// chain of launch, table, first tiles and joining (6.7 us for one of 503).
 // Prefill: the vector unit beside the matrix cores, 0.75 and 0.46 of a SIMD's
-// cycles for 8 x 512 FP32 rows at 8,192 (185-208 us, 0.8 PFLOP/s of products
+// cycles for 8 x 512 FP32 rows at 8,192 (185-205 us, 0.8 PFLOP/s of products
 // counting both parts; a large FP16 matrix product reaches 1.15 here), 0.66 and
-// 0.35 for 16.8k BF16 rows of prompts (272 us, 0.7 PFLOP/s). Of about 150 vector
+// 0.35 for 16.8k BF16 rows of prompts (268-275 us, 0.7 PFLOP/s). Of about 150 vector
 // instructions a step of 32 tokens and 32 columns, 64 convert codes, 16 scale
 // scores, 16 are exponentials (four cycles each) and 32 split probabilities.
 // Hence: sums of probabilities by a matrix instruction (an operand of ones), the

@@ -69,18 +69,18 @@ constexpr int kKv8LeastChunk = 128;  // tokens
 
 // Divides `items` work-groups of up to max_length tokens.
 //
-// Alone with its columns, a work-group takes about 5.5 us and 3.9 for every
-// 1,000 tokens; splitting the tokens takes a second launch (3 to 4 us) and the
-// chip's memory rate. One row of 3 KV heads of 64, alone and split: 7.6 and
-// 9.6 us at 500 tokens, 11 and 9.9 at 1,500, 17 and 10.3 at 3,000, 119 and 13
-// at 30,000; 48 heads of rows 10.8 and 11.7 at 1,500, 15 and 12.8 at 3,000; 192
-// 17 and 20.5 at 3,000, 32 and 35 at 8,000. Half as many chunks for very few
-// work-groups: 13 instead of 16 us for the row of 30,000, but 39 instead of 32
-// for 16 of them.
+// Alone with its columns, a work-group of four wavefronts takes about 5 us and
+// 4 for every 1,000 tokens; splitting the tokens takes a second launch (2 to 3
+// us) and then the chip's memory rate. One row of 3 KV heads of 64, alone and
+// split: 6.9 and 8.5 us at 500 tokens, 10.1 and 8.8 at 1,500, 14.4 and 9.2 at
+// 3,000, 90 and 12 at 30,000; 48 heads of rows 10.1 and 10.7 at 1,500, 14.6 and
+// 11.7 at 3,000; 192 16.0 and 19.8 at 3,000, 31.5 and 35.5 at 8,000. Half as many
+// chunks for very few work-groups: 12 instead of 15 us for the row of 30,000,
+// but 39 instead of 31 for 16 of them.
 // Eight wavefronts where the work-groups leave the chip idle and each has
-// enough to join for: 17.0 instead of 18.7 us for 192 heads of 3,000 tokens,
-// 8.4 instead of 7.9 at 500; 27 instead of 25.6 for 384 heads of 3,000; dims of
-// 128 take four up to 2,048 tokens (13.9 and 13.5 at 1,500, 21.6 and 23.6 at
+// enough to join for: 16.0 instead of 18.1 us for 192 heads of 3,000 tokens,
+// 7.4 instead of 7.2 at 500; 26.6 instead of 25.0 for 384 heads of 3,000; dims of
+// 128 take four up to 2,048 tokens (13.7 and 13.6 at 1,500, 25.4 and 23.0 at
 // 4,096).
 inline void kv8_split(Kv8Plan* p, int64_t items, int dim, int max_length) {
     const int64_t length = max_length > 0 ? max_length : 1;
@@ -112,14 +112,14 @@ inline int64_t kv8_items(int rows, int sequences, int group, int column_tiles) {
 }
 
 // Two column tiles share a conversion of the codes, where that leaves
-// work-groups enough (1 and 2 tiles, us; 3 heads of 64, then 8 of 128): 18.6
-// and 20.2 for 512 rows at 1,500 tokens, 57 and 52 for 16 x 256, 445 and 365
-// at 16,000; 34 and 30 for 512 rows at 1,500, 176 and 137 for 16 x 256, 35.5
-// and 36.4 for prompts of 256. dims of 256 have no registers for two.
+// work-groups enough (1 and 2 tiles, us; 3 heads of 64, then 8 of 128): 17.3
+// and 18.0 for 512 rows at 1,500 tokens, 57 and 49 for 16 x 256, 460 and 378
+// at 16,000; 32 and 28 for 512 rows at 1,500, 187 and 134 for 16 x 256, 34.5
+// and 35.0 for prompts of 256. dims of 256 have no registers for two.
 // One wavefront a work-group saves the joining where there is work for the
-// chip without dealing tokens (1 and 4 wavefronts, us): 15 and 20 for 16 x 256
-// rows of prompts, 36 and 79 for the wide heads, 272 and 483 for 16.8k rows of
-// prompts of up to 2,000, but 152 and 109 for 16 x 256 rows at 4,000.
+// chip without dealing tokens (1 and 4 wavefronts, us): 15 and 18.5 for 16 x
+// 256 rows of prompts, 34.5 and 67 for the wide heads, 134 and 162 for those at
+// 1,500, but 149 and 107 for 16 x 256 rows of 3 heads at 4,000.
 inline Kv8Plan kv8_prefill_plan(int rows, int sequences, int kv_heads, int group, int dim, int max_length) {
     Kv8Plan p{1, 4, 0, 0};
     if (dim <= 128 && max_length > 512 &&
