@@ -758,3 +758,109 @@ def test_two_streams_with_workspaces_of_their_own(torch_cuda):
         torch.cuda.synchronize()
         for c, want in zip(calls, alone):
             assert torch.equal(c[6], want)
+
+
+def test_prefill_replayed_with_other_rows(torch_cuda):
+    """One captured prompt step (append and prefill attention of two layers) replayed for other counts: more and fewer
+    rows, sequences without any, single tokens, rows behind the last sequence left alone."""
+    torch = torch_cuda
+    service = Service(torch, INT8, F32)
+    capacity = 60
+    d = [torch.zeros((capacity, 640), device="cuda") for _ in range(2)]
+    out = [torch.zeros((capacity, 384), device="cuda") for _ in range(2)]
+    d_starts, d_used = service.device.ints([0, 0, 0, 0]), service.device.ints([0, 0, 0])
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    service.launch(d, out, d_starts, d_used, None, capacity, stream.cuda_stream)
+    stream.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        service.launch(d, out, d_starts, d_used, None, capacity, stream.cuda_stream)
+    used = np.zeros(3, dtype=np.int32)
+    for counts in ([20, 33, 7], [1, 1, 1], [0, 50, 0], [17, 0, 30], [0, 0, 0], [40, 1, 2]):
+        starts = starts_of(counts)
+        x = service.rows(capacity)
+        for a, b in zip(d, x):
+            a.copy_(torch.from_numpy(b.reshape(capacity, -1)))
+        for o in out:
+            o.fill_(7.0)
+        d_starts.copy_(torch.from_numpy(starts))
+        d_used.copy_(torch.from_numpy(used))
+        service.space.fill_(255)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        service.check(out, service.want(x, starts, used), True, f"counts {counts}")
+        service.device.check_bytes(service.cache)
+        for o in out:
+            assert bool((o[int(starts[-1]):] == 7.0).all())
+        used = used + np.array(counts, dtype=np.int32)
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_any_shape(torch_cuda, seed):
+    """Everything drawn: heads, dims, pages, formats, types, paddings, alignments, rotations, counts and lengths; three
+    steps of append and prefill, then decode, then reading back."""
+    from .kv8_reference import rotate
+    rng = np.random.default_rng(1000 + seed)
+    pick = lambda *a: a[rng.integers(len(a))]
+    kv_heads, group = int(pick(1, 2, 3, 5, 8)), int(pick(1, 2, 3, 4, 7, 8, 9, 16))
+    heads, dim, bt = kv_heads * group, int(pick(64, 64, 128, 256)), int(pick(16, 32, 64, 128))
+    fmt, kind = int(pick(INT8, E4M3)), int(pick(F32, BF16, F16))
+    pad, shift = int(pick(0, 0, 1, 4, 8)), int(pick(0, 0, 1, 4))
+    dims, interleaved = int(pick(0, dim, dim // 2, 2, 22)), bool(rng.integers(2))
+    sequences, steps = int(pick(1, 2, 5)), 3
+    counts = rng.integers(0, int(pick(2, 20, 90)), (steps, sequences)) + (rng.random((steps, sequences)) < 0.3)
+    total = counts.sum(0) + 1
+    cache = Cache(blocks_for(total, bt), 2, kv_heads, bt, dim, fmt, rng)
+    tables = tables_for(rng, cache.blocks, total, bt)
+    device = Device(torch_cuda, cache)
+    cos, sin = angles(int(total.max()) + 1, dims)
+    d_cos, d_sin = torch_cuda.from_numpy(cos).cuda(), torch_cuda.from_numpy(sin).cuda()
+    rope = mp.Rope(d_cos.data_ptr(), d_sin.data_ptr(), len(cos), dims, int(interleaved))
+    layer, scale = int(rng.integers(2)), float(rng.uniform(0.5, 1.5)) / dim ** 0.5
+    used = np.zeros(sequences, dtype=np.int32)
+    d_tables = device.ints(tables)
+    what = f"{kv_heads}x{group} dim {dim} bt {bt} fmt {fmt} type {kind} pad {pad} shift {shift} rope {dims} {interleaved}"
+    for step in range(steps + 1):
+        new = counts[step] if step < steps else np.ones(sequences, dtype=np.int64)
+        starts = starts_of(new)
+        rows = int(starts[-1]) + 1
+        q, k, v = (rounded(rng.standard_normal((rows, h, dim)) * 1.5 ** step, kind) for h in (heads, kv_heads, kv_heads))
+        mq, q_at, q_stride = device.rows(q.reshape(rows, -1), kind, pad, shift)
+        mk, k_at, k_stride = device.rows(k.reshape(rows, -1), kind, pad, shift)
+        mv, v_at, v_stride = device.rows(v.reshape(rows, -1), kind, pad, shift)
+        d_starts, d_used = device.ints(starts), device.ints(used)
+        mp.kv8_append(device.view, layer, k_at, k_stride, v_at, v_stride, kind, d_tables.data_ptr(), tables.shape[1],
+                      d_starts.data_ptr(), d_used.data_ptr(), sequences, rows, rope=rope, q=q_at, q_stride=q_stride,
+                      q_out=q_at, q_out_stride=q_stride, heads=heads)
+        cache.append(layer, k, v, tables, starts, used, (cos, sin, dims, interleaved))
+        device.check_bytes(cache)
+        turned = device.back(mq, heads * dim).reshape(rows, heads, dim)
+        for s in range(sequences):
+            for i in range(int(new[s])):
+                r, p = starts[s] + i, used[s] + i
+                want = rounded(rotate(q[r], cos[p], sin[p], dims, interleaved), kind) if dims else q[r]
+                assert np.array_equal(turned[r], want), what
+        longest = int((used + new).max()) + int(pick(0, 1, 5000))
+        if step < steps:
+            got = run_prefill(device, layer, turned, kind, tables, starts, used, longest, scale, pad, shift)
+        else:
+            got = run_decode(device, layer, turned[:sequences], kind, tables, used + 1, longest, scale, pad, shift)
+        for s in range(sequences):
+            if not new[s]:
+                continue
+            v_max = np.abs(cache.tokens(layer, 1, tables[s], int(used[s] + new[s]))).max()
+            for i in sorted({0, int(new[s]) // 2, int(new[s]) - 1}):
+                r = starts[s] + i
+                want, err = cache.attention(layer, turned[r], tables[s], int(used[s]) + i + 1, scale)
+                check_row(got[r], want, err, kind, v_max, step < steps, f"{what}: step {step}, sequence {s}, row {i}")
+        used = used + new.astype(np.int32)
+    starts = starts_of(used)
+    rows = int(starts[-1])
+    out = [device.rows(np.zeros((rows, kv_heads * dim)), kind, pad, shift) for _ in range(2)]
+    d_starts, d_used = device.ints(starts), device.ints(np.zeros(sequences))
+    mp.kv8_read(device.view, layer, d_tables.data_ptr(), tables.shape[1], d_starts.data_ptr(), d_used.data_ptr(),
+                sequences, rows, kind, out[0][1], out[0][2], out[1][1], out[1][2])
+    for which in range(2):
+        want = np.concatenate([cache.tokens(layer, which, tables[s], int(used[s])).transpose(1, 0, 2) for s in range(sequences)])
+        assert np.array_equal(device.back(out[which][0], kv_heads * dim), rounded(want.reshape(rows, -1), kind)), what
