@@ -864,3 +864,36 @@ def test_any_shape(torch_cuda, seed):
     for which in range(2):
         want = np.concatenate([cache.tokens(layer, which, tables[s], int(used[s])).transpose(1, 0, 2) for s in range(sequences)])
         assert np.array_equal(device.back(out[which][0], kv_heads * dim), rounded(want.reshape(rows, -1), kind)), what
+
+
+@FORMATS
+@pytest.mark.parametrize("dim, heads, kind", [(64, 3, F32), (64, 2, BF16), (128, 5, BF16), (256, 2, F32), (256, 16, F32)])
+def test_values_of_far_magnitudes(torch_cuda, fmt, dim, heads, kind):
+    """Pages of values up to 2^200 apart: every row is right to the largest value that it sees, whatever the pages
+    behind it hold, whether a page shares a pair of tiles with the larger one or comes pairs later."""
+    rng = np.random.default_rng(20)
+    total = 150
+    for name, powers in (("up", [-60, -30, -14, 0, 9, 30, 60, 90, 100, 110]),
+                         ("down", [100, 80, 60, 40, 20, 0, -20, -40, -60, -80]),
+                         ("leaps", [-100, 100, -100, 90, 0, 20, 101, -126, 17, 110]),
+                         ("zeros", [-200, 0, -200, -200, 7, 7, 30, -200, -200, 50])):
+        cache = Cache(10, 1, 1, 16, dim, fmt, rng)
+        tables = rng.permutation(10).astype(np.int32)[None]
+        k, v = (rng.standard_normal((total, 1, dim)).astype(np.float32) for _ in range(2))
+        for page, power in enumerate(powers):
+            v[16 * page:16 * page + 16] *= np.float32(2.0 ** power if power > -200 else 0)
+        cache.append(0, k, v, tables, [0, total], [0])
+        q = rounded(rng.standard_normal((total, heads, dim)), kind)
+        scale = 1 / dim ** 0.5
+        device = Device(torch_cuda, cache)
+        values = np.abs(cache.tokens(0, 1, tables[0], total)).max((0, 2))
+        for many in (total, 600, 60000):
+            got = run_prefill(device, 0, q, kind, tables, [0, total], [0], many, scale)
+            for i in range(total):
+                want, err = cache.attention(0, q[i], tables[0], i + 1, scale)
+                check_row(got[i], want, err, kind, values[:i + 1].max(), True, f"{name}, at most {many}, row {i}")
+        lengths = np.array([1, 15, 16, 17, 32, 40, 48, 64, 100, total], dtype=np.int32)
+        got = run_decode(device, 0, q[lengths - 1], kind, np.repeat(tables, 10, 0), lengths, total, scale)
+        for i, n in enumerate(lengths):
+            want, err = cache.attention(0, q[n - 1], tables[0], int(n), scale)
+            check_row(got[i], want, err, kind, values[:n].max(), False, f"{name}, decode of {n}")

@@ -25,7 +25,8 @@
 //   sixteenth of a BF16 output's step).
 // The key scale multiplies the score with the softmax scale; the value scale,
 // as a power of two relative to the largest met so far, is applied with the
-// conversion of the value codes, where it is exact.
+// conversion of the value codes, where it is exact (value_power; a column's
+// sums keep the largest scale that it has seen itself).
 //
 // What bounds it. Decode: memory, 5.3 TB/s over 256 rows of about 1,050 tokens,
 // 8 heads of 128 in E4M3 (558 MB in 105 us); rows of a few hundred tokens the
@@ -202,7 +203,10 @@ kv8_attention_kernel(Kv8Attention a) {
 #pragma unroll
         for (int n = 0; n < kDims; ++n) o[t][n] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    uint32_t v_top = 0;  // bits of the value scale that o is held in
+    uint32_t v_top = 0;  // bits of the largest value scale met
+    float v_held[NT];    // the scale that o is held in: the largest that the column has seen
+#pragma unroll
+    for (int t = 0; t < NT; ++t) v_held[t] = 0.0f;
     const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
     const float part_factor = MODE == kPacked && !(c & 8) ? 0.0f : -1.0f;
 
@@ -304,19 +308,44 @@ kv8_attention_kernel(Kv8Attention a) {
                         if (token0 + kTile * h <= qpos[t]) l[t] = f4{1.f, 1.f, 1.f, 1.f} * quiet_nan();
                 }
         }
-        // The value scale: o is held in the largest met so far.
-        const uint32_t v_now = max(v_bits[0], v_bits[1]);
+        // The value scale: o is held in the largest that its column has seen.
+        // Columns that end before a larger one keep theirs: they take nothing
+        // of what is converted for the others. Where the pair's second tile is
+        // far larger, the first one's codes stay as they are for the columns
+        // that end with it, and for the others its probabilities are reduced
+        // (but not in their sum).
+        uint32_t v_first = max(v_bits[0], v_top);  // what the first tile is converted to
+        const uint32_t v_now = max(v_first, v_bits[1]);
         if (v_now > v_top) {
-            if (v_top) {
-                const float keep = __uint_as_float(v_top) / __uint_as_float(v_now);
+            const bool apart = !DECODE && v_first && v_now - v_first > kApart << 23;
+            if (!apart) v_first = v_now;
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t) {
+                const bool both = DECODE || token0 + kTile <= qpos[t];
+                if (apart) {
+                    const float less = both ? (float)((v_now - v_first) >> 23) : 0.0f;
+                    float taken = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float reduced = s[t][0][i] - less;
+                        taken += __builtin_amdgcn_exp2f(s[t][0][i]) - __builtin_amdgcn_exp2f(reduced);
+                        s[t][0][i] = reduced;
+                    }
+                    taken = column_sum(taken);
+                    l[t] += f4{taken, taken, taken, taken};
+                }
+                if (DECODE || token0 <= qpos[t]) {
+                    const float to = __uint_as_float(both ? v_now : v_first), keep = v_held[t] / to;
+                    v_held[t] = to;
 #pragma unroll
                     for (int n = 0; n < kDims; ++n) o[t][n] *= keep;
+                }
             }
             v_top = v_now;
+        } else {
+            v_first = v_top;
         }
-        const Convert<FORMAT> convert0(value_power(v_bits[0], v_top)), convert1(value_power(v_bits[1], v_top));
+        const Convert<FORMAT> convert0(value_power(v_bits[0], v_first)), convert1(value_power(v_bits[1], v_top));
         base_v[0] = base[0], base_v[1] = base[1], size_v = size;
         find_pair(n + kDepth + 1);
         f4 s_next[NT][2];
@@ -383,7 +412,7 @@ kv8_attention_kernel(Kv8Attention a) {
     // share of the result, as values.
     float best[NT], total[NT], weight[NT];
     const auto weigh = [&](int t, float scaled) {
-        weight[t] = sum[t] == 0.0f ? 0.0f : scaled / total[t] * __uint_as_float(v_top);
+        weight[t] = sum[t] == 0.0f ? 0.0f : scaled / total[t] * v_held[t];
     };
     const auto store = [&](int t, int n, f4 x) {
         const int column = first + 16 * t + c;

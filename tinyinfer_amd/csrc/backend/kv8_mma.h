@@ -3,8 +3,6 @@
 #pragma once
 #include "kv8.h"
 
-
-
 namespace mphip {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -305,7 +303,14 @@ __device__ __forceinline__ void clear_past(int left, u4 (&raw)[DIM / 64]) {
     for (int j = 0; j < DIM / 64; ++j) raw[j] &= keep;
 }
 
-// A value scale as a power of two of the largest; 2^-40 of it is nothing.
+// Powers of two between the value scales of a pair of tiles up to which the
+// first is converted to the second's scale: exact in FP16 (E4M3's smallest code
+// is 2^-9, FP16's smallest number 2^-24).
+constexpr uint32_t kApart = 8;
+
+// A value scale as a power of two of the largest its columns see. Codes are
+// exact down to 2^-24 of it (E4M3: 2^-15), below that rounded to 2^-25 of it,
+// 2^-31 (2^-33) of its page's largest value; 2^-40 of it is nothing.
 __device__ __forceinline__ float value_power(uint32_t bits, uint32_t top) {
     return __uint_as_float((uint32_t)max((int)(bits - top) + (127 << 23), (127 - 40) << 23));
 }
