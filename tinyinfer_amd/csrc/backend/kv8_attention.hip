@@ -335,10 +335,13 @@ kv8_attention_kernel(Kv8Attention a) {
                     l[t] += f4{taken, taken, taken, taken};
                 }
                 if (DECODE || token0 <= qpos[t]) {
-                    const float to = __uint_as_float(both ? v_now : v_first), keep = v_held[t] / to;
-                    v_held[t] = to;
+                    const float to = __uint_as_float(both ? v_now : v_first);
+                    if (v_top) {
+                        const float keep = v_held[t] / to;
 #pragma unroll
-                    for (int n = 0; n < kDims; ++n) o[t][n] *= keep;
+                        for (int n = 0; n < kDims; ++n) o[t][n] *= keep;
+                    }
+                    v_held[t] = to;
                 }
             }
             v_top = v_now;
