@@ -897,3 +897,33 @@ def test_values_of_far_magnitudes(torch_cuda, fmt, dim, heads, kind):
         for i, n in enumerate(lengths):
             want, err = cache.attention(0, q[n - 1], tables[0], int(n), scale)
             check_row(got[i], want, err, kind, values[:n].max(), False, f"{name}, decode of {n}")
+
+
+@FORMATS
+@pytest.mark.parametrize("dim, heads", [(64, 1), (64, 16), (128, 4), (256, 2)])
+@pytest.mark.parametrize("kind", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_prefill_probabilities_are_not_rounded_to_16_bits(torch_cuda, fmt, dim, heads, kind):
+    """Tokens in turn of probability 1 and value 1, and of probability (1 + 2^-11)/2 and value -2: after an even number
+    of them the result is -2^-11 / 1.5 (to 2^-12), of which a probability rounded to FP16 leaves 0 or twice as much: off
+    by 3.3e-4 where FP32 arithmetic is by 7e-5 at most (kv8_reference.bound) and the row type's half step is 1.3e-6."""
+    total, rng = 64, np.random.default_rng(21)
+    cache = Cache(5, 1, 1, 16, dim, fmt, rng)
+    tables = np.array([[3, 0, 4, 1]], dtype=np.int32)
+    code = {x: (128 + x if fmt == INT8 else int(np.flatnonzero(VALUES[E4M3] == x)[0])) for x in (0, 1, -2)}
+    cache.scales[:] = 1
+    for page in tables[0]:
+        for which, even, odd in ((0, 0, 1), (1, 1, -2)):
+            data = cache.bytes[which][page, 0, 0]
+            data[:] = code[0]
+            data[cache.places[which][0::2, 3]] = code[even]
+            data[cache.places[which][1::2, 3]] = code[odd]
+    q = np.zeros((total, heads, dim), dtype=np.float32)
+    q[:, :, 3] = -1
+    scale = float(np.float32(np.log(2) - np.log1p(2.0 ** -11)))
+    device = Device(torch_cuda, cache)
+    for longest in (total, 1 << 20):
+        got = run_prefill(device, 0, q, kind, tables, [0, total], [0], longest, scale)
+        for i in range(total):
+            want, err = cache.attention(0, q[i], tables[0], i + 1, scale)
+            assert i % 2 == 0 or abs(want[0, 3] + 2.0 ** -11 / 1.5) < 2.0 ** -12 and err.max() < 7e-5
+            check_row(got[i], want, err, kind, 0, False, f"row {i} of {longest}")

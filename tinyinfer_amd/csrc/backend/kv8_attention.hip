@@ -19,10 +19,12 @@
 //   high and columns 8..15 the low parts of the same heads, so the second
 //   product costs nothing;
 // - kTwo: two products into the same sums;
-// - kOne: FP16 and BF16 rows: a query element is one FP16 number (2^-12 for
-//   FP16's and BF16's own bits: exact, but for elements below 2^-29 of the
-//   largest), a probability is rounded to FP16 (2^-12 of its size, a
-//   sixteenth of a BF16 output's step).
+// - kOne: FP16 and BF16 rows: a query element is one FP16 number (FP16's and
+//   BF16's own bits: exact down to 2^-39 of the largest), so the scores take
+//   one product; a probability is two, as for FP32 rows. In one FP16 number it
+//   is off by up to 2^-11 of its size, as much as an FP16 result is rounded by,
+//   and more than that where values cancel: 338 instead of 289 us for 16.8k
+//   BF16 rows of prompts keep a row as exact as the decode of it.
 // The key scale multiplies the score with the softmax scale; the value scale,
 // as a power of two relative to the largest met so far, is applied with the
 // conversion of the value codes, where it is exact (value_power; a column's
@@ -75,7 +77,7 @@ kv8_attention_kernel(Kv8Attention a) {
     constexpr int kDepth = DECODE && DIM < 256 ? 2 : 1;
     constexpr int kSteps = DIM / 32;             // of the contraction over dims
     constexpr int kDims = DIM / 16;              // 16-dim tiles of the output
-    constexpr int kParts = MODE == kTwo ? 2 : 1;  // operands of a query or probability
+    constexpr int kQueryParts = MODE == kTwo ? 2 : 1, kParts = MODE == kPacked ? 1 : 2;  // of a query, of a probability
     constexpr int kColumns = MODE == kPacked ? 8 : 16;
     static_assert(MODE != kPacked || (NT == 1 && DECODE), "one row's heads");
     extern __shared__ f4 shared_s[];  // join_bytes
@@ -187,9 +189,9 @@ kv8_attention_kernel(Kv8Attention a) {
         tiles.take_scales(t);
     }
     tiles.look_ahead();
-    Half8 q[kParts][NT][kSteps];
+    Half8 q[kQueryParts][NT][kSteps];
     float factor[NT];
-    split_queries<DIM, NT, MODE, kParts>(a, f32, raw_q, qpos, c, q, factor);
+    split_queries<DIM, NT, MODE, kQueryParts>(a, f32, raw_q, qpos, c, q, factor);
 
     // o, and the sum of the probabilities as one more row of the product with
     // the values (a matrix of ones), whose four registers are the same.
@@ -221,7 +223,7 @@ kv8_attention_kernel(Kv8Attention a) {
                 Convert<FORMAT>::plain(raw[h][i / 2][2 * (i % 2)], &k.two[0], &k.two[1]);
                 Convert<FORMAT>::plain(raw[h][i / 2][2 * (i % 2) + 1], &k.two[2], &k.two[3]);
 #pragma unroll
-                for (int part = 0; part < kParts; ++part)
+                for (int part = 0; part < kQueryParts; ++part)
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
                         to[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.all, q[part][t][i].all, to[t][h], 0, 0, 0);
@@ -364,9 +366,8 @@ kv8_attention_kernel(Kv8Attention a) {
                     const float x = __builtin_amdgcn_exp2f(s[t][h][i]), y = __builtin_amdgcn_exp2f(s[t][h][i + 1]);
                     const h2 high = {(_Float16)x, (_Float16)y};
                     if (MODE != kPacked) p[0][t].two[2 * h + i / 2] = high;
-                    if (MODE != kOne)
-                        p[kParts - 1][t].two[2 * h + i / 2] =
-                            h2{(_Float16)mix_low(high, part_factor, x), (_Float16)mix_high(high, part_factor, y)};
+                    p[kParts - 1][t].two[2 * h + i / 2] =
+                        h2{(_Float16)mix_low(high, part_factor, x), (_Float16)mix_high(high, part_factor, y)};
                 }
 #pragma unroll
         for (int part = 0; part < kParts; ++part)
