@@ -239,8 +239,10 @@ int mp_hip_paged_attention_decode_noalloc(const float* q, const float* keys, con
  *
  * What the device finds: a token whose page id is not in 0 .. blocks-1 or
  * whose page lies past table_stride is not written; an attention row that
- * needs such a page is NaN, as is one longer than max_length and one that
- * meets a NaN or an infinity in q or a NaN in the pages it sees. */
+ * needs such a page is NaN, as is one longer than max_length, one with a NaN
+ * or an infinity in q, and one that sees a NaN key or scale; one that sees a
+ * NaN among the value bytes is NaN in its dim. Rows that do not see them are
+ * as without them. */
 enum { MP_TYPE_F32 = 0, MP_TYPE_BF16 = 1, MP_TYPE_F16 = 2 };
 enum { MP_KV8_INT8 = 0, MP_KV8_E4M3 = 1 };
 

@@ -927,3 +927,80 @@ def test_prefill_probabilities_are_not_rounded_to_16_bits(torch_cuda, fmt, dim, 
             want, err = cache.attention(0, q[i], tables[0], i + 1, scale)
             assert i % 2 == 0 or abs(want[0, 3] + 2.0 ** -11 / 1.5) < 2.0 ** -12 and err.max() < 7e-5
             check_row(got[i], want, err, kind, 0, False, f"row {i} of {longest}")
+
+
+@pytest.mark.parametrize("dim, heads, kind", [(64, 3, F32), (128, 5, BF16), (256, 2, F32), (64, 16, F16), (128, 16, F32)])
+def test_nan_bytes_among_the_values(torch_cuda, dim, heads, kind):
+    """Single E4M3 NaN bytes under finite scales, anywhere in a pair of tiles: a row that sees one is NaN in its dim and
+    right in the others, one before it is right in all; alone, split, and in the batch that two column tiles take."""
+    rng = np.random.default_rng(22)
+    total, n = 90, 24
+    cache = Cache(7, 1, 1, 16, dim, E4M3, rng)
+    tables = np.array([[3, 1, 4, 0, 5, 6]], dtype=np.int32)
+    fill(cache, rng, tables, [total])
+    q = rounded(rng.standard_normal((total, heads, dim)), kind)
+    scale = 1 / dim ** 0.5
+    clean = [cache.attention(0, q[i], tables[0], i + 1, scale) for i in range(total)]
+    bad = [(17, 5, 0x7F), (18, 5, 0xFF), (31, 16, 0x7F), (32, 63, 0xFF), (47, 0, 0x7F), (48, dim - 1, 0x7F), (77, 20, 0xFF), (89, 33, 0x7F)]
+    for token, d, byte in bad:
+        cache.bytes[1][tables[0, token // 16], 0, 0, cache.places[1][token % 16, d]] = byte
+    lost = np.zeros((total, dim), dtype=bool)
+    for token, d, _ in bad:
+        lost[token:, d] = True
+    device = Device(torch_cuda, cache)
+
+    def check(got, what):
+        for i in range(total):
+            assert np.array_equal(np.isnan(got[i]), np.repeat(lost[i:i + 1], heads, 0)), f"{what}, row {i}"
+            want, err = clean[i]
+            check_row(got[i][:, ~lost[i]], want[:, ~lost[i]], err, kind, 0, False, f"{what}, row {i}")
+
+    for longest in (total, 5000, 20000):
+        check(run_prefill(device, 0, q, kind, tables, [0, total], [0], longest, scale), f"at most {longest}")
+    # Chunks behind a history, so that other tokens are the first and the last of a work-group.
+    for first in (16, 18, 47, 61):
+        got = run_prefill(device, 0, q[first:], kind, tables, [0, total - first], [first], total, scale)
+        check(np.concatenate((np.where(lost[:first, None], np.nan, [rounded(c[0], kind) for c in clean[:first]]), got)), f"from {first}")
+    many = np.arange(n + 1) * total
+    for longest in (total, 6000):
+        got = run_prefill(device, 0, np.tile(q, (n, 1, 1)), kind, np.repeat(tables, n, 0), many, [0] * n, longest, scale)
+        for s in (0, 13, n - 1):
+            check(got[many[s]:many[s + 1]], f"sequence {s} of {n}, at most {longest}")
+    lengths = np.array([17, 18, 31, 48, 77, 78, 90], dtype=np.int32)
+    for longest in (total, 5000):
+        got = run_decode(device, 0, q[lengths - 1], kind, np.repeat(tables, 7, 0), lengths, longest, scale)
+        for i, m in enumerate(lengths):
+            assert np.array_equal(np.isnan(got[i]), np.repeat(lost[m - 1:m], heads, 0))
+
+
+@FORMATS
+def test_prompt_past_the_rotation_tables(torch_cuda, fmt):
+    """A prompt that runs past the rotation tables is appended without its last rows, whose slots keep what was there:
+    the rows before them are right, those past the tables are NaN."""
+    torch, rng = torch_cuda, np.random.default_rng(23)
+    total, most, heads, dim = 60, 38, 3, 64
+    cache = Cache(5, 1, 1, 16, dim, fmt, rng)
+    if fmt == E4M3:
+        for b in cache.bytes:
+            b[rng.random(b.shape) < 0.1] = 0x7F
+    tables = np.array([[2, 0, 4, 1]], dtype=np.int32)
+    x = rng.standard_normal((total, heads + 2, dim)).astype(np.float32)
+    cos, sin = angles(most, dim)
+    device = Device(torch, cache)
+    d = torch.from_numpy(x.reshape(total, -1)).cuda()
+    d_angles = [torch.from_numpy(a).cuda() for a in (cos, sin)]
+    rope = mp.Rope(d_angles[0].data_ptr(), d_angles[1].data_ptr(), most, dim, 0)
+    ints = [device.ints(a) for a in (tables, [0, total], [0])]
+    at, width = d.data_ptr(), x.shape[1] * dim
+    mp.kv8_append(device.view, 0, at + 4 * heads * dim, width, at + 4 * (heads + 1) * dim, width, F32,
+                  ints[0].data_ptr(), 4, ints[1].data_ptr(), ints[2].data_ptr(), 1, total, rope=rope, q=at,
+                  q_stride=width, q_out=at, q_out_stride=width, heads=heads)
+    cache.append(0, x[:, heads:heads + 1], x[:, heads + 1:], tables, [0, total], [0], (cos, sin, dim, False))
+    device.check_bytes(cache)
+    turned = device.back(d, heads * dim).reshape(total, heads, dim)
+    for longest in (total, 5000):
+        got = run_prefill(device, 0, turned, F32, tables, [0, total], [0], longest, 0.125)
+        assert np.isnan(got[most:]).all()
+        for i in range(most):
+            want, err = cache.attention(0, turned[i], tables[0], i + 1, 0.125)
+            check_row(got[i], want, err, F32, 0, False, f"row {i} of {longest}")

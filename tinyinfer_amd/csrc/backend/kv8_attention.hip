@@ -209,6 +209,7 @@ kv8_attention_kernel(Kv8Attention a) {
     float v_held[NT];    // the scale that o is held in: the largest that the column has seen
 #pragma unroll
     for (int t = 0; t < NT; ++t) v_held[t] = 0.0f;
+    uint64_t nan_met = 0;  // NaN bytes among values that some columns see and others do not
     const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
     const float part_factor = MODE == kPacked && !(c & 8) ? 0.0f : -1.0f;
 
@@ -268,6 +269,9 @@ kv8_attention_kernel(Kv8Attention a) {
                 clear_past<DIM>(last + 1 - token0 - kTile - 4 * g, v[1]);
             }
         }
+        // A block of its own: in the one above dims of 256 spill 15 registers.
+        if (FORMAT == MP_KV8_E4M3 && !DECODE && token0 + kKv8Pair - 1 > used + first / a.group)
+            nan_met |= __builtin_amdgcn_ballot_w64(clear_nan<DIM>(v));
         // The reference is raised only where a score is past the limit.
         bool need = false;
         float top[NT];
@@ -395,6 +399,15 @@ kv8_attention_kernel(Kv8Attention a) {
             tiles.go_on(n + kDepth + 1);
             step(n, raw_k[(d + 1) % kDepth], raw_v[d]);
             if (++n >= pairs && d + 1 < kDepth) break;
+        }
+    }
+
+    // NaN bytes among the values: where all columns see a pair the products did
+    // it; the others are of the last 16 NT tokens, two pairs at most.
+    if (FORMAT == MP_KV8_E4M3 && !DECODE && nan_met) {
+        for (int n = max(pairs - 2, 0); n < pairs; ++n) {
+            const uint64_t at[2] = {tiles.base(n, 0), tiles.base(n, 1)};
+            spread_nan<DIM, NT>((pair0 + n * waves) * kKv8Pair + 4 * g, qpos, a.kv.values, at, lane, o);
         }
     }
 

@@ -303,6 +303,65 @@ __device__ __forceinline__ void clear_past(int left, u4 (&raw)[DIM / 64]) {
     for (int j = 0; j < DIM / 64; ++j) raw[j] &= keep;
 }
 
+// 0x80 in the bytes that are E4M3 NaNs (0x7F and 0xFF), 0 in the others.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// Makes the NaN bytes of a lane's values 0, whose product with the probability
+// of 0 of a token that a column does not see is 0; nonzero where there were any.
+template <int DIM>
+__device__ __forceinline__ uint32_t clear_nan(u4 (&raw)[2][DIM / 64]) {
+    uint32_t met = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < DIM / 16; ++n) {
+            const uint32_t is = nan_bytes(raw[h][n / 4][n % 4]);
+            raw[h][n / 4][n % 4] &= ~((is >> 7) * 0xFFu);
+            met |= is;
+        }
+    return met;
+}
+
+// o becomes NaN in the dims of the columns that see a NaN byte among the
+// values of a pair of tiles; `token`: the lane's first of the first tile's.
+// Which ones do is a product as well, of marks where bytes are NaN with marks
+// where columns see tokens.
+template <int DIM, int NT>
+__device__ __forceinline__ void spread_nan(int token, const int (&qpos)[NT], uint8_t* pool, const uint64_t (&base)[2],
+                                           int lane, f4 (&o)[NT][DIM / 16]) {
+    Half8 seen[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) seen[t].one[4 * h + i] = token + kTile * h + i <= qpos[t] ? 1 : 0;
+#pragma unroll
+    for (int j = 0; j < DIM / 64; ++j) {
+        u4 raw[2][1];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_tile<64>(pool, base[h] + 1024 * j, kTile * 64, lane, raw[h]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            Half8 marks;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // 0x80 as the FP16 number 0x2000, 2^-7
+                const uint32_t is = nan_bytes(raw[h][0][k]) >> 2;
+                marks.two[2 * h] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0u, is, 0x010C000Cu));
+                marks.two[2 * h + 1] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0u, is, 0x030C020Cu));
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const f4 none = {0.f, 0.f, 0.f, 0.f};
+                const f4 met = __builtin_amdgcn_mfma_f32_16x16x32_f16(marks.all, seen[t].all, none, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (met[i] != 0.0f) o[t][4 * j + k][i] = quiet_nan();
+            }
+        }
+    }
+}
+
 // Powers of two between the value scales of a pair of tiles up to which the
 // first is converted to the second's scale: exact in FP16 (E4M3's smallest code
 // is 2^-9, FP16's smallest number 2^-24).
