@@ -1004,3 +1004,31 @@ def test_prompt_past_the_rotation_tables(torch_cuda, fmt):
         for i in range(most):
             want, err = cache.attention(0, turned[i], tables[0], i + 1, 0.125)
             check_row(got[i], want, err, F32, 0, False, f"row {i} of {longest}")
+
+
+@FORMATS
+@pytest.mark.parametrize("power", [-126, -115])
+@pytest.mark.parametrize("dim, heads, kind", [(64, 3, F32), (128, 12, BF16), (256, 2, F32)])
+def test_values_near_the_smallest(torch_cuda, fmt, power, dim, heads, kind):
+    """Value scales of the smallest numbers over up to 20,000 tokens: the result is a normal float of the values' size,
+    and as near as for any other scale; decode and prefill, alone and split."""
+    rng = np.random.default_rng(24)
+    cache = Cache(40, 1, 1, 16, dim, fmt, rng)
+    for b in cache.bytes:  # keys of both signs, positive values
+        b[:] = rng.integers(1, 256, b.shape) if fmt == INT8 else rng.integers(0, 0x7F, b.shape)
+    cache.bytes[1][:] = rng.integers(130, 256, cache.bytes[1].shape) if fmt == INT8 else rng.integers(0x38, 0x7F, cache.bytes[1].shape)
+    cache.scales[..., 0] = 2.0 ** -9
+    cache.scales[..., 1] = 2.0 ** power
+    tables = rng.integers(0, 40, (4, 1250)).astype(np.int32)
+    lengths = [3, 64, 1000, 20000]
+    q = rounded(rng.standard_normal((4, heads, dim)) * 0.1, kind)
+    device = Device(torch_cuda, cache)
+    want = [cache.attention(0, q[i], tables[i], lengths[i], 0.1) for i in range(4)]
+    for pick, longest in (([0, 1], 64), ([0, 1, 2], 1000), ([0, 1, 2, 3], 20000)):
+        got = run_decode(device, 0, q[pick], kind, tables[pick], [lengths[i] for i in pick], longest, 0.1)
+        pre = run_prefill(device, 0, q[pick], kind, tables[pick], np.arange(len(pick) + 1), [lengths[i] - 1 for i in pick],
+                          longest, 0.1)
+        for i in pick:
+            assert np.all(want[i][0] > 2.0 ** -126.01)  # no smaller than the smallest value
+            check_row(got[i], *want[i], kind, 0, False, f"decode of {lengths[i]}, at most {longest}")
+            check_row(pre[i], *want[i], kind, 0, False, f"prefill at {lengths[i]}, at most {longest}")

@@ -426,11 +426,11 @@ kv8_attention_kernel(Kv8Attention a) {
         }
     }
     // Reference and sum over the wavefronts; what turns this one's o into its
-    // share of the result, as values.
+    // share of the result. The values' scale comes after it: their product is
+    // below the normal numbers for scales near the smallest, the result is not.
     float best[NT], total[NT], weight[NT];
-    const auto weigh = [&](int t, float scaled) {
-        weight[t] = sum[t] == 0.0f ? 0.0f : scaled / total[t] * v_held[t];
-    };
+    const auto weigh = [&](int t, float scaled) { weight[t] = sum[t] == 0.0f ? 0.0f : scaled / total[t]; };
+    const auto share = [&](int t, int n) { return o[t][n] * weight[t] * v_held[t]; };
     const auto store = [&](int t, int n, f4 x) {
         const int column = first + 16 * t + c;
         if ((MODE == kPacked && c >= a.group) || column >= columns) return;
@@ -453,7 +453,7 @@ kv8_attention_kernel(Kv8Attention a) {
             total[t] = sum[t];
             weigh(t, 1.0f);
 #pragma unroll
-            for (int n = 0; n < kDims; ++n) store(t, n, o[t][n] * weight[t]);
+            for (int n = 0; n < kDims; ++n) store(t, n, share(t, n));
         }
         return;
     }
@@ -487,7 +487,7 @@ kv8_attention_kernel(Kv8Attention a) {
 #pragma unroll
             for (int n = 0; n < kAt; ++n)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) o_s[(wave * kAt + n) * NT + t][lane] = o[t][n0 + n] * weight[t];
+                for (int t = 0; t < NT; ++t) o_s[(wave * kAt + n) * NT + t][lane] = share(t, n0 + n);
             __syncthreads();
             for (int i = wave; i < kAt * NT; i += kCount) {
                 f4 x[kCount];
