@@ -305,11 +305,12 @@ int mp_hip_kv8_attention_workspace(const mp_kv8_cache* cache, int32_t rows, int3
  * at most max_length): out = sum_t softmax_t(scale * q.k_t) v_t, query head h
  * on KV head h / (heads / kv_heads), at most 16 query heads per KV head. A
  * row of no tokens (length 0 or less) gives zeros. `scale` is finite (to
- * 2.3e38) and not negative. out may be q, with its stride. The result, before
- * it is rounded to the rows' type, is off by about 1e-6 of the largest value
- * that the row sees, as FP32 sums are; pages whose value scale is more than
- * 2^24 (INT8) or 2^15 (E4M3) below that of such a page are held to 2^-31 of
- * the largest value. Pages that a row does not see do not touch this. */
+ * 2.3e38) and not negative. out may be q, with its stride; with another one
+ * and more than one row the call is refused. The result, before it is rounded
+ * to the rows' type, is off by about 1e-6 of the largest value that the row
+ * sees, as FP32 sums are; pages whose value scale is more than 2^24 (INT8) or
+ * 2^15 (E4M3) below that of such a page are held to 2^-31 of the largest
+ * value. Pages that a row does not see do not touch this. */
 int mp_hip_kv8_attention_decode(const mp_kv8_cache* cache, int32_t layer, const void* q, int64_t q_stride,
                                 int32_t type, const int32_t* tables, int32_t table_stride, const int32_t* lengths,
                                 int32_t rows, int32_t heads, int32_t max_length, float scale, void* out,
@@ -319,8 +320,7 @@ int mp_hip_kv8_attention_decode(const mp_kv8_cache* cache, int32_t layer, const 
  * tokens 0 .. p of its sequence, all of them in the pages already (append
  * first); used[s] + the rows of s is at most max_length. Any mix of counts,
  * single tokens among them. Rows of every type have the accuracy of FP32 sums,
- * as in decode, and are rounded once, to their type. out may be q, with its
- * stride. */
+ * as in decode, and are rounded once, to their type. out may be q, as there. */
 int mp_hip_kv8_attention_prefill(const mp_kv8_cache* cache, int32_t layer, const void* q, int64_t q_stride,
                                  int32_t type, const int32_t* tables, int32_t table_stride, const int32_t* starts,
                                  const int32_t* used, int32_t sequences, int32_t rows, int32_t heads,

@@ -133,3 +133,13 @@ def test_workspace_sizes():
     size = ctypes.c_size_t()
     assert mp.lib().mp_hip_kv8_attention_workspace(cache(), 1, 1, 9, 64, None) == mp.MP_INVALID_ARGUMENT
     assert mp.lib().mp_hip_kv8_attention_workspace(None, 1, 1, 9, 64, ctypes.byref(size)) == mp.MP_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("call", [decode, prefill])
+def test_attention_over_its_queries_with_another_stride_is_refused(call):
+    """A row's output would lie over the queries of others."""
+    q = 1 << 16
+    for strides in (dict(q_stride=576, out_stride=640), dict(q_stride=640, out_stride=576)):
+        refused(lambda: call(q=q, out=q, **strides), "one stride")
+    refused(lambda: call(q=q, out=q, q_stride=640, out_stride=576, rows=2, type=mp.TYPE_BF16), "one stride")
+    call(q=q, out=q, q_stride=640, out_stride=576, rows=0)  # nothing to lie over

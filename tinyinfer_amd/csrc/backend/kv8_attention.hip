@@ -620,6 +620,8 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
     if (!wrong) wrong = kv8_wrong_matrix(q, q_stride, (int64_t)heads * cache->dim, type);
     if (!wrong) wrong = kv8_wrong_matrix(out, out_stride, (int64_t)heads * cache->dim, type);
     if (wrong) return kv8_refuse(wrong);
+    if (q == out && q_stride != out_stride && rows > 1)
+        return kv8_refuse("8-bit attention: a result in place of the queries needs one stride");
     if (kv8_bad_ints(used) || (!decode && kv8_bad_ints(starts)))
         return kv8_refuse("8-bit attention: lengths, starts or used are missing or misaligned");
     if (!(scale >= 0) || !isfinite((float)(scale * 1.4426950408889634074)))
