@@ -234,8 +234,13 @@ int mp_hip_paged_attention_decode_noalloc(const float* q, const float* keys, con
  * starts[s+1]-1 (device int32, sequences + 1 of them, not decreasing), at
  * positions used[s], used[s]+1, ... (device int32), and page table tables +
  * s*table_stride (device int32). Rows outside starts[0] .. starts[sequences]-1
- * are not touched. A sequence without rows is nothing, and neither is one to
- * append or read with used[s] outside 0 .. 2^30.
+ * are not touched. A sequence without rows is nothing. One with used[s]
+ * outside 0 .. 2^30 has no tokens: append writes and read reads none of it (an
+ * append's q_out has its queries, NaN where they are to turn). rows and
+ * sequences are at most 2^20 each. Refused as too large for a launch: attention
+ * of more than 2^22 rows times query heads; append and read of more than 2^21
+ * pages times KV heads (2^22 with 32 tokens a page, 2^23 with 16), where every
+ * sequence is taken to begin and end inside a page.
  *
  * What the device finds: a token whose page id is not in 0 .. blocks-1 or
  * whose page lies past table_stride is not written; an attention row that
@@ -276,8 +281,8 @@ typedef struct mp_rope {
  * simply appended again; a scale that the step had raised stays as it is.
  * A NaN or infinity in the new tokens makes the scale NaN, and with it the
  * head's keys (or values) of the page, until the page is written from slot 0.
- * Rows at or past rope->positions are not written, and their q_out is NaN.
- * `rope` may be NULL. k and v must not overlap the cache; sequences that
+ * Rows at or past rope->positions are not written (their slots keep what was
+ * there), and their q_out is NaN. `rope` may be NULL. k and v must not overlap the cache; sequences that
  * write must not share the page that they write. */
 int mp_hip_kv8_append(const mp_kv8_cache* cache, int32_t layer, const void* k, int64_t k_stride, const void* v,
                       int64_t v_stride, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride,
@@ -293,10 +298,11 @@ int mp_hip_kv8_read(const mp_kv8_cache* cache, int32_t layer, const int32_t* tab
                     void* k, int64_t k_stride, void* v, int64_t v_stride, void* stream);
 
 /* Bytes of workspace with which both attention calls below run `rows` rows of
- * `sequences` sequences (decode: as many as rows) of up to max_length tokens.
- * 0 is possible, and then the pointer may be NULL. A workspace holds nothing
- * between calls; calls that may overlap, replayed graphs among them, need
- * workspaces of their own. */
+ * `sequences` sequences (decode: as many as rows) of up to max_length tokens,
+ * and any of fewer or shorter ones. 0 is possible, and then the pointer may be
+ * NULL; else it is 16-byte aligned. A workspace holds nothing between calls;
+ * calls that may overlap, replayed graphs among them, need workspaces of their
+ * own. */
 int mp_hip_kv8_attention_workspace(const mp_kv8_cache* cache, int32_t rows, int32_t sequences, int32_t heads,
                                    int32_t max_length, size_t* bytes);
 

@@ -1032,3 +1032,31 @@ def test_values_near_the_smallest(torch_cuda, fmt, power, dim, heads, kind):
             assert np.all(want[i][0] > 2.0 ** -126.01)  # no smaller than the smallest value
             check_row(got[i], *want[i], kind, 0, False, f"decode of {lengths[i]}, at most {longest}")
             check_row(pre[i], *want[i], kind, 0, False, f"prefill at {lengths[i]}, at most {longest}")
+
+
+@pytest.mark.parametrize("dims", [0, 64])
+def test_append_of_sequences_without_positions(torch_cuda, dims):
+    """Sequences at positions below 0 or past 2^30 write no tokens; their queries pass, or are NaN where they turn. The
+    others are as without them."""
+    rng = np.random.default_rng(25)
+    cache = Cache(4, 1, 1, 16, 64, INT8, rng)
+    device = Device(torch_cuda, cache)
+    tables = np.array([[0, 1], [2, 3], [0, 1], [2, 2], [3, 3]], dtype=np.int32)
+    counts, used = [3, 20, 2, 2, 2], np.array([-1, 5, -2 ** 31, 2 ** 30 + 1, 2 ** 31 - 1], dtype=np.int32)
+    starts = starts_of(counts)
+    rows = int(starts[-1])
+    k, v, q = (rng.standard_normal((rows, 1, 64)).astype(np.float32) for _ in range(3))
+    cos, sin = angles(30, 64)
+    d_angles = [torch_cuda.from_numpy(a).cuda() for a in (cos, sin)]
+    rope = mp.Rope(d_angles[0].data_ptr(), d_angles[1].data_ptr(), 30, dims, 0)
+    mk, mv, mq, mo = (device.rows(x.reshape(rows, -1), F32) for x in (k, v, q, np.zeros((rows, 64))))
+    ints = [device.ints(a) for a in (tables, starts, used)]
+    mp.kv8_append(device.view, 0, mk[1], 64, mv[1], 64, F32, ints[0].data_ptr(), 2, ints[1].data_ptr(),
+                  ints[2].data_ptr(), 5, rows, rope=rope, q=mq[1], q_stride=64, q_out=mo[1], q_out_stride=64, heads=1)
+    cache.append(0, k[3:23], v[3:23], tables[1:2], [0, 20], [5], (cos, sin, dims, False))
+    device.check_bytes(cache)
+    got, inside = device.back(mo[0], 64), (np.arange(rows) >= 3) & (np.arange(rows) < 23)
+    if dims:
+        assert np.isnan(got[~inside]).all() and np.isfinite(got[inside]).all()
+    else:
+        assert np.array_equal(got, q.reshape(rows, 64))

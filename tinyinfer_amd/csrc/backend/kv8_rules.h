@@ -137,7 +137,8 @@ inline size_t kv8_partial_floats(const Kv8Plan& p, int rows, int heads, int dim)
 }
 
 // Floats that hold the partial results of any call of up to these sizes:
-// items * splits < 2 * kKv8MostGroups while there is more than one split.
+// items * splits < 2 * kKv8MostGroups while there is more than one split, for
+// any number of sequences (more of them are more items and fewer splits).
 inline size_t kv8_workspace_floats(int rows, int sequences, int heads, int kv_heads, int dim, int max_length) {
     (void)sequences;
     const int64_t splits = kv8_ceil(max_length > 0 ? max_length : 1, kKv8LeastChunk);
