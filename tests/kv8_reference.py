@@ -161,3 +161,31 @@ def rounded(x: np.ndarray, kind: int) -> np.ndarray:
     import torch
     t = {F32: torch.float32, BF16: torch.bfloat16, F16: torch.float16}[kind]
     return torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).to(t).float().numpy()
+
+
+def likely_bound(p, z, q, k, v, scale):
+    """How far FP32 arithmetic is off where its roundings have random signs, u = 2^-24 a rounding, about six standard
+    deviations. A score sums dim products of q's high and low parts: 2 dim roundings of partial sums that are about
+    |q k| (the norm of the products), and the split's 2^-23 of each, 4 sqrt(2 dim) u |q k| in all; factor and
+    reference round it again, where the difference to the reference is below 16 or as far as z is from the largest:
+    (4 |z| + 4 |z - z_max| + 16) u. A probability has that relative error, averaged over the row as if all signs were
+    the same; exp2, its split and the weights 8 u; sums over T tokens 2 sqrt(T) u. Numerator and denominator: twice."""
+    u, (tokens, dim) = 2.0 ** -24, v.shape
+    norm = np.sqrt((k ** 2) @ (q.astype(np.float64) ** 2)) * scale
+    dz = u * (4 * math.sqrt(2 * dim) * norm + 4 * np.abs(z) + 4 * np.abs(z - z.max()) + 16)
+    return 2 * (p @ dz + (2 * math.sqrt(tokens) + 8) * u) * np.abs(v).max()
+
+
+def attention_close(cache, layer, q, table, length, scale):
+    """Cache.attention with `likely_bound` in the place of the worst case."""
+    heads = q.shape[0]
+    k, v = (cache.tokens(layer, kind, table, length) for kind in range(2))
+    out, err = np.empty((heads, cache.dim)), np.empty((heads, 1))
+    for h in range(heads):
+        kh = h // (heads // cache.kv_heads)
+        z = k[kh] @ q[h].astype(np.float64) * scale
+        p = np.exp(z - z.max())
+        p /= p.sum()
+        out[h] = p @ v[kh]
+        err[h] = likely_bound(p, z, q[h], k[kh], v[kh], scale)
+    return out, err

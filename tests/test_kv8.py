@@ -8,7 +8,7 @@ import pytest
 
 from tinyinfer_amd import backend as mp
 
-from .kv8_reference import BF16, E4M3, F16, F32, INT8, VALUES, Cache, rounded
+from .kv8_reference import BF16, E4M3, F16, F32, INT8, VALUES, Cache, attention_close, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -1060,3 +1060,45 @@ def test_append_of_sequences_without_positions(torch_cuda, dims):
         assert np.isnan(got[~inside]).all() and np.isfinite(got[inside]).all()
     else:
         assert np.array_equal(got, q.reshape(rows, 64))
+
+
+def check_close(got, want, err, kind, what):
+    limit = err + HALF_STEP[kind] * np.abs(want)
+    off = np.abs(got - want)
+    assert np.all(off <= limit), f"{what}: off by {off.max():.3e}, {float((off / limit).max()):.2f} of what is allowed"
+
+
+@FORMATS
+@pytest.mark.parametrize("kv_heads, heads, dim, bt, kind, pad, shift", SHAPES)
+def test_attention_is_close(torch_cuda, fmt, kv_heads, heads, dim, bt, kind, pad, shift):
+    """Rows of ordinary data within what rounding to FP32 gives in earnest (kv8_reference.likely_bound), far below its
+    worst case: a query or a probability held in a single 16-bit number is found out
+    (test_kv8_rules.test_single_parts_are_too_far_off)."""
+    rng = np.random.default_rng(heads * dim + bt + 7)
+    lengths = [n for n in LENGTHS if n > 0]
+    cache = Cache(blocks_for(lengths, bt), 1, kv_heads, bt, dim, fmt, rng)
+    tables = tables_for(rng, cache.blocks, lengths, bt)
+    fill(cache, rng, tables, lengths)
+    device = Device(torch_cuda, cache)
+    q = rounded(rng.standard_normal((len(lengths), heads, dim)), kind)
+    scale = 1.3 / dim ** 0.5
+    rows = np.arange(len(lengths) + 1)
+    want = [attention_close(cache, 0, q[i], tables[i], n, scale) for i, n in enumerate(lengths)]
+    for longest in (777, 5000, 100000):
+        got = run_decode(device, 0, q, kind, tables, lengths, longest, scale, pad, shift)
+        pre = run_prefill(device, 0, q, kind, tables, rows, [n - 1 for n in lengths], longest, scale, pad, shift)
+        for i, n in enumerate(lengths):
+            check_close(got[i], *want[i], kind, f"decode of {n} of at most {longest}")
+            check_close(pre[i], *want[i], kind, f"prefill at {n} of at most {longest}")
+    # A whole prompt.
+    total = 129
+    cache = Cache(blocks_for([total], bt), 1, kv_heads, bt, dim, fmt, rng)
+    tables = tables_for(rng, cache.blocks, [total], bt)
+    fill(cache, rng, tables, [total])
+    device = Device(torch_cuda, cache)
+    q = rounded(rng.standard_normal((total, heads, dim)), kind)
+    for longest in (total, 100000):
+        got = run_prefill(device, 0, q, kind, tables, [0, total], [0], longest, scale, pad, shift)
+        for i in (0, 1, 2, 14, 15, 16, 17, 31, 32, 40, 63, 64, 100, 127, 128):
+            want, err = attention_close(cache, 0, q[i], tables[0], i + 1, scale)
+            check_close(got[i], want, err, kind, f"row {i} of at most {longest}")

@@ -6,9 +6,12 @@ import shutil
 import subprocess
 from pathlib import Path
 
+import numpy as np
 import pytest
 
 from tinyinfer_amd import backend as mp
+
+from .kv8_reference import E4M3, INT8, Cache, likely_bound
 
 ROOT = Path(__file__).resolve().parent.parent
 GXX = shutil.which("g++")
@@ -143,3 +146,51 @@ def test_attention_over_its_queries_with_another_stride_is_refused(call):
         refused(lambda: call(q=q, out=q, **strides), "one stride")
     refused(lambda: call(q=q, out=q, q_stride=640, out_stride=576, rows=2, type=mp.TYPE_BF16), "one stride")
     call(q=q, out=q, q_stride=640, out_stride=576, rows=0)  # nothing to lie over
+
+
+def evaluated(q, k, v, scale, q_parts, p_parts):
+    """One row's attention as FP32 sums of products with FP16 numbers: q and p as the sum of one or two of them."""
+    f = np.float32
+
+    def parts(x, n):
+        high = x.astype(np.float16).astype(f)
+        return [high, (x - high).astype(np.float16).astype(f)][:n]
+
+    up = f(2.0 ** (14 - np.floor(np.log2(np.abs(q).max()))))
+    k, v, s = k.astype(f), v.astype(f), np.zeros(len(k), dtype=f)
+    for d in range(0, len(q), 8):
+        for part in parts(q * up, q_parts):
+            s += k[:, d:d + 8] @ part[d:d + 8]
+    s *= f(scale * 1.4426950408889634) / up
+    out, total = np.zeros(v.shape[1], dtype=f), f(0)
+    for part in parts(np.exp2(s - s.max() + f(11)), p_parts):
+        for t in range(0, len(k), 32):
+            out += part[t:t + 32] @ v[t:t + 32]
+            total += part[t:t + 32].sum(dtype=f)
+    return out / total
+
+
+@pytest.mark.parametrize("fmt", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_single_parts_are_too_far_off(dim, fmt):
+    """The limit that attention is held to on the GPU (kv8_reference.likely_bound) finds out a query or a probability
+    that has lost its low part, at every dim; with both parts arithmetic in FP32 is far inside of it."""
+    rng = np.random.default_rng(dim + fmt)
+    worst = {}
+    for n in (1, 2, 15, 16, 17, 31, 32, 33, 63, 65, 127, 128, 129, 300, 777):
+        pages = -(-n // 16)
+        cache = Cache(pages, 1, 1, 16, dim, fmt, rng)
+        table = np.arange(pages, dtype=np.int32)[None]
+        k, v = (rng.standard_normal((n, 1, dim)).astype(np.float32) for _ in range(2))
+        k *= np.exp(0.5 * rng.standard_normal(dim)).astype(np.float32)
+        cache.append(0, k, v, table, [0, n], [0])
+        k, v = (cache.tokens(0, kind, table[0], n)[0] for kind in range(2))
+        for _ in range(3):
+            q, scale = rng.standard_normal(dim).astype(np.float32), 1.3 / dim ** 0.5
+            z = k @ q.astype(np.float64) * scale
+            p = np.exp(z - z.max())
+            p /= p.sum()
+            for parts in ((2, 2), (1, 2), (2, 1)):
+                off = np.abs(evaluated(q, k, v, scale, *parts) - p @ v).max() / likely_bound(p, z, q, k, v, scale)
+                worst[parts] = max(worst.get(parts, 0.0), off)
+    assert worst[2, 2] < 0.1 and worst[1, 2] > 1 and worst[2, 1] > 1, worst
