@@ -9,6 +9,7 @@ import pytest
 from tinyinfer_amd import backend as mp
 
 from .kv8_reference import BF16, E4M3, F16, F32, INT8, VALUES, Cache, attention_close, rounded
+from .kv8_sizes import WALKS
 
 pytestmark = pytest.mark.gpu
 
@@ -1102,3 +1103,32 @@ def test_attention_is_close(torch_cuda, fmt, kv_heads, heads, dim, bt, kind, pad
         for i in (0, 1, 2, 14, 15, 16, 17, 31, 32, 40, 63, 64, 100, 127, 128):
             want, err = attention_close(cache, 0, q[i], tables[0], i + 1, scale)
             check_close(got[i], want, err, kind, f"row {i} of at most {longest}")
+
+
+@pytest.mark.parametrize("walk", WALKS, ids=[w.name for w in WALKS])
+def test_wavefronts_that_walk_far(torch_cuda, walk):
+    """Every page with scales of its own and nearly equal scores, so that a page or a scale taken from another place
+    shows: calls beyond 32 and 64 steps of a wavefront, and of eight wavefronts. Lengths from half the longest on."""
+    rng = np.random.default_rng(len(walk.name) + walk.dim)
+    cache = Cache(300, 1, walk.kv_heads, walk.bt, walk.dim, walk.fmt, rng)
+    if walk.fmt == E4M3:
+        for b in cache.bytes:
+            b[(b & 127) == 127] = 0
+    for kind, low, high in ((0, -10, -7), (1, -3, 4)):
+        cache.scales[..., kind] = 2.0 ** rng.integers(low, high, cache.scales.shape[:-1]).astype(np.float32)
+    n, counts, heads = len(walk.counts), np.array(walk.counts), walk.kv_heads * walk.group
+    lengths = np.linspace(walk.longest // 2, walk.longest, n).astype(np.int32)
+    tables = rng.integers(0, 300, (n, -(-walk.longest // walk.bt))).astype(np.int32)
+    device, scale = Device(torch_cuda, cache), 1 / walk.dim ** 0.5
+    q = rounded(rng.standard_normal((int(counts.sum()), heads, walk.dim)) * 0.5, walk.kind)
+    starts = starts_of(counts)
+    if walk.decode:
+        got = run_decode(device, 0, q, walk.kind, tables, lengths, walk.longest, scale)
+    else:
+        got = run_prefill(device, 0, q, walk.kind, tables, starts, lengths - counts, walk.longest, scale)
+    assert np.isfinite(got).all()
+    for s in sorted({0, n // 3, n - 2, n - 1}):
+        for i in {0, int(counts[s]) - 1}:
+            r = starts[s] + i
+            want, err = attention_close(cache, 0, q[r], tables[s], int(lengths[s] - counts[s]) + i + 1, scale)
+            check_close(got[r], want, err, walk.kind, f"sequence {s}, row {i}")

@@ -12,6 +12,7 @@ import pytest
 from tinyinfer_amd import backend as mp
 
 from .kv8_reference import E4M3, INT8, Cache, likely_bound
+from .kv8_sizes import WALKS
 
 ROOT = Path(__file__).resolve().parent.parent
 GXX = shutil.which("g++")
@@ -194,3 +195,22 @@ def test_single_parts_are_too_far_off(dim, fmt):
                 off = np.abs(evaluated(q, k, v, scale, *parts) - p @ v).max() / likely_bound(p, z, q, k, v, scale)
                 worst[parts] = max(worst.get(parts, 0.0), off)
     assert worst[2, 2] < 0.1 and worst[1, 2] > 1 and worst[2, 1] > 1, worst
+
+
+@pytest.mark.skipif(GXX is None, reason="g++ not available")
+def test_plans_of_the_far_walks(tmp_path):
+    """The calls of kv8_sizes.py take the paths that they are there for."""
+    exe = tmp_path / "kv8_plan_of"
+    subprocess.run([GXX, "-std=c++17", "-Wall", "-Werror", f"-I{ROOT / 'tinyinfer_amd' / 'csrc' / 'backend'}",
+                    str(ROOT / "tests" / "native" / "kv8_plan_of.cpp"), "-o", str(exe)], check=True)
+    got = {}
+    for w in WALKS:
+        out = subprocess.run([str(exe), *(str(int(x)) for x in (w.decode, sum(w.counts), len(w.counts), w.kv_heads,
+                                                                w.group, w.dim, w.longest))],
+                             capture_output=True, text=True, check=True, timeout=60).stdout
+        got[w.name] = tuple(int(x) for x in out.split()[:3])
+    assert got == {w.name: w.plan for w in WALKS}
+    steps = {(w.decode, w.plan[1], w.dim): 0 for w in WALKS}
+    for w in WALKS:
+        steps[w.decode, w.plan[1], w.dim] = max(steps[w.decode, w.plan[1], w.dim], w.steps)
+    assert sum(n > 64 for n in steps.values()) >= 5 and sum(n > 32 for n in steps.values()) >= 8, steps
