@@ -48,7 +48,7 @@ struct AppendArgs {
     void* q_out;
     int64_t q_stride, q_out_stride;
     int heads, type, format;
-    bool wide[2];
+    bool k_wide;  // the keys' rows by 16 bytes (8 of 16-bit types); values are taken one by one
     bool q_by_16;  // rows, strides and the turning dims are whole 16 bytes
     int kv_groups;  // work-groups before those of the queries
 };
@@ -179,7 +179,6 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const Unit& u, 
     const int head = u.head, kind = u.kind;
     const void* const src = kind ? a.x[1] : a.x[0];
     const int64_t stride = kind ? a.x_stride[1] : a.x_stride[0];
-    const bool wide = kind ? a.wide[1] : a.wide[0];
     float x[kLoads][16];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
@@ -191,7 +190,7 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const Unit& u, 
             const int64_t at = (t.row0 + c - t.first) * stride + (int64_t)head * DIM;
 #pragma unroll
             for (int j = 0; j < kLoads; ++j)
-                load_rotated(src, a.type, wide, at, 64 * j + 16 * g, t.pos0 + c, a.rope, x[j]);
+                load_rotated(src, a.type, a.k_wide, at, 64 * j + 16 * g, t.pos0 + c, a.rope, x[j]);
         }
     } else if (t.found) {
 #pragma unroll
@@ -429,7 +428,7 @@ struct ReadArgs {
     void* x[2];
     int64_t x_stride[2];
     int type, format;
-    bool wide[2];
+    bool k_wide;
 };
 
 template <int TYPE, int FORMAT, int DIM>
@@ -444,7 +443,6 @@ __global__ __launch_bounds__(512) void kv8_read_kernel(ReadArgs a) {
     const int head = u.head, kind = u.kind;
     void* const dst = kind ? a.x[1] : a.x[0];
     const int64_t stride = kind ? a.x_stride[1] : a.x_stride[0];
-    const bool wide = kind ? a.wide[1] : a.wide[0];
     const size_t index = kv8_head(a.kv, max(t.block, 0), head);
     const float scale =
         t.block >= 0 ? reinterpret_cast<const float*>(a.kv.scales + index)[kind] : quiet_nan();
@@ -459,7 +457,7 @@ __global__ __launch_bounds__(512) void kv8_read_kernel(ReadArgs a) {
             const int64_t at = (t.row0 + c - t.first) * stride + (int64_t)head * DIM + 64 * j + 16 * g;
 #pragma unroll
             for (int n = 0; n < 4; ++n)
-                store_four(dst, a.type, wide, at + 4 * n, decode(byte_of(w[n], 0), a.format) * scale,
+                store_four(dst, a.type, a.k_wide, at + 4 * n, decode(byte_of(w[n], 0), a.format) * scale,
                            decode(byte_of(w[n], 1), a.format) * scale, decode(byte_of(w[n], 2), a.format) * scale,
                            decode(byte_of(w[n], 3), a.format) * scale);
         } else {
@@ -551,7 +549,7 @@ extern "C" int mp_hip_kv8_append(const mp_kv8_cache* cache, int32_t layer, const
         a.q = q, a.q_out = q_out;
         a.q_stride = q_stride, a.q_out_stride = q_out_stride;
         a.heads = heads, a.type = type, a.format = cache->format;
-        a.wide[0] = kv8_wide(k, k_stride, type), a.wide[1] = kv8_wide(v, v_stride, type);
+        a.k_wide = kv8_wide(k, k_stride, type);
         const int per16 = 16 / (int)kv8_element(type);
         a.q_by_16 = q && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0 &&
                     q_stride % per16 == 0 && q_out_stride % per16 == 0 &&
@@ -594,7 +592,7 @@ extern "C" int mp_hip_kv8_read(const mp_kv8_cache* cache, int32_t layer, const i
         a.x[0] = k, a.x[1] = v;
         a.x_stride[0] = k_stride, a.x_stride[1] = v_stride;
         a.type = type, a.format = cache->format;
-        a.wide[0] = kv8_wide(k, k_stride, type), a.wide[1] = kv8_wide(v, v_stride, type);
+        a.k_wide = kv8_wide(k, k_stride, type);
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const StreamDevice device(s);
         if (device.status != hipSuccess) return kv8_done(device.status, "8-bit read: device of the stream");
