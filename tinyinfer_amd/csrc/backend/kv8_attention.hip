@@ -23,22 +23,23 @@
 //   BF16's own bits: exact down to 2^-39 of the largest), so the scores take
 //   one product; a probability is two, as for FP32 rows. In one FP16 number it
 //   is off by up to 2^-11 of its size, as much as an FP16 result is rounded by,
-//   and more than that where values cancel: 338 instead of 289 us for 16.8k
-//   BF16 rows of prompts keep a row as exact as the decode of it.
+//   and more than that where values cancel: 331-339 instead of 269-280 us for
+//   16.8k BF16 rows of prompts keep a row as exact as the decode of it.
 // The key scale multiplies the score with the softmax scale; the value scale,
 // as a power of two relative to the largest met so far, is applied with the
 // conversion of the value codes, where it is exact (value_power; a column's
 // sums keep the largest scale that it has seen itself).
 //
 // What bounds it. Decode: memory, 5.3 TB/s over 256 rows of about 1,050 tokens,
-// 8 heads of 128 in E4M3 (558 MB in 105 us); rows of a few hundred tokens the
-// chain of launch, table, first tiles and joining (6.7 us for one of 503).
-// Prefill: the vector unit beside the matrix cores, 0.75 and 0.46 of a SIMD's
-// cycles for 8 x 512 FP32 rows at 8,192 (185-205 us, 0.8 PFLOP/s of products
-// counting both parts; a large FP16 matrix product reaches 1.15 here), 0.66 and
-// 0.35 for 16.8k BF16 rows of prompts (268-275 us, 0.7 PFLOP/s). Of about 150 vector
-// instructions a step of 32 tokens and 32 columns, 64 convert codes, 16 scale
-// scores, 16 are exponentials (four cycles each) and 32 split probabilities.
+// 8 heads of 128 in E4M3 (558 MB in 105 us, 564 MB by the counters); rows of a
+// few hundred tokens the chain of launch, table, first tiles and joining (6.9 us
+// for one of 503).
+// Prefill: the vector unit beside the matrix cores, 0.76 and 0.46 of a SIMD's
+// cycles for 8 x 512 FP32 rows at 8,192 (186-210 us, 0.8 PFLOP/s of products
+// counting both parts; a large FP16 matrix product reaches 1.15 here), 0.68 and
+// 0.46 for 16.8k BF16 rows of prompts (331-339 us, 0.84 PFLOP/s). Of about 150
+// vector instructions a step of 32 tokens and 32 columns, 64 convert codes, 16
+// scale scores, 16 are exponentials (four cycles each) and 32 split probabilities.
 // Hence: sums of probabilities by a matrix instruction (an operand of ones), the
 // reference raised only past 2^15, masks under a branch, one test a pair of
 // tiles, tile lookups by the lanes for 32 pairs at once instead of 90 scalar

@@ -87,6 +87,10 @@ union Half8 {
 __device__ __forceinline__ int scalar_int(const void* p, uint32_t offset) {
     return *(const __attribute__((address_space(4))) int32_t*)((uintptr_t)p + offset);
 }
+// In asm, as are the two below (the compiler makes two or three instructions of
+// them, 32 more a step). It puts no waits around asm: what these read comes
+// from ordinary vector instructions, exponentials by way of the conversion to
+// `half`, never straight from an exponential or a matrix instruction.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));

@@ -82,6 +82,11 @@ constexpr int kKv8LeastChunk = 128;  // tokens
 // 7.4 instead of 7.2 at 500; 26.6 instead of 25.0 for 384 heads of 3,000; dims of
 // 128 take four up to 2,048 tokens (13.7 and 13.6 at 1,500, 25.4 and 23.0 at
 // 4,096).
+// What it does not see is which rows are long: from kKv8MostGroups work-groups
+// on, and below 1,024 + 40 x work-groups tokens, a row that is far longer than
+// the others is walked by one work-group a head. One of 8,000 tokens among 64
+// rows, the others of 300: 29 us with 3 heads of 64, 53 with 8 of 128, where the
+// long row alone takes 11 and 12; one of 32,000 among 64 rows of 8 heads 178, alone 20.
 inline void kv8_split(Kv8Plan* p, int64_t items, int dim, int max_length) {
     const int64_t length = max_length > 0 ? max_length : 1;
     int64_t splits = 1;
@@ -112,14 +117,20 @@ inline int64_t kv8_items(int rows, int sequences, int group, int column_tiles) {
 }
 
 // Two column tiles share a conversion of the codes, where that leaves
-// work-groups enough (1 and 2 tiles, us; 3 heads of 64, then 8 of 128): 17.3
-// and 18.0 for 512 rows at 1,500 tokens, 57 and 49 for 16 x 256, 460 and 378
-// at 16,000; 32 and 28 for 512 rows at 1,500, 187 and 134 for 16 x 256, 34.5
-// and 35.0 for prompts of 256. dims of 256 have no registers for two.
-// One wavefront a work-group saves the joining where there is work for the
-// chip without dealing tokens (1 and 4 wavefronts, us): 15 and 18.5 for 16 x
-// 256 rows of prompts, 34.5 and 67 for the wide heads, 134 and 162 for those at
-// 1,500, but 149 and 107 for 16 x 256 rows of 3 heads at 4,000.
+// work-groups enough: from 1.5 million (3 << 19) work-groups of one tile times
+// tokens on, six thousand a CU, between 0.6 and 2 million where both sides were
+// measured (1 and 2 tiles, us; 3 heads of 64 in FP32, then 8 of 128 in BF16):
+// 17.3 and 18.0 for 512 rows at 1,500 tokens (0.6 million), 57 and 49 for 16 x
+// 256 (4 million), 460 and 378 at 16,000; 37 and 34 for 512 rows at 1,500 (2
+// million), 219 and 174 for 16 x 256. Up to 512 tokens there is no more than
+// the one walk to share: 38.6 and 39.4 for prompts of 256 (2 million). dims of
+// 256 have no registers for two.
+// One wavefront a work-group saves the joining where there is work for the chip
+// without dealing tokens: from 4,096 work-groups on (four a SIMD), from 512 on
+// (two a CU) up to 512 tokens (16 steps), and where there are two steps to deal (1
+// and 4 wavefronts, us): 15 and 18.5 for 16 x 256 rows of prompts, 39 and 71 for
+// the wide heads, 174 and 201 for those at 1,500, but 149 and 107 for 16 x 256
+// rows of 3 heads at 4,000 (1,200 work-groups).
 inline Kv8Plan kv8_prefill_plan(int rows, int sequences, int kv_heads, int group, int dim, int max_length) {
     Kv8Plan p{1, 4, 0, 0};
     if (dim <= 128 && max_length > 512 &&
