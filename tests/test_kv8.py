@@ -1132,3 +1132,33 @@ def test_wavefronts_that_walk_far(torch_cuda, walk):
             r = starts[s] + i
             want, err = attention_close(cache, 0, q[r], tables[s], int(lengths[s] - counts[s]) + i + 1, scale)
             check_close(got[r], want, err, walk.kind, f"sequence {s}, row {i}")
+
+
+@pytest.mark.parametrize("walk", [w for w in WALKS if w.fmt == E4M3 and not w.decode and max(w.counts) > 1],
+                         ids=lambda w: w.name)
+def test_nan_bytes_at_the_end_of_a_far_walk(torch_cuda, walk):
+    """NaN bytes among the values of each sequence's last page, which only some of its last rows see, behind walks whose
+    tile places have been exchanged: NaN in those rows' dims and nowhere else."""
+    rng = np.random.default_rng(26 + walk.dim)
+    n, counts, heads = len(walk.counts), np.array(walk.counts), walk.kv_heads * walk.group
+    cache = Cache(100 + n, 1, walk.kv_heads, walk.bt, walk.dim, E4M3, rng)
+    for b in cache.bytes:
+        b[(b & 127) == 127] = 0
+    cache.scales[:] = 2.0 ** -9
+    lengths = np.linspace(walk.longest - 40, walk.longest, n).astype(np.int32)
+    tables = rng.integers(0, 100, (n, -(-walk.longest // walk.bt))).astype(np.int32)
+    lost = np.zeros((int(counts.sum()), walk.kv_heads, walk.dim), dtype=bool)
+    starts = starts_of(counts)
+    for s in range(n):
+        page = (lengths[s] - 1) // walk.bt
+        tables[s, page] = 100 + s
+        for _ in range(4):
+            slot, head, d = rng.integers(lengths[s] - page * walk.bt), rng.integers(walk.kv_heads), rng.integers(walk.dim)
+            cache.bytes[1][100 + s, 0, head, cache.places[1][slot, d]] = rng.choice([0x7F, 0xFF])
+            first = max(page * walk.bt + slot - (lengths[s] - counts[s]), 0)  # row that is the first to see it
+            lost[starts[s] + first:starts[s + 1], head, d] = True
+    device = Device(torch_cuda, cache)
+    q = rounded(rng.standard_normal((int(counts.sum()), heads, walk.dim)) * 0.5, walk.kind)
+    got = run_prefill(device, 0, q, walk.kind, tables, starts, lengths - counts, walk.longest, 1 / walk.dim ** 0.5)
+    assert lost.any() and not lost.all()
+    assert np.array_equal(np.isnan(got), np.repeat(lost, walk.group, 1))
