@@ -282,8 +282,8 @@ typedef struct mp_rope {
  * A NaN or infinity in the new tokens makes the scale NaN, and with it the
  * head's keys (or values) of the page, until the page is written from slot 0.
  * Rows at or past rope->positions are not written (their slots keep what was
- * there), and their q_out is NaN. `rope` may be NULL. k and v must not overlap the cache; sequences that
- * write must not share the page that they write. */
+ * there), and their q_out is NaN. `rope` may be NULL. k and v must not overlap
+ * the cache; sequences that write must not share the page that they write. */
 int mp_hip_kv8_append(const mp_kv8_cache* cache, int32_t layer, const void* k, int64_t k_stride, const void* v,
                       int64_t v_stride, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride,
                       int32_t heads, int32_t type, const mp_rope* rope, const int32_t* tables, int32_t table_stride,

@@ -86,7 +86,8 @@ constexpr int kKv8LeastChunk = 128;  // tokens
 // on, and below 1,024 + 40 x work-groups tokens, a row that is far longer than
 // the others is walked by one work-group a head. One of 8,000 tokens among 64
 // rows, the others of 300: 29 us with 3 heads of 64, 53 with 8 of 128, where the
-// long row alone takes 11 and 12; one of 32,000 among 64 rows of 8 heads 178, alone 20.
+// long row alone takes 11 and 12; one of 32,000 among 64 rows of 8 heads 178,
+// alone 20.
 inline void kv8_split(Kv8Plan* p, int64_t items, int dim, int max_length) {
     const int64_t length = max_length > 0 ? max_length : 1;
     int64_t splits = 1;
