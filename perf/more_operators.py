@@ -6,8 +6,8 @@
 - "product": rows of floats or of 8 bits times a 4-bit matrix, alone or as the gated pair silu(x G^T) * (x W^T).
 
 A 4-bit weight is an E2M1 number times the power of two of its group, 32 weights along a row. An element of an 8-bit
-row is an E4M3 number times the power of two of its group of 32. A scale byte b stands for 2^(b - 127): the smallest
-power, from 2^-100 on, with which the group's largest magnitude is in range (6 and 448).
+row is a whole number, -127 to 127, times the power of two of its group of 32. A scale byte b stands for 2^(b - 127):
+the smallest power, from 2^-100 on, with which the group's largest magnitude is in range (6 and 127).
 
 Order of a matrix's bytes: codes by tiles of 16 rows and 128 columns, [rows/16][columns/128][columns%128/32][rows%16]
 [16 bytes], a byte holding an even column in its low half and the next in its high half; scales [rows/16][columns/512]
@@ -38,7 +38,7 @@ def _pack(name, n, k, dtype):
 
 
 def _product(name, rows, k, n, x, out, gated=False):
-    """x: the rows' type, "mx8" for 8 bits; out: the results'."""
+    """x: the rows' type, "i8" for 8 bits; out: the results'."""
     return dict(name=name, kind="product", rows=rows, n=n, k=k, x=x, out=out, gated=gated)
 
 
@@ -49,7 +49,7 @@ def listed():
         # The final norm of a batch whose rows are not a multiple of anything, without a residual.
         _norm("norm_odd", 777, 2047, "f16", "f16", False),
         # Prompts of a wider model packed in one batch, to rows of 8 bits for the products behind it.
-        _norm("norm_prompts", 4096, 4096, "bf16", "mx8"),
+        _norm("norm_prompts", 4096, 4096, "bf16", "i8"),
         # The attention's output of a decode step of 64 sequences, to 8 bits for the projection.
         _convert("convert_64", 64, 576, "f32"),
         # The same of packed prompts in a wider model.
@@ -67,7 +67,7 @@ def listed():
         # The last, ragged chunk of a prompt, query, key and value projections in one.
         _product("qkv_203", 203, 576, 960, "f32", "f32"),
         # Packed prompts through a wider model's gated pair, 8 bits in and out: the matrix cores are what counts.
-        _product("gated_prompts", 4096, 4096, 12288, "mx8", "mx8", True),
+        _product("gated_prompts", 4096, 4096, 12288, "i8", "i8", True),
     ]
 
 
@@ -79,18 +79,18 @@ def _drawn(rng):
     dtype = rng.choice(["f32", "bf16", "f16"])
     pick = rng.random()
     if pick < 0.25:
-        out = rng.choice([dtype, dtype, "mx8", rng.choice(["f32", "bf16", "f16"])])
-        width = 32 * _log(rng, 1, 512) if out == "mx8" else _log(rng, 1, 16384)
+        out = rng.choice([dtype, dtype, "i8", rng.choice(["f32", "bf16", "f16"])])
+        width = 32 * _log(rng, 1, 512) if out == "i8" else _log(rng, 1, 16384)
         return _norm("", _log(rng, 1, 16384), width, dtype, out, rng.random() < 0.6)
     if pick < 0.35:
         return _convert("", _log(rng, 1, 16384), 32 * _log(rng, 1, 512), dtype)
     if pick < 0.45:
         return _pack("", _log(rng, 1, 50000), 32 * _log(rng, 1, 512), dtype)
-    x = rng.choice([dtype, "mx8"])
+    x = rng.choice([dtype, "i8"])
     gated = rng.random() < 0.4
     # A row of 8 bits out of a product is what the gated pair gives the next one.
-    out = "mx8" if gated and rng.random() < 0.4 else dtype
-    n = 32 * _log(rng, 1, 512) if out == "mx8" else _log(rng, 1, 50000)
+    out = "i8" if gated and rng.random() < 0.4 else dtype
+    n = 32 * _log(rng, 1, 512) if out == "i8" else _log(rng, 1, 50000)
     rows = _log(rng, 1, 300) if rng.random() < 0.6 else _log(rng, 1, 5000)
     return _product("", rows, 32 * _log(rng, 1, 512), n, x, out, gated)
 
@@ -113,7 +113,7 @@ def draw(rng):
 
 
 def _size(dtype):
-    return {"f32": 4, "bf16": 2, "f16": 2, "mx8": 1 + 1 / 32}[dtype]
+    return {"f32": 4, "bf16": 2, "f16": 2, "i8": 1 + 1 / 32}[dtype]
 
 
 def work(case):
@@ -121,17 +121,17 @@ def work(case):
     if kind == "norm":
         n = case["rows"] * case["width"]
         each = _size(case["dtype"]) * (3 if case["residual"] else 1) + _size(case["out"])
-        back = _size("mx8") + 4 if case["out"] == "mx8" else 0  # read back as floats
+        back = _size("i8") + 4 if case["out"] == "i8" else 0  # read back as floats
         return {"bytes": n * (each + back) + 4 * case["width"], "flops": 5 * n}
     if kind == "convert":
         n = case["rows"] * case["width"]
-        return {"bytes": n * 2 * (_size(case["dtype"]) + _size("mx8")), "flops": 3 * n}
+        return {"bytes": n * 2 * (_size(case["dtype"]) + _size("i8")), "flops": 3 * n}
     if kind == "pack":
         n = case["n"] * case["k"]
         return {"bytes": n * 2 * (_size(case["dtype"]) + 17 / 32), "flops": 3 * n}
     matrices = 2 if case["gated"] else 1
     rows, n, k = case["rows"], case["n"], case["k"]
-    back = rows * n * (_size("mx8") + 2) if case["out"] == "mx8" else 0
+    back = rows * n * (_size("i8") + 2) if case["out"] == "i8" else 0
     return {"bytes": matrices * n * k * 17 / 32 + rows * k * _size(case["x"]) + rows * n * _size(case["out"]) + back,
             "flops": 2 * matrices * rows * n * k}
 
@@ -151,28 +151,20 @@ def _power(scales, dtype):
     return torch.ldexp(torch.ones((), dtype=dtype, device=scales.device), scales.int() - 127)
 
 
-def _nearest8(x):
-    """x, within 448, rounded to E4M3 numbers, ties to even, in x's own precision."""
-    _, exponent = torch.frexp(x)
-    step = (exponent - 4).clamp(min=-9)
-    one = torch.ones((), dtype=x.dtype, device=x.device)
-    return torch.round(x * torch.ldexp(one, -step)) * torch.ldexp(one, step)
-
-
 def _to_rows8(x):
     """Rows of 8 bits of x [rows, width]: codes, scale bytes in rows of whole words."""
     rows, width = x.shape
     groups = x.reshape(rows, width // 32, 32)
-    scales = _scale_bytes(groups.abs().amax(-1), 0.875, 9)
-    codes = _nearest8(groups / _power(scales, x.dtype)[..., None])
+    scales = _scale_bytes(groups.abs().amax(-1), 0.9921875, 7)
+    codes = torch.round(groups / _power(scales, x.dtype)[..., None])
     padded = torch.zeros((rows, -(-width // 128) * 4), dtype=torch.uint8, device=x.device)
     padded[:, :width // 32] = scales
-    return codes.float().to(torch.float8_e4m3fn).view(torch.uint8).reshape(rows, width), padded
+    return codes.to(torch.int8).reshape(rows, width), padded
 
 
 def _from_rows8(codes, scales):
     rows, width = codes.shape
-    x = codes.view(torch.float8_e4m3fn).float().view(rows, width // 32, 32)
+    x = codes.float().view(rows, width // 32, 32)
     return (x * _power(scales[:, :width // 32], torch.float32)[..., None]).reshape(rows, width)
 
 
@@ -232,7 +224,7 @@ def _weights(gen, n, k):
 
 
 def _rows8_buffers(rows, width):
-    return torch.empty((rows, width), dtype=torch.uint8, device="cuda"), \
+    return torch.empty((rows, width), dtype=torch.int8, device="cuda"), \
         torch.empty((rows, -(-width // 128) * 4), dtype=torch.uint8, device="cuda")
 
 
@@ -248,13 +240,13 @@ def prepare(case, seed):
     if case["kind"] in ("norm", "convert"):
         rows, width = case["rows"], case["width"]
         state["x"] = _activations(gen, rows, width, case["dtype"])
-        out = case.get("out", "mx8")
+        out = case.get("out", "i8")
         if case["kind"] == "norm":
             state["weight"] = 1 + 0.1 * _normal(gen, width)
             if case["residual"]:
                 state["residual"] = (4 * _normal(gen, rows, width)).to(TYPES[case["dtype"]])
                 state["sum"] = torch.empty_like(state["residual"])
-        if out == "mx8":
+        if out == "i8":
             state["codes"], state["scales"] = _rows8_buffers(rows, width)
             back = torch.float32 if case["kind"] == "norm" else TYPES[case["dtype"]]
             state["out"] = torch.empty((rows, width), dtype=back, device="cuda")
@@ -268,14 +260,14 @@ def prepare(case, seed):
         state["out"] = torch.empty_like(state["x"])
     else:
         rows, n, k = case["rows"], case["n"], case["k"]
-        if case["x"] == "mx8":
+        if case["x"] == "i8":
             state["x"] = _to_rows8(_activations(gen, rows, k, "f32"))
         else:
             state["x"] = _activations(gen, rows, k, case["x"])
         state["matrix"] = _to_matrix(_weights(gen, n, k))
         if case["gated"]:
             state["gate"] = _to_matrix(_weights(gen, n, k))
-        if case["out"] == "mx8":
+        if case["out"] == "i8":
             state["codes"], state["scales"] = _rows8_buffers(rows, n)
             state["out"] = torch.empty((rows, n), dtype=torch.bfloat16, device="cuda")
         else:
@@ -295,7 +287,7 @@ def _handles(state):
         return mp.Rows(t.data_ptr(), t.shape[1], None, 0, types[t.dtype])
 
     def rows8(codes, scales):
-        return mp.Rows(codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1], mp.TYPE_MX8)
+        return mp.Rows(codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1], mp.TYPE_I8)
 
     def matrix(m):
         return mp.W4Matrix(m[0].data_ptr(), m[1].data_ptr(), case["n"], case["k"])
@@ -303,7 +295,7 @@ def _handles(state):
     own_rows = {"out": floats(state["out"])}
     own_rows["x"] = rows8(*state["x"]) if isinstance(state["x"], tuple) else floats(state["x"])
     if "codes" in state:
-        own_rows["mx8"] = rows8(state["codes"], state["scales"])
+        own_rows["i8"] = rows8(state["codes"], state["scales"])
     for name in ("residual", "sum"):
         own_rows[name] = floats(state[name]) if name in state else None
     for name in ("matrix", "gate"):
@@ -322,7 +314,7 @@ def _run_own(state):
     from tinyinfer_amd import backend as mp
     case, at = state["case"], state["own"]
     stream = torch.cuda.current_stream().cuda_stream
-    to = at.get("mx8", at["out"])
+    to = at.get("i8", at["out"])
     if case["kind"] == "pack":
         mp.w4_pack(at["matrix"], 0, at["x"], case["n"], stream=stream)
         mp.w4_read(at["matrix"], state["ids"].data_ptr(), case["n"], at["out"], stream=stream)
@@ -336,7 +328,7 @@ def _run_own(state):
     else:
         mp.w4_product(at["matrix"], at["x"], rows, to, gate=at["gate"], workspace=state["workspace"].data_ptr(),
                       workspace_bytes=state["workspace_bytes"], stream=stream)
-    if "mx8" in at:
+    if "i8" in at:
         mp.convert_rows(to, rows, state["out"].shape[1], at["out"], stream=stream)
     return {"out": state["out"], "sum": state["sum"]} if "sum" in state else {"out": state["out"]}
 
@@ -351,19 +343,19 @@ def _run_plain(state):
         return {"out": _from_rows8(*_to_rows8(state["x"].float())).to(out)}
     if case["kind"] == "norm":
         # Values next to the border of two codes need more than 32 bits.
-        wide = torch.float64 if case["out"] == "mx8" else torch.float32
+        wide = torch.float64 if case["out"] == "i8" else torch.float32
         x = state["x"].to(wide)
         if case["residual"]:
             x = x + state["residual"].to(wide)
         y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-5) * state["weight"].to(wide)
-        found = {"out": _from_rows8(*_to_rows8(y)) if case["out"] == "mx8" else y.to(out)}
+        found = {"out": _from_rows8(*_to_rows8(y)) if case["out"] == "i8" else y.to(out)}
         return found | {"sum": x.to(state["sum"].dtype)} if case["residual"] else found
-    x = _from_rows8(*state["x"]) if case["x"] == "mx8" else state["x"].float()
+    x = _from_rows8(*state["x"]) if case["x"] == "i8" else state["x"].float()
     y = torch.matmul(x, _from_matrix(*state["matrix"], case["n"], case["k"]).T)
     if case["gated"]:
         g = torch.matmul(x, _from_matrix(*state["gate"], case["n"], case["k"]).T)
         y = g / (1 + torch.exp(-g)) * y
-    return {"out": _from_rows8(*_to_rows8(y)).to(out) if case["out"] == "mx8" else y.to(out)}
+    return {"out": _from_rows8(*_to_rows8(y)).to(out) if case["out"] == "i8" else y.to(out)}
 
 
 def run(state):
@@ -373,15 +365,13 @@ def run(state):
 # ---- in 64 bits ------------------------------------------------------------------
 
 
-def _numbers(exponent_bits, mantissa_bits, bias, device):
-    """The numbers of a small floating-point format, by code; the sign is the highest bit."""
+def _numbers4(device):
+    """The E2M1 numbers by code: sign, two bits of exponent, one of mantissa."""
     found = []
-    for code in range(1 << (1 + exponent_bits + mantissa_bits)):
-        e = code >> mantissa_bits & ((1 << exponent_bits) - 1)
-        m = code & ((1 << mantissa_bits) - 1)
-        x = math.ldexp(m, 1 - bias - mantissa_bits) if e == 0 else \
-            math.ldexp((1 << mantissa_bits) + m, e - bias - mantissa_bits)
-        found.append(-x if code >> (exponent_bits + mantissa_bits) else x)
+    for code in range(16):
+        e, m = code >> 1 & 3, code & 1
+        x = m / 2 if e == 0 else math.ldexp(2 + m, e - 2)
+        found.append(-x if code & 8 else x)
     return torch.tensor(found, dtype=torch.float64, device=device)
 
 
@@ -409,14 +399,14 @@ def _rows64(x):
     codes, scales = x
     width = codes.shape[1]
     column = torch.arange(width, device="cuda")
-    return _numbers(4, 3, 7, "cuda")[codes.long()] * torch.exp2(scales[:, column // 32].double() - 127)
+    return codes.double() * torch.exp2(scales[:, column // 32].double() - 127)
 
 
 def _matrix64(matrix, n, k):
     codes, scales = matrix
     column = torch.arange(k, device="cuda")
     steps, words = -(-k // 128), -(-k // 512)
-    table = _numbers(2, 1, 1, "cuda")
+    table = _numbers4("cuda")
     parts = []
     for first in range(0, n, 4096):  # in parts, so that the places stay small
         row = torch.arange(first, min(n, first + 4096), device="cuda")[:, None]
@@ -430,23 +420,23 @@ def _matrix64(matrix, n, k):
 
 def exact(case, seed):
     state = prepare(case, seed)
-    eight = _numbers(4, 3, 7, "cuda")[:127]
+    eight = torch.arange(128, dtype=torch.float64, device="cuda")
     if case["kind"] == "pack":
-        four = _numbers(2, 1, 1, "cuda")[:8]
+        four = _numbers4("cuda")[:8]
         x = state["x"]
         return {"out": torch.cat([_held(x[i:i + 4096].double(), four, 6.0) for i in range(0, case["n"], 4096)])}
     x = _rows64(state["x"])
     if case["kind"] == "convert":
-        return {"out": _held(x, eight, 448.0)}
+        return {"out": _held(x, eight, 127.0)}
     if case["kind"] == "norm":
         if case["residual"]:
             x = x + state["residual"].double()
         y = x / torch.sqrt((x * x).sum(-1, keepdim=True) / case["width"] + 1e-5) * state["weight"].double()
-        found = {"out": _held(y, eight, 448.0) if case["out"] == "mx8" else y}
+        found = {"out": _held(y, eight, 127.0) if case["out"] == "i8" else y}
         return found | {"sum": x} if case["residual"] else found
     # Made contiguous first, as elsewhere: the product's right operand is no transposed view.
     y = torch.mm(x, _matrix64(state["matrix"], case["n"], case["k"]).T.contiguous())
     if case["gated"]:
         g = torch.mm(x, _matrix64(state["gate"], case["n"], case["k"]).T.contiguous())
         y = y * g * torch.sigmoid(g)
-    return {"out": _held(y, eight, 448.0) if case["out"] == "mx8" else y}
+    return {"out": _held(y, eight, 127.0) if case["out"] == "i8" else y}
