@@ -333,6 +333,96 @@ int mp_hip_kv8_attention_prefill(const mp_kv8_cache* cache, int32_t layer, const
                                  int32_t max_length, float scale, void* out, int64_t out_stride, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
+/* ---- Weights in 4 bits, rows in 8 bits ------------------------------------
+ * (no counterpart in the reference, whose weights are FP32). What a model
+ * needs around the 8-bit cache above: its weights packed to 4 bits, products
+ * of rows with them, the norm between layers, and rows of 8 bits for prompts.
+ * Stand-alone calls of the same manner: the caller's DEVICE buffers and stream
+ * (NULL: the null stream), asynchronous, no allocation, no state kept between
+ * calls, capturable into a HIP graph; on the stream's device. Refusals are
+ * MP_INVALID_ARGUMENT with a message in mp_hip_last_error(NULL).
+ *
+ * Rows. FP32, BF16 or FP16 as above, any alignment of their type (16 bytes of
+ * base and stride for full speed), or MP_TYPE_I8: a whole number, -127 to 127,
+ * per element in `data`, `stride` bytes from row to row, times a power of two
+ * per 32 elements, the byte b in `scales` for 2^(b - 127) (27 to 247; 255: NaN),
+ * `scale_stride` bytes from row to row. 8-bit rows are whole groups of 32
+ * elements; data and stride are 16-byte aligned, scales and their stride 4-byte
+ * (the scales' rows are whole words, also the last, whose rest may be anything).
+ * A group is written with the smallest power of two, from 2^-100 on, that holds
+ * its largest magnitude, elements rounded to nearest, ties to even; a group with
+ * a NaN, an infinity or a magnitude above 127 * 2^120 has the scale NaN. For
+ * float rows scales and scale_stride are not looked at. At most 2^20 rows a call,
+ * and rows, conversions and reads of at most 2^33 elements.
+ *
+ * Rows that a call writes may not overlap what it reads unless it says so.
+ *
+ * Matrices. `rows` (1 to 2^24) by `depth` (a multiple of 32 up to 2^20)
+ * weights; each is an E2M1 number (0, 0.5, 1, 1.5, 2, 3, 4, 6, or their
+ * negatives) times a power of two per 32 weights along the row, chosen like
+ * that of 8-bit rows (a magnitude above 6 * 2^120 makes it NaN). Codes lie by tiles of 16 rows and 128 columns,
+ * [rows/16][depth/128][column%128/32][row%16][16 bytes], even columns in the
+ * low halves of the bytes, code 8 + c the negative of c; scale bytes as above, 27
+ * to 247, are
+ * [rows/16][depth/512][column%128/32][row%16][column%512/128]: the matrix cores'
+ * operands. Tiles are whole, filled up with zeros. Both are 16-byte aligned and
+ * of the sizes that mp_hip_w4_sizes says. */
+enum { MP_TYPE_I8 = 3 };
+
+typedef struct mp_rows {
+    void* data;
+    int64_t stride;
+    uint8_t* scales;
+    int64_t scale_stride;
+    int32_t type;
+} mp_rows;
+
+typedef struct mp_w4_matrix {
+    uint8_t* codes;
+    uint8_t* scales;
+    int32_t rows, depth;
+} mp_w4_matrix;
+
+int mp_hip_w4_sizes(int32_t rows, int32_t depth, size_t* code_bytes, size_t* scale_bytes);
+
+/* Packs float rows into rows first .. first+rows-1 of a matrix (query, key and
+ * value weights go into one matrix by three calls). The other rows stay as they
+ * are; the call that packs the last row writes the zeros behind it. */
+int mp_hip_w4_pack(const mp_w4_matrix* w, int32_t first, const mp_rows* x, int32_t rows, void* stream);
+
+/* Rows ids[0 .. count-1] (device int32) of a matrix as float rows: an embedding
+ * lookup in a 4-bit table. An id that is no row of the matrix gives NaN. */
+int mp_hip_w4_read(const mp_w4_matrix* w, const int32_t* ids, int32_t count, const mp_rows* out, void* stream);
+
+/* Rows of `width` elements from one type to another, float rows to 8 bits and
+ * back among them. out may be x, as the same rows. */
+int mp_hip_convert_rows(const mp_rows* x, int32_t rows, int32_t width, const mp_rows* out, void* stream);
+
+/* Root-mean-square norm with the residual's addition: t = x + residual
+ * (residual NULL: t = x), out = t * weight / sqrt(mean(t^2) + epsilon) per row of
+ * `width` elements, and t itself to `sum` (NULL: not written; not without a
+ * residual). x, residual and sum are float rows of one type, out rows of any,
+ * weight FP32. Everything is computed in 64 bits and rounded once, out from the
+ * exact t, not from the rounded sum. A row of zeros with epsilon 0 is NaN. sum
+ * may be x or the residual, and out may be x, as the same rows. */
+int mp_hip_rms_norm(const mp_rows* x, const mp_rows* residual, const mp_rows* sum, const float* weight, float epsilon,
+                    int32_t rows, int32_t width, const mp_rows* out, void* stream);
+
+/* Products: out[r][n] = sum_k x[r][k] w[n][k], or with a `gate` matrix of w's
+ * size the gated pair g / (1 + exp(-g)) * u of g = x gate^T and u = x w^T. x and
+ * out are rows of any type (8-bit results need w->rows to be a multiple of 32).
+ * One to 2^20 rows: single tokens read the weights' 4 bits once, prompts are the
+ * matrix cores' work. Rows and weights count as they are, sums are FP32, and the
+ * result is rounded once, to out's type. A row with a NaN or an
+ * infinity has no finite result, and a NaN scale of a matrix's row none in its
+ * column; other rows and columns are as without them. The workspace (16-byte
+ * aligned; mp_hip_w4_product_workspace says its size for the same or more rows; 0 is
+ * possible, and then it may be NULL) holds nothing between calls; calls that may
+ * overlap, replayed graphs among them, need workspaces of their own. */
+int mp_hip_w4_product_workspace(const mp_w4_matrix* w, int32_t type, int32_t rows, int32_t gated, size_t* bytes);
+int mp_hip_w4_product(const mp_w4_matrix* w, const mp_w4_matrix* gate, const mp_rows* x, int32_t rows,
+                      const mp_rows* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Applies queued table entries and copies, then waits for all work on the
  * context's stream (StreamBlas::synchronize). */
 int mp_hip_sync(mp_hip* h);

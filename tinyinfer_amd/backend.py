@@ -44,7 +44,7 @@ class KernelTimes(ctypes.Structure):
 
 
 TIME_ATTENTION, TIME_PROJECTION, TIME_HEAD, TIME_SAMPLED = 1, 2, 4, 8
-TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_I8 = 0, 1, 2, 3
 KV8_INT8, KV8_E4M3 = 0, 1
 
 
@@ -58,6 +58,18 @@ class Rope(ctypes.Structure):
     """Rotary tables on the device and how heads turn by them (mp_rope)."""
     _fields_ = [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p)] + [
         (n, ctypes.c_int32) for n in ("positions", "dims", "interleaved")]
+
+
+class Rows(ctypes.Structure):
+    """Rows of elements on the device, with scales where they are of 8 bits (mp_rows)."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_int64), ("scales", ctypes.c_void_p),
+                ("scale_stride", ctypes.c_int64), ("type", ctypes.c_int32)]
+
+
+class W4Matrix(ctypes.Structure):
+    """A matrix of 4-bit weights on the device (mp_w4_matrix)."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("rows", ctypes.c_int32),
+                ("depth", ctypes.c_int32)]
 
 
 class BackendError(RuntimeError):
@@ -93,6 +105,14 @@ def _bind(lib):
                                                 vp, i64, vp, size, vp]
     lib.mp_hip_kv8_attention_prefill.argtypes = [cache, i32, vp, i64, i32, vp, i32, vp, vp, i32, i32, i32, i32,
                                                  ctypes.c_float, vp, i64, vp, size, vp]
+    rows, matrix = ctypes.POINTER(Rows), ctypes.POINTER(W4Matrix)
+    lib.mp_hip_w4_sizes.argtypes = [i32, i32, ctypes.POINTER(size), ctypes.POINTER(size)]
+    lib.mp_hip_w4_pack.argtypes = [matrix, i32, rows, i32, vp]
+    lib.mp_hip_w4_read.argtypes = [matrix, vp, i32, rows, vp]
+    lib.mp_hip_convert_rows.argtypes = [rows, i32, i32, rows, vp]
+    lib.mp_hip_rms_norm.argtypes = [rows, rows, rows, vp, ctypes.c_float, i32, i32, rows, vp]
+    lib.mp_hip_w4_product_workspace.argtypes = [matrix, i32, i32, i32, ctypes.POINTER(size)]
+    lib.mp_hip_w4_product.argtypes = [matrix, matrix, rows, i32, rows, vp, size, vp]
     lib.mp_hip_sync.argtypes = [vp]
     lib.mp_hip_stats.argtypes = [vp, ctypes.POINTER(Counters)]
     lib.mp_hip_kv_pools.argtypes = [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_size_t)]
@@ -263,7 +283,7 @@ def paged_attention_decode_fast(q, keys, values, tables, table_stride: int, leng
         raise BackendError(status, f"mp_hip_paged_attention_decode_fast failed ({status}): {message}")
 
 
-def _kv8_check(status: int, name: str):
+def _check_call(status: int, name: str):
     if status:
         message = (lib().mp_hip_last_error(None) or b"").decode()
         raise BackendError(status, f"{name} failed ({status}): {message}")
@@ -275,7 +295,7 @@ def kv8_append(cache: Kv8Cache, layer: int, k, k_stride: int, v, v_stride: int, 
     """New tokens' keys (rotated by `rope`) and values into the pages of an
     8-bit cache, and the rotated queries to q_out (raw device pointers;
     strides in elements). Asynchronous on `stream`."""
-    _kv8_check(lib().mp_hip_kv8_append(cache, layer, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride,
+    _check_call(lib().mp_hip_kv8_append(cache, layer, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride,
                                        heads, type, rope, tables, table_stride, starts, used, sequences, rows,
                                        stream), "mp_hip_kv8_append")
 
@@ -283,14 +303,14 @@ def kv8_append(cache: Kv8Cache, layer: int, k, k_stride: int, v, v_stride: int, 
 def kv8_read(cache: Kv8Cache, layer: int, tables, table_stride: int, starts, used, sequences: int, rows: int,
              type: int, k, k_stride: int, v, v_stride: int, stream: int | None = None):
     """Tokens of an 8-bit cache as rows of values. Asynchronous on `stream`."""
-    _kv8_check(lib().mp_hip_kv8_read(cache, layer, tables, table_stride, starts, used, sequences, rows, type, k,
+    _check_call(lib().mp_hip_kv8_read(cache, layer, tables, table_stride, starts, used, sequences, rows, type, k,
                                      k_stride, v, v_stride, stream), "mp_hip_kv8_read")
 
 
 def kv8_attention_workspace(cache: Kv8Cache, rows: int, sequences: int, heads: int, max_length: int) -> int:
     """Workspace bytes for the attention calls of up to these sizes."""
     size = ctypes.c_size_t()
-    _kv8_check(lib().mp_hip_kv8_attention_workspace(cache, rows, sequences, heads, max_length, ctypes.byref(size)),
+    _check_call(lib().mp_hip_kv8_attention_workspace(cache, rows, sequences, heads, max_length, ctypes.byref(size)),
                "mp_hip_kv8_attention_workspace")
     return size.value
 
@@ -300,7 +320,7 @@ def kv8_attention_decode(cache: Kv8Cache, layer: int, q, q_stride: int, type: in
                          workspace=None, workspace_bytes: int = 0, stream: int | None = None):
     """Attention of one query row per sequence over an 8-bit cache; `lengths`
     on the device. Asynchronous on `stream`."""
-    _kv8_check(lib().mp_hip_kv8_attention_decode(cache, layer, q, q_stride, type, tables, table_stride, lengths, rows,
+    _check_call(lib().mp_hip_kv8_attention_decode(cache, layer, q, q_stride, type, tables, table_stride, lengths, rows,
                                                  heads, max_length, scale, out, out_stride, workspace,
                                                  workspace_bytes, stream), "mp_hip_kv8_attention_decode")
 
@@ -310,6 +330,49 @@ def kv8_attention_prefill(cache: Kv8Cache, layer: int, q, q_stride: int, type: i
                           out_stride: int, workspace=None, workspace_bytes: int = 0, stream: int | None = None):
     """Causal attention of packed rows over an 8-bit cache that holds them
     already. Asynchronous on `stream`."""
-    _kv8_check(lib().mp_hip_kv8_attention_prefill(cache, layer, q, q_stride, type, tables, table_stride, starts, used,
+    _check_call(lib().mp_hip_kv8_attention_prefill(cache, layer, q, q_stride, type, tables, table_stride, starts, used,
                                                   sequences, rows, heads, max_length, scale, out, out_stride,
                                                   workspace, workspace_bytes, stream), "mp_hip_kv8_attention_prefill")
+
+
+def w4_sizes(rows: int, depth: int) -> tuple[int, int]:
+    """Bytes of the codes and of the scales of a 4-bit matrix."""
+    codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
+    _check_call(lib().mp_hip_w4_sizes(rows, depth, ctypes.byref(codes), ctypes.byref(scales)), "mp_hip_w4_sizes")
+    return codes.value, scales.value
+
+
+def w4_pack(matrix: W4Matrix, first: int, x: Rows, rows: int, stream: int | None = None):
+    """Float rows into rows first .. first+rows-1 of a 4-bit matrix. Asynchronous on `stream`."""
+    _check_call(lib().mp_hip_w4_pack(matrix, first, x, rows, stream), "mp_hip_w4_pack")
+
+
+def w4_read(matrix: W4Matrix, ids, count: int, out: Rows, stream: int | None = None):
+    """Rows `ids` (device int32) of a 4-bit matrix as float rows. Asynchronous on `stream`."""
+    _check_call(lib().mp_hip_w4_read(matrix, ids, count, out, stream), "mp_hip_w4_read")
+
+
+def convert_rows(x: Rows, rows: int, width: int, out: Rows, stream: int | None = None):
+    """Rows from one type to another, to 8 bits and back among them. Asynchronous on `stream`."""
+    _check_call(lib().mp_hip_convert_rows(x, rows, width, out, stream), "mp_hip_convert_rows")
+
+
+def rms_norm(x: Rows, weight, epsilon: float, rows: int, width: int, out: Rows, residual: Rows | None = None,
+             sum: Rows | None = None, stream: int | None = None):
+    """Root-mean-square norm of x (+ residual, the sum to `sum`); weight: device FP32. Asynchronous on `stream`."""
+    _check_call(lib().mp_hip_rms_norm(x, residual, sum, weight, epsilon, rows, width, out, stream), "mp_hip_rms_norm")
+
+
+def w4_product_workspace(matrix: W4Matrix, type: int, rows: int, gated: bool = False) -> int:
+    """Workspace bytes of w4_product for up to `rows` rows of a type."""
+    size = ctypes.c_size_t()
+    _check_call(lib().mp_hip_w4_product_workspace(matrix, type, rows, int(gated), ctypes.byref(size)),
+                "mp_hip_w4_product_workspace")
+    return size.value
+
+
+def w4_product(matrix: W4Matrix, x: Rows, rows: int, out: Rows, gate: W4Matrix | None = None, workspace=None,
+               workspace_bytes: int = 0, stream: int | None = None):
+    """Rows times a 4-bit matrix, or with `gate` silu(x gate^T) * (x matrix^T). Asynchronous on `stream`."""
+    _check_call(lib().mp_hip_w4_product(matrix, gate, x, rows, out, workspace, workspace_bytes, stream),
+                "mp_hip_w4_product")

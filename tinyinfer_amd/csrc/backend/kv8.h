@@ -21,16 +21,13 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#include <new>
-#include <string>
-
 #include "../../../include/mp_hip.h"
+#include "elements.h"
+#include "entry.h"
 #include "kv8_rules.h"
 #include "lanes.h"
 
 namespace mphip {
-
-void set_free_error(const std::string& message);
 
 // One layer of a cache on the device.
 struct Kv8Layer {
@@ -48,37 +45,6 @@ __device__ __forceinline__ size_t kv8_head(const Kv8Layer& kv, int block, int he
 
 // ---- across a wavefront, without a way through LDS -----------------------------
 
-// Of the four lanes (c, 0..3) of a column, by swapping rows of 16 lanes and
-// halves of the wavefront between two copies: no way through LDS.
-__device__ __forceinline__ float column_max(float v) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ uint32_t column_max(uint32_t v) {
-    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max((uint32_t)r[0], (uint32_t)r[1]);
-    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max((uint32_t)r[0], (uint32_t)r[1]);
-}
-__device__ __forceinline__ float column_sum(float v) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float wave_max(float v) {
-    v = fmaxf(v, dpp<kDppQuadXor1>(v));
-    return column_max(row_quads_max(fmaxf(v, dpp<kDppQuadXor2>(v))));
-}
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    v = max(v, dpp_u<kDppQuadXor1>(v));
-    v = max(v, dpp_u<kDppQuadXor2>(v));
-    v = max(v, dpp_u<kDppRowRor4>(v));
-    return column_max(max(v, dpp_u<kDppRowRor8>(v)));
-}
-__device__ __forceinline__ float wave_sum(float v) { return column_sum(row_sum(v)); }
 // The sum over the lanes up to this one: within rows of 16, then the rows'
 // totals (row_shr 1, 2, 4, 8; row_bcast 15 and 31).
 __device__ __forceinline__ int wave_prefix(int v) {
@@ -138,82 +104,12 @@ __device__ __forceinline__ bool kv8_find(const Kv8Rows& r, int item, Items items
     return false;
 }
 
-// ---- elements of the caller's type -------------------------------------------
-
-__device__ __forceinline__ float from_bf16(uint32_t low_half) { return __uint_as_float(low_half << 16); }
-__device__ __forceinline__ float from_f16(uint32_t low_half) {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)low_half);
-}
-// Rounded to nearest, ties to even; NaN stays NaN.
-__device__ __forceinline__ uint16_t to_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
-__device__ __forceinline__ uint16_t to_f16(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
-
-__device__ __forceinline__ float load_one(const void* p, int type, int64_t i) {
-    if (type == MP_TYPE_F32) return static_cast<const float*>(p)[i];
-    const uint32_t b = static_cast<const uint16_t*>(p)[i];
-    return type == MP_TYPE_BF16 ? from_bf16(b) : from_f16(b);
-}
-__device__ __forceinline__ void store_one(void* p, int type, int64_t i, float x) {
-    if (type == MP_TYPE_F32) static_cast<float*>(p)[i] = x;
-    else static_cast<uint16_t*>(p)[i] = type == MP_TYPE_BF16 ? to_bf16(x) : to_f16(x);
-}
-
-// N (a multiple of 4) consecutive elements from i on; `wide`: they start at a
-// multiple of 16 bytes (FP32) or 8 (16-bit types).
-template <int N>
-__device__ __forceinline__ void load_row(const void* p, int type, bool wide, int64_t i, float (&x)[N]) {
-    if (!wide) {
-#pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = load_one(p, type, i + k);
-    } else if (type == MP_TYPE_F32) {
-#pragma unroll
-        for (int k = 0; k < N; k += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + k);
-            x[k] = v.x, x[k + 1] = v.y, x[k + 2] = v.z, x[k + 3] = v.w;
-        }
-    } else {
-        uint2 v[N / 4];
-#pragma unroll
-        for (int k = 0; k < N; k += 4)
-            v[k / 4] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i + k);
-#pragma unroll
-        for (int k = 0; k < N; k += 2) {
-            const uint32_t two = k % 4 ? v[k / 4].y : v[k / 4].x;
-            x[k] = type == MP_TYPE_BF16 ? from_bf16(two) : from_f16(two & 0xFFFF);
-            x[k + 1] = type == MP_TYPE_BF16 ? __uint_as_float(two & 0xFFFF0000u) : from_f16(two >> 16);
-        }
-    }
-}
-__device__ __forceinline__ void store_four(void* p, int type, bool wide, int64_t i, float a, float b, float c,
-                                           float d) {
-    if (!wide) {
-        store_one(p, type, i, a);
-        store_one(p, type, i + 1, b);
-        store_one(p, type, i + 2, c);
-        store_one(p, type, i + 3, d);
-    } else if (type == MP_TYPE_F32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(a, b, c, d);
-    } else {
-        const bool bf = type == MP_TYPE_BF16;
-        const uint32_t lo = (bf ? to_bf16(a) : to_f16(a)) | (uint32_t)(bf ? to_bf16(b) : to_f16(b)) << 16;
-        const uint32_t hi = (bf ? to_bf16(c) : to_f16(c)) | (uint32_t)(bf ? to_bf16(d) : to_f16(d)) << 16;
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(lo, hi);
-    }
-}
-
 // ---- host side of the entries ---------------------------------------------
-
-inline size_t kv8_element(int type) { return type == MP_TYPE_F32 ? 4 : 2; }
 
 // Whether rows at `p` with this stride can be read and written by fours.
 inline bool kv8_wide(const void* p, int64_t stride, int type) {
-    const size_t four = 4 * kv8_element(type);
+    const size_t four = 4 * element_bytes(type);
     return reinterpret_cast<uintptr_t>(p) % four == 0 && stride % 4 == 0;
-}
-
-inline int kv8_refuse(const char* message) {
-    set_free_error(message);
-    return MP_INVALID_ARGUMENT;
 }
 
 // nullptr, or what is wrong with a cache and a layer of it.
@@ -237,7 +133,7 @@ inline const char* kv8_wrong_cache(const mp_kv8_cache* c, int layer) {
 }
 inline const char* kv8_wrong_matrix(const void* p, int64_t stride, int64_t width, int type) {
     if (type != MP_TYPE_F32 && type != MP_TYPE_BF16 && type != MP_TYPE_F16) return "8-bit cache: unknown element type";
-    if (!p || reinterpret_cast<uintptr_t>(p) % kv8_element(type)) return "8-bit cache: a row matrix is missing or misaligned";
+    if (!p || reinterpret_cast<uintptr_t>(p) % element_bytes(type)) return "8-bit cache: a row matrix is missing or misaligned";
     if (stride < width || stride > (int64_t)1 << 40) return "8-bit cache: a row stride is smaller than the row";
     return nullptr;
 }
@@ -253,49 +149,6 @@ inline bool kv8_bad_ints(const int32_t* p) { return !p || reinterpret_cast<uintp
 inline Kv8Layer kv8_layer(const mp_kv8_cache& c, int layer) {
     return Kv8Layer{c.keys, c.values, reinterpret_cast<float2*>(c.scales), c.blocks, c.layers, layer, c.kv_heads,
                     c.dim, __builtin_ctz((unsigned)c.block_tokens)};
-}
-
-// Makes the device of a caller's stream current for a call's launches.
-class StreamDevice {
-public:
-    explicit StreamDevice(hipStream_t s) {
-        // The null, legacy and per-thread streams belong to the current device.
-        if (reinterpret_cast<uintptr_t>(s) <= 2) return;
-        hipDevice_t wanted = 0;
-        int current = 0;
-        status = hipStreamGetDevice(s, &wanted);
-        if (status == hipSuccess) status = hipGetDevice(&current);
-        if (status != hipSuccess || wanted == current) return;
-        status = hipSetDevice(wanted);
-        if (status == hipSuccess) previous_ = current;
-    }
-    ~StreamDevice() {
-        if (previous_ >= 0) (void)hipSetDevice(previous_);
-    }
-    StreamDevice(const StreamDevice&) = delete;
-    StreamDevice& operator=(const StreamDevice&) = delete;
-    hipError_t status = hipSuccess;
-
-private:
-    int previous_ = -1;
-};
-
-inline int kv8_done(hipError_t e, const char* what) {
-    if (e == hipSuccess) return MP_OK;
-    set_free_error(std::string(what) + ": " + hipGetErrorString(e));
-    return MP_DEVICE_ERROR;
-}
-
-// No exception leaves a C entry.
-template <typename Body>
-int kv8_entry(Body body) {
-    try {
-        return body();
-    } catch (const std::bad_alloc&) {
-        return MP_OUT_OF_MEMORY;
-    } catch (...) {
-        return MP_DEVICE_ERROR;
-    }
 }
 
 }  // namespace mphip

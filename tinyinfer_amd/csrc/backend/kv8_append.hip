@@ -496,7 +496,7 @@ hipError_t with_constants(int type, int format, int dim, const F& f) {
 
 int threads_for(int bt) { return bt == 128 ? 512 : kThreads; }
 
-int too_large() { return kv8_refuse("8-bit cache: rows times heads are too many for one call"); }
+int too_large() { return refuse_call("8-bit cache: rows times heads are too many for one call"); }
 constexpr int64_t kMaxGroups = 1 << 22;  // 2^31 threads of 512
 
 }  // namespace
@@ -508,31 +508,31 @@ extern "C" int mp_hip_kv8_append(const mp_kv8_cache* cache, int32_t layer, const
                                  const int32_t* tables, int32_t table_stride, const int32_t* starts,
                                  const int32_t* used, int32_t sequences, int32_t rows, void* stream) {
     using namespace mphip;
-    return kv8_entry([&]() -> int {
+    return c_entry([&]() -> int {
         const char* wrong = kv8_wrong_cache(cache, layer);
         if (!wrong) wrong = kv8_wrong_rows(tables, table_stride, sequences, rows);
-        if (wrong) return kv8_refuse(wrong);
+        if (wrong) return refuse_call(wrong);
         const int64_t width = (int64_t)cache->kv_heads * cache->dim;
         wrong = kv8_wrong_matrix(k, k_stride, width, type);
         if (!wrong) wrong = kv8_wrong_matrix(v, v_stride, width, type);
-        if (wrong) return kv8_refuse(wrong);
+        if (wrong) return refuse_call(wrong);
         if (kv8_bad_ints(starts) || kv8_bad_ints(used))
-            return kv8_refuse("8-bit cache: starts or used are missing or misaligned");
+            return refuse_call("8-bit cache: starts or used are missing or misaligned");
         if (q) {
-            if (heads < 1 || heads > kKv8MaxHeads) return kv8_refuse("8-bit cache: heads must be 1 to 1,024");
+            if (heads < 1 || heads > kKv8MaxHeads) return refuse_call("8-bit cache: heads must be 1 to 1,024");
             wrong = kv8_wrong_matrix(q, q_stride, (int64_t)heads * cache->dim, type);
             if (!wrong) wrong = kv8_wrong_matrix(q_out, q_out_stride, (int64_t)heads * cache->dim, type);
-            if (wrong) return kv8_refuse(wrong);
+            if (wrong) return refuse_call(wrong);
             if (q == q_out && q_stride != q_out_stride)
-                return kv8_refuse("8-bit cache: queries rotated in place need one stride");
+                return refuse_call("8-bit cache: queries rotated in place need one stride");
         }
         RopeView view{nullptr, nullptr, 0, 0, false};
         if (rope && rope->dims != 0) {
             if (rope->dims < 0 || rope->dims % 2 || rope->dims > cache->dim)
-                return kv8_refuse("8-bit cache: rotated dims must be even and at most dim");
+                return refuse_call("8-bit cache: rotated dims must be even and at most dim");
             if (!rope->cos || !rope->sin || reinterpret_cast<uintptr_t>(rope->cos) % 4 ||
                 reinterpret_cast<uintptr_t>(rope->sin) % 4 || rope->positions < 1)
-                return kv8_refuse("8-bit cache: rotation tables are missing, misaligned or empty");
+                return refuse_call("8-bit cache: rotation tables are missing, misaligned or empty");
             view = RopeView{rope->cos, rope->sin, rope->positions, rope->dims / 2, rope->interleaved != 0};
         }
         if (rows == 0 || sequences == 0) return MP_OK;
@@ -550,20 +550,20 @@ extern "C" int mp_hip_kv8_append(const mp_kv8_cache* cache, int32_t layer, const
         a.q_stride = q_stride, a.q_out_stride = q_out_stride;
         a.heads = heads, a.type = type, a.format = cache->format;
         a.k_wide = kv8_wide(k, k_stride, type);
-        const int per16 = 16 / (int)kv8_element(type);
+        const int per16 = 16 / (int)element_bytes(type);
         a.q_by_16 = q && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0 &&
                     q_stride % per16 == 0 && q_out_stride % per16 == 0 &&
                     (view.interleaved ? 2 * view.half : view.half) % per16 == 0;
         a.kv_groups = (int)kv_groups;
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const StreamDevice device(s);
-        if (device.status != hipSuccess) return kv8_done(device.status, "8-bit append: device of the stream");
+        if (device.status != hipSuccess) return call_done(device.status, "8-bit append: device of the stream");
         const hipError_t e = with_constants(type, cache->format, cache->dim, [&](auto t, auto f, auto d) {
             kv8_append_kernel<decltype(t)::value, decltype(f)::value, decltype(d)::value>
                 <<<(unsigned)(kv_groups + q_groups), threads, 0, s>>>(a);
             return hipGetLastError();
         });
-        return kv8_done(e, "8-bit append launch");
+        return call_done(e, "8-bit append launch");
     });
 }
 
@@ -571,16 +571,16 @@ extern "C" int mp_hip_kv8_read(const mp_kv8_cache* cache, int32_t layer, const i
                                const int32_t* starts, const int32_t* used, int32_t sequences, int32_t rows,
                                int32_t type, void* k, int64_t k_stride, void* v, int64_t v_stride, void* stream) {
     using namespace mphip;
-    return kv8_entry([&]() -> int {
+    return c_entry([&]() -> int {
         const char* wrong = kv8_wrong_cache(cache, layer);
         if (!wrong) wrong = kv8_wrong_rows(tables, table_stride, sequences, rows);
-        if (wrong) return kv8_refuse(wrong);
+        if (wrong) return refuse_call(wrong);
         const int64_t width = (int64_t)cache->kv_heads * cache->dim;
         wrong = kv8_wrong_matrix(k, k_stride, width, type);
         if (!wrong) wrong = kv8_wrong_matrix(v, v_stride, width, type);
-        if (wrong) return kv8_refuse(wrong);
+        if (wrong) return refuse_call(wrong);
         if (kv8_bad_ints(starts) || kv8_bad_ints(used))
-            return kv8_refuse("8-bit cache: starts or used are missing or misaligned");
+            return refuse_call("8-bit cache: starts or used are missing or misaligned");
         if (rows == 0 || sequences == 0) return MP_OK;
         const int bt = cache->block_tokens, threads = threads_for(bt), waves = threads / 64;
         const int64_t units = kv8_most_pages(rows, sequences, bt) * cache->kv_heads * 2, per_group = waves / (bt / kTile);
@@ -595,12 +595,12 @@ extern "C" int mp_hip_kv8_read(const mp_kv8_cache* cache, int32_t layer, const i
         a.k_wide = kv8_wide(k, k_stride, type);
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const StreamDevice device(s);
-        if (device.status != hipSuccess) return kv8_done(device.status, "8-bit read: device of the stream");
+        if (device.status != hipSuccess) return call_done(device.status, "8-bit read: device of the stream");
         const hipError_t e = with_constants(type, cache->format, cache->dim, [&](auto t, auto f, auto d) {
             kv8_read_kernel<decltype(t)::value, decltype(f)::value, decltype(d)::value>
                 <<<(unsigned)groups, threads, 0, s>>>(a);
             return hipGetLastError();
         });
-        return kv8_done(e, "8-bit read launch");
+        return call_done(e, "8-bit read launch");
     });
 }

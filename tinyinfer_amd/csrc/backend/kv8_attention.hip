@@ -620,15 +620,15 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
     if (!wrong) wrong = kv8_wrong_rows(tables, table_stride, sequences, rows);
     if (!wrong) wrong = kv8_wrong_matrix(q, q_stride, (int64_t)heads * cache->dim, type);
     if (!wrong) wrong = kv8_wrong_matrix(out, out_stride, (int64_t)heads * cache->dim, type);
-    if (wrong) return kv8_refuse(wrong);
+    if (wrong) return refuse_call(wrong);
     if (q == out && q_stride != out_stride && rows > 1)
-        return kv8_refuse("8-bit attention: a result in place of the queries needs one stride");
+        return refuse_call("8-bit attention: a result in place of the queries needs one stride");
     if (kv8_bad_ints(used) || (!decode && kv8_bad_ints(starts)))
-        return kv8_refuse("8-bit attention: lengths, starts or used are missing or misaligned");
+        return refuse_call("8-bit attention: lengths, starts or used are missing or misaligned");
     if (!(scale >= 0) || !isfinite((float)(scale * 1.4426950408889634074)))
-        return kv8_refuse("8-bit attention: scale must be finite (to 2.3e38) and not negative");
+        return refuse_call("8-bit attention: scale must be finite (to 2.3e38) and not negative");
     if ((int64_t)rows * heads > kKv8MostColumns)
-        return kv8_refuse("8-bit attention: rows times heads are too many for one call");
+        return refuse_call("8-bit attention: rows times heads are too many for one call");
     if (rows == 0 || sequences == 0) return MP_OK;
     const int group = heads / cache->kv_heads;
     const Kv8Plan p = decode ? kv8_decode_plan(rows, cache->kv_heads, cache->dim, max_length)
@@ -636,9 +636,9 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
                                                 max_length);
     const size_t need = kv8_partial_floats(p, rows, heads, cache->dim) * sizeof(float);
     if (need > workspace_bytes || (need && !workspace))
-        return kv8_refuse("8-bit attention: the workspace is smaller than mp_hip_kv8_attention_workspace says");
+        return refuse_call("8-bit attention: the workspace is smaller than mp_hip_kv8_attention_workspace says");
     if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
-        return kv8_refuse("8-bit attention: the workspace must be 16-byte aligned");
+        return refuse_call("8-bit attention: the workspace must be 16-byte aligned");
     Kv8Attention a{};
     a.kv = kv8_layer(*cache, layer);
     a.rows = Kv8Rows{tables, starts, used, table_stride, sequences, rows};
@@ -652,7 +652,7 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
     a.partial_ml = reinterpret_cast<float2*>(a.partial_out + (need ? (size_t)rows * heads * p.splits * cache->dim : 0));
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const StreamDevice device(s);
-    if (device.status != hipSuccess) return kv8_done(device.status, "8-bit attention: device of the stream");
+    if (device.status != hipSuccess) return call_done(device.status, "8-bit attention: device of the stream");
     if (cache->format == MP_KV8_INT8) launch_format<MP_KV8_INT8>(s, p, a, decode);
     else launch_format<MP_KV8_E4M3>(s, p, a, decode);
     hipError_t e = hipGetLastError();
@@ -670,7 +670,7 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
         }
         e = hipGetLastError();
     }
-    return kv8_done(e, "8-bit attention launch");
+    return call_done(e, "8-bit attention launch");
 }
 
 }  // namespace
@@ -679,11 +679,11 @@ int attention(const mp_kv8_cache* cache, int layer, const void* q, int64_t q_str
 extern "C" int mp_hip_kv8_attention_workspace(const mp_kv8_cache* cache, int32_t rows, int32_t sequences,
                                               int32_t heads, int32_t max_length, size_t* bytes) {
     using namespace mphip;
-    return kv8_entry([&]() -> int {
-        if (!bytes) return kv8_refuse("8-bit attention: no place for the workspace's size");
-        if (const char* wrong = wrong_attention(cache, 0, heads, max_length)) return kv8_refuse(wrong);
+    return c_entry([&]() -> int {
+        if (!bytes) return refuse_call("8-bit attention: no place for the workspace's size");
+        if (const char* wrong = wrong_attention(cache, 0, heads, max_length)) return refuse_call(wrong);
         if (sequences < 0 || sequences > kKv8MaxRows || rows < 0 || rows > kKv8MaxRows)
-            return kv8_refuse("8-bit cache: sequences and rows must be 0 to 1,048,576");
+            return refuse_call("8-bit cache: sequences and rows must be 0 to 1,048,576");
         *bytes = kv8_workspace_floats(rows, sequences, heads, cache->kv_heads, cache->dim, max_length) * sizeof(float);
         return MP_OK;
     });
@@ -695,7 +695,7 @@ extern "C" int mp_hip_kv8_attention_decode(const mp_kv8_cache* cache, int32_t la
                                            float scale, void* out, int64_t out_stride, void* workspace,
                                            size_t workspace_bytes, void* stream) {
     using namespace mphip;
-    return kv8_entry([&]() -> int {
+    return c_entry([&]() -> int {
         return attention(cache, layer, q, q_stride, type, tables, table_stride, nullptr, lengths, rows, rows, heads,
                          max_length, scale, out, out_stride, workspace, workspace_bytes, stream, true);
     });
@@ -708,7 +708,7 @@ extern "C" int mp_hip_kv8_attention_prefill(const mp_kv8_cache* cache, int32_t l
                                             int64_t out_stride, void* workspace, size_t workspace_bytes,
                                             void* stream) {
     using namespace mphip;
-    return kv8_entry([&]() -> int {
+    return c_entry([&]() -> int {
         return attention(cache, layer, q, q_stride, type, tables, table_stride, starts, used, sequences, rows, heads,
                          max_length, scale, out, out_stride, workspace, workspace_bytes, stream, false);
     });

@@ -11,6 +11,7 @@ namespace mphip {
 // DPP controls (GFX9): quad permutations and rotations within a 16-lane row.
 constexpr int kDppQuadXor1 = 0xB1;  // quad_perm [1,0,3,2]
 constexpr int kDppQuadXor2 = 0x4E;  // quad_perm [2,3,0,1]
+constexpr int kDppHalfMirror = 0x141;  // lane i with 7 - i, of 8
 constexpr int kDppRowRor4 = 0x124;
 constexpr int kDppRowRor8 = 0x128;
 
@@ -51,6 +52,45 @@ __device__ __forceinline__ float rows_sum(float v) {
 }
 __device__ __forceinline__ float rows_max(float v) {
     return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)), fmaxf(lane_value(v, 32), lane_value(v, 48)));
+}
+
+// Of the four lanes (c, 0..3) of a column, by swapping rows of 16 lanes and
+// halves of the wavefront between two copies: no way through LDS.
+__device__ __forceinline__ float column_max(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ uint32_t column_max(uint32_t v) {
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)r[0], (uint32_t)r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+__device__ __forceinline__ float column_sum(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp<kDppQuadXor1>(v));
+    return column_max(row_quads_max(fmaxf(v, dpp<kDppQuadXor2>(v))));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, dpp_u<kDppQuadXor1>(v));
+    v = max(v, dpp_u<kDppQuadXor2>(v));
+    v = max(v, dpp_u<kDppRowRor4>(v));
+    return column_max(max(v, dpp_u<kDppRowRor8>(v)));
+}
+__device__ __forceinline__ float wave_sum(float v) { return column_sum(row_sum(v)); }
+
+// Orders a wavefront's own accesses to LDS: what its lanes wrote before, all of
+// them read after.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 }  // namespace mphip
