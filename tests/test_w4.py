@@ -374,7 +374,7 @@ def test_products_to_every_type(torch_cuda, kind, to, rows, n, k, pad):
 @pytest.mark.parametrize("pad, shift", [(1, 0), (0, 1), (5, 3), (2, 2)])
 def test_products_of_any_alignment(torch_cuda, kind, pad, shift):
     rng = np.random.default_rng(pad + 10 * shift)
-    for rows, n, k in ((1, 37, 96), (20, 51, 160), (70, 35, 64)):
+    for rows, n, k in ((1, 37, 96), (20, 51, 160), (70, 35, 64), (130, 16291, 96)):
         x = ref.rounded(rng.standard_normal((rows, k)), kind)
         w = ref.held(rng.standard_normal((n, k)), E2M1)
         matrix, source = Matrix(torch_cuda, n, k, w), Floats(torch_cuda, x, kind, pad, shift)
@@ -387,7 +387,7 @@ def test_products_of_any_alignment(torch_cuda, kind, pad, shift):
 
 
 @ANY
-@pytest.mark.parametrize("rows", [3, 40, 300])
+@pytest.mark.parametrize("rows", [3, 40, 300, 2000])
 def test_nan_stays_in_its_row_and_column(torch_cuda, kind, rows):
     rng = np.random.default_rng(rows)
     n, k = 50, 288
@@ -547,3 +547,18 @@ def test_a_decode_step_of_a_layer(torch_cuda):
     check(inner_rows.back(), h2.back(), up_w, gate_w)
     mp.w4_product(down.view, inner_rows.rows, rows, last.rows)
     check(last.back(), inner_rows.back(), down_w)
+
+
+@ANY
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("rows, n, k", [(129, 16500, 96), (640, 5000, 32), (1000, 4120, 192), (2049, 2000, 544), (130, 17000, 576)])
+def test_products_of_many_rows(torch_cuda, kind, gated, rows, n, k):
+    check_product(torch_cuda, np.random.default_rng(rows + n + k), rows, n, k, kind, F32, gated)
+
+
+@ANY
+@pytest.mark.parametrize("to", [F32, BF16, F16, I8], ids=["f32", "bf16", "f16", "i8"])
+@pytest.mark.parametrize("rows, n, k, pad", [(1025, 4128, 160, 16), (4097, 1056, 64, 0)])
+def test_products_of_many_rows_to_every_type(torch_cuda, kind, to, rows, n, k, pad):
+    for gated in (False, True):
+        check_product(torch_cuda, np.random.default_rng(n + k), rows, n, k, kind, to, gated, pad)

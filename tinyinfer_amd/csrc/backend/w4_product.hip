@@ -1,32 +1,15 @@
 // Products of rows with 4-bit matrices: wavefronts that share columns and deal
 // the depth among themselves.
-#include "w4.h"
+#include "w4_product.h"
 
 namespace mphip {
 namespace {
 
-typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-
-struct ProductArgs {
-    W4View m[2];  // the matrix, the gate
-    int n, depth, rows;
-    RowsView x, out;
-    bool x_wide, out_wide;
-    int column_blocks, row_blocks;
-};
-
-// The rows' operand of 128 columns: lane (c, g) has row c at columns 32g ..+31,
-// as sums of 1 (8 bits, BF16), 2 (FP16) or 3 (FP32) BF16 numbers that hold them
-// exactly: each takes the next 8 bits.
+// The rows' operand of 128 columns: lane (c, g) has row c at columns 32g ..+31.
 template <int KIND>
 struct Operand {
-    static constexpr int PARTS = KIND == MP_TYPE_F32 ? 3 : KIND == MP_TYPE_F16 ? 2 : 1;
+    static constexpr int PARTS = parts_of(KIND);
     u4 part[4][PARTS];  // 8 columns each
-    // The upper halves of two numbers.
-    static __device__ __forceinline__ uint32_t halves(float u, float v) {
-        return __builtin_amdgcn_perm(__float_as_uint(v), __float_as_uint(u), 0x07060302u);
-    }
     __device__ __forceinline__ void load(const ProductArgs& a, int64_t row, int step, int g) {
         const int column = step * kW4Step + 32 * g;
         const int64_t at = row * a.x.stride + column;
@@ -46,8 +29,8 @@ struct Operand {
 #pragma unroll
                 for (int k = 0; k < 4; k += 2) {
                     const f4 x = from_codes8(codes[s / 2][s % 2 * 2 + k / 2], scale);
-                    part[s][0][k] = halves(x[0], x[1]);
-                    part[s][0][k + 1] = halves(x[2], x[3]);
+                    part[s][0][k] = upper_halves(x[0], x[1]);
+                    part[s][0][k + 1] = upper_halves(x[2], x[3]);
                 }
         } else if constexpr (KIND == MP_TYPE_BF16) {
             const uint16_t* const from = static_cast<const uint16_t*>(a.x.data) + at;
@@ -71,7 +54,7 @@ struct Operand {
                     float u = x[k], v = x[k + 1];
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) {
-                        part[s][p][k / 2] = halves(u, v);
+                        part[s][p][k / 2] = upper_halves(u, v);
                         u -= __uint_as_float(__float_as_uint(u) & 0xFFFF0000u);
                         v -= __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
                     }
@@ -85,35 +68,16 @@ struct Operand {
 // columns 32g ..+31) times the rows' operand.
 template <int KIND>
 __device__ __forceinline__ void multiply(const u4& codes, uint32_t scale, const Operand<KIND>& x, f4* sum) {
-    // E2M1 numbers times their scale are BF16 numbers: one conversion for two.
     const float power = scale_power(scale & 0xFF);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        b2 w[4];
-        w[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[s], power, 0);
-        w[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[s], power, 1);
-        w[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[s], power, 2);
-        w[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[s], power, 3);
-        const b8 wide = {w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
+        const b8 w = weights8(codes[s], power);
 #pragma unroll
         for (int p = 0; p < Operand<KIND>::PARTS; ++p)
-            *sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide, __builtin_bit_cast(b8, x.part[s][p]), *sum, 0, 0, 0);
+            *sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, __builtin_bit_cast(b8, x.part[s][p]), *sum, 0, 0, 0);
     }
 }
 
-__device__ __forceinline__ float gated(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
-
-// Results of `row`, columns n ..+3 of a tile.
-__device__ __forceinline__ void store_result(const ProductArgs& a, int64_t row, int n, const f4& v) {
-    const int64_t at = row * a.out.stride + n;
-    if (n + 3 < a.n) {
-        store_four(a.out.data, a.out.type, a.out_wide, at, v[0], v[1], v[2], v[3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < a.n) store_one(a.out.data, a.out.type, at + i, v[i]);
-    }
-}
 // Results of `row`, columns n ..+3 and n + 16 ..+3, as 8 bits; n + 16's group of
 // 32 begins at this tile. The four lanes of a column have a row's group.
 __device__ __forceinline__ void store_result8(const ProductArgs& a, int64_t row, int n, int g, const f4& v, const f4& w,
@@ -249,7 +213,7 @@ extern "C" int mp_hip_w4_product_workspace(const mp_w4_matrix* w, int32_t type, 
         if (wrong) return refuse_call(wrong);
         if (type < MP_TYPE_F32 || type > MP_TYPE_I8) return refuse_call("rows: element type unknown or not taken here");
         if (rows < 0 || rows > kW4MostRows) return refuse_call("4-bit product: 0 to 1,048,576 rows a call");
-        *bytes = 0;
+        *bytes = rows > kW4FewRows ? w4_tiles_workspace(rows, w->depth, type) : 0;
         return MP_OK;
     });
 }
@@ -268,9 +232,17 @@ extern "C" int mp_hip_w4_product(const mp_w4_matrix* w, const mp_w4_matrix* gate
         if (rows < 0 || rows > kW4MostRows) return refuse_call("4-bit product: 0 to 1,048,576 rows a call");
         if (x->data == out->data) return refuse_call("4-bit product: no result in place of the rows");
         if (rows == 0) return MP_OK;
-        const bool pairs = out->type == MP_TYPE_I8;
+        const bool pairs = out->type == MP_TYPE_I8, tiled = w4_tiled(rows, w->rows, gate != nullptr);
+        const size_t need = tiled ? w4_tiles_workspace(rows, w->depth, x->type) : 0;
+        if (need > workspace_bytes || (need && !workspace))
+            return refuse_call("4-bit product: the workspace is smaller than mp_hip_w4_product_workspace says");
+        if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
+            return refuse_call("4-bit product: the workspace must be 16-byte aligned");
         const W4Plan p = w4_few_plan(rows, w->rows, w->depth, gate != nullptr, pairs);
-        if (w4_groups(p, rows, w->rows) > kW4MostGroups) return refuse_call("4-bit product: too large for one call");
+        if (tiled ? w4_tiles_groups(rows, w->rows, gate != nullptr) > kW4MostGroups ||
+                        w4_ceil(rows, kTileRows) * w4_ceil(w->depth, kTileDepth) > kW4MostGroups
+                  : w4_groups(p, rows, w->rows) > kW4MostGroups)
+            return refuse_call("4-bit product: too large for one call");
         ProductArgs a{};
         a.m[0] = view(*w);
         if (gate) a.m[1] = view(*gate);
@@ -282,7 +254,8 @@ extern "C" int mp_hip_w4_product(const mp_w4_matrix* w, const mp_w4_matrix* gate
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const StreamDevice device(s);
         if (device.status != hipSuccess) return call_done(device.status, "4-bit product: device of the stream");
-        if (x->type == MP_TYPE_F32) few_columns<MP_TYPE_F32>(a, p, gate != nullptr, s);
+        if (tiled) w4_tiles(a, x->type, gate != nullptr, workspace, s);
+        else if (x->type == MP_TYPE_F32) few_columns<MP_TYPE_F32>(a, p, gate != nullptr, s);
         else if (x->type == MP_TYPE_BF16) few_columns<MP_TYPE_BF16>(a, p, gate != nullptr, s);
         else if (x->type == MP_TYPE_F16) few_columns<MP_TYPE_F16>(a, p, gate != nullptr, s);
         else few_columns<MP_TYPE_I8>(a, p, gate != nullptr, s);

@@ -47,4 +47,26 @@ inline W4Plan w4_few_plan(int rows, int n, int depth, bool gated, bool pairs) {
     return p;
 }
 
+// Many rows: work-groups of 128 rows by 256 columns (128 of each matrix of a
+// gated pair), the rows laid out before in blocks of 128 rows and 64 columns:
+// 8-bit rows as two planes of E2M3 numbers, 24 bytes a lane each, and their
+// scales; float rows as 1 to 3 parts of 16 KB.
+constexpr int kW4FewRows = 64, kTileRows = 128, kTileColumns = 256, kTileDepth = 64;
+constexpr int kPlaneBytes = 64 * 24, kEightTile = 2 * kPlaneBytes + 256;  // of 32 rows
+constexpr int kEightBlock = 4 * kEightTile, kPartBlock = kTileRows * kTileDepth * 2;
+
+constexpr int w4_block_bytes(int type) {
+    return type == 3 ? kEightBlock : kPartBlock * (type == 0 ? 3 : type == 2 ? 2 : 1);  // MP_TYPE_*
+}
+constexpr size_t w4_tiles_workspace(int64_t rows, int64_t depth, int type) {
+    return (size_t)(w4_ceil(rows, kTileRows) * w4_ceil(depth, kTileDepth)) * w4_block_bytes(type);
+}
+constexpr int64_t w4_tiles_groups(int64_t rows, int64_t n, bool gated) {
+    return w4_ceil(rows, kTileRows) * w4_ceil(n, gated ? kTileColumns / 2 : kTileColumns);
+}
+// Where tiles pay.
+constexpr bool w4_tiled(int rows, int n, bool gated) {
+    return rows > kW4FewRows && w4_tiles_groups(rows, n, gated) >= 128;
+}
+
 }  // namespace mphip
