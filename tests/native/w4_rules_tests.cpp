@@ -21,14 +21,17 @@ static void few() {
                 for (int gated = 0; gated < 2; ++gated)
                     for (int pairs = 0; pairs < (n % 32 ? 1 : 2); ++pairs) {
                         const W4Plan p = w4_few_plan(rows, n, depth, gated, pairs);
-                        expect(p.column_tiles == 1 || p.column_tiles == 2 || p.column_tiles == 4, "column tiles", rows, n);
-                        expect(p.row_tiles == 1 || p.row_tiles == 2 || p.row_tiles == 4, "row tiles", rows, n);
-                        expect(!pairs || p.column_tiles % 2 == 0, "groups of 32 results lie in one block", rows, n);
+                        expect(p.side == 16 ? p.row_tiles == 1 && (p.column_tiles == 1 || p.column_tiles == 2 || p.column_tiles == 4)
+                                            : p.side == 32 && (p.row_tiles == 1 || p.row_tiles == 2) &&
+                                                  (p.column_tiles == 1 || p.column_tiles == 2),
+                               "a kernel for every plan", rows, n);
+                        expect(!gated || p.side == 16 || p.row_tiles * p.column_tiles < 4, "a gated kernel, too", rows, n);
+                        expect(!pairs || p.side * p.column_tiles % 32 == 0, "groups of 32 results lie in one block", rows, n);
                         expect(p.waves >= 1 && p.waves <= 8, "wavefronts", rows, n);
-                        expect(p.waves == 1 || p.waves <= w4_steps(depth), "a step for every wavefront", rows, depth);
-                        expect(p.waves * p.column_tiles * p.row_tiles * (gated + 1) <= 64, "partial results in 64 KB", rows, n);
-                        const int64_t columns = w4_ceil(w4_tiles(n), p.column_tiles), blocks = w4_ceil(w4_tiles(rows), p.row_tiles);
-                        expect(columns * p.column_tiles * 16 >= n && blocks * p.row_tiles * 16 >= rows, "all covered", rows, n);
+                        expect(p.waves == 1 || p.waves <= w4_ceil(depth, p.side == 16 ? 128 : 64), "work for every wavefront", rows, depth);
+                        expect(w4_few_shared(p, gated) <= 65536, "partial results in 64 KB", rows, n);
+                        const int64_t columns = w4_ceil(n, p.side * p.column_tiles), blocks = w4_ceil(rows, p.side * p.row_tiles);
+                        expect(columns * p.column_tiles * p.side >= n && blocks * p.row_tiles * p.side >= rows, "all covered", rows, n);
                         expect(w4_groups(p, rows, n) == columns * blocks, "groups", rows, n);
                     }
 }

@@ -48,8 +48,100 @@ __device__ __forceinline__ void store_result(const ProductArgs& a, int64_t row, 
     }
 }
 
-// Products of many rows: rows laid out for the matrix cores in the workspace,
-// then tiles of 256 columns and 128 rows.
-void w4_tiles(const ProductArgs& a, int kind, bool gate, void* workspace, hipStream_t s);
+// Results of `row`, columns n ..+31, as 8 bits: lane (c, g) has columns n + 16t +
+// 4g ..+3 of two tiles t of 16 columns (SIDE 16), or n + 8q + 4g ..+3 for q = 0..3
+// of one of 32 columns. All lanes of a row come together.
+template <int SIDE, int N>
+__device__ __forceinline__ void store_result8(const ProductArgs& a, int64_t row, int n, int g, const f4 (&v)[N],
+                                              bool there) {
+    static_assert(N == (SIDE == 32 ? 4 : 2));
+    uint32_t amax = 0;
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) amax = max(amax, magnitude(v[t][i]));
+    if constexpr (SIDE == 32) {
+        const auto both = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
+        amax = max((uint32_t)both[0], (uint32_t)both[1]);
+    } else {
+        amax = column_max(amax);
+    }
+    if (!there) return;
+    const uint32_t byte = scale_byte8(amax);
+    const float inverse = scale_inverse(byte);
+    uint8_t* const codes = static_cast<uint8_t*>(a.out.data) + row * a.out.stride + n + 4 * g;
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+        *reinterpret_cast<uint32_t*>(codes + 32 / N * t) = to_codes8(v[t][0], v[t][1], v[t][2], v[t][3], inverse);
+    if (g == 0) a.out.scales[row * a.out.scale_stride + n / kW4Group] = (uint8_t)byte;
+}
+
+// 8 columns of a row, as they lie and as the BF16 numbers whose sums they are.
+template <int KIND>
+struct Run8 {
+    static constexpr int BYTES = 8 * (KIND == MP_TYPE_I8 ? 1 : KIND == MP_TYPE_F32 ? 4 : 2), WORDS = BYTES / 4;
+    uint32_t raw[WORDS];
+    float scale;
+    // Zeros where there is no such row or column.
+    __device__ __forceinline__ void load(const ProductArgs& a, int64_t row, int column) {
+        if (row >= a.rows || column >= a.depth) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) raw[i] = 0;
+            scale = 0.0f;
+            return;
+        }
+        const uint8_t* const from = static_cast<const uint8_t*>(a.x.data) + (row * a.x.stride + column) * (BYTES / 8);
+        if constexpr (KIND == MP_TYPE_I8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(from);
+            raw[0] = v.x, raw[1] = v.y;
+            scale = scale_number(a.x.scales[row * a.x.scale_stride + column / kW4Group]);
+        } else if (a.x_wide) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const u4 v = reinterpret_cast<const u4*>(from)[i / 4];
+                raw[i] = v[0], raw[i + 1] = v[1], raw[i + 2] = v[2], raw[i + 3] = v[3];
+            }
+        } else if constexpr (KIND == MP_TYPE_F32) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) raw[i] = reinterpret_cast<const uint32_t*>(from)[i];
+        } else {
+            const uint16_t* const halves = reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) raw[i] = halves[2 * i] | (uint32_t)halves[2 * i + 1] << 16;
+        }
+    }
+    __device__ __forceinline__ void split(u4 (&part)[parts_of(KIND)]) const {
+        if constexpr (KIND == MP_TYPE_BF16) {
+            part[0] = u4{raw[0], raw[1], raw[2], raw[3]};
+        } else if constexpr (KIND == MP_TYPE_I8) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const f4 x = from_codes8(raw[k], scale);
+                part[0][2 * k] = upper_halves(x[0], x[1]);
+                part[0][2 * k + 1] = upper_halves(x[2], x[3]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float u, v;
+                if constexpr (KIND == MP_TYPE_F32) {
+                    u = __uint_as_float(raw[2 * k]), v = __uint_as_float(raw[2 * k + 1]);
+                } else {
+                    u = from_f16(raw[k] & 0xFFFF), v = from_f16(raw[k] >> 16);
+                }
+#pragma unroll
+                for (int p = 0; p < parts_of(KIND); ++p) {
+                    part[p][k] = upper_halves(u, v);
+                    u -= __uint_as_float(__float_as_uint(u) & 0xFFFF0000u);
+                    v -= __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+                }
+            }
+        }
+    }
+};
+
+// Products of more rows, by tiles: 256 columns by 128 rows (`large`; 8-bit rows are
+// laid out in the workspace before) or 128 by 64.
+void w4_tiles(const ProductArgs& a, int kind, bool gate, bool large, void* workspace, hipStream_t s);
 
 }  // namespace mphip

@@ -24,49 +24,56 @@ constexpr size_t w4_scale_bytes(int64_t rows, int64_t depth) { return (size_t)(w
 constexpr int64_t kRowsMostElements = (int64_t)1 << 33;
 
 // A product by wavefronts that share a block of columns and deal the depth
-// among themselves: `column_tiles` and `row_tiles` of 16 a wavefront, `waves`
+// among themselves: `column_tiles` and `row_tiles` of `side` a wavefront, `waves`
 // of them a work-group.
 struct W4Plan {
-    int column_tiles, row_tiles, waves;
+    int side, column_tiles, row_tiles, waves;
 };
 
 constexpr int64_t w4_groups(const W4Plan& p, int rows, int n) {
-    return w4_ceil(w4_tiles(n), p.column_tiles) * w4_ceil(w4_tiles(rows), p.row_tiles);
+    return w4_ceil(n, p.side * p.column_tiles) * w4_ceil(rows, p.side * p.row_tiles);
+}
+// Bytes of LDS in which a work-group's sums meet.
+constexpr size_t w4_few_shared(const W4Plan& p, bool gated) {
+    return (size_t)p.waves * p.column_tiles * p.row_tiles * (gated ? 2 : 1) * p.side * p.side * 4;
 }
 
 constexpr int64_t kW4MostGroups = 1 << 22;  // 2^31 threads of 512
 
-inline W4Plan w4_few_plan(int rows, int n, int depth, bool gated, bool pairs) {
-    const int row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    W4Plan p{4, row_tiles, 8};
-    while (p.column_tiles > (pairs ? 2 : 1) && w4_groups(p, rows, n) < 512) p.column_tiles /= 2;
-    const int64_t steps = w4_steps(depth);
-    // Partial results of all wavefronts fit 64 KB.
-    const int tiles = p.column_tiles * p.row_tiles * (gated ? 2 : 1);
-    while (p.waves > 1 && (p.waves > steps || p.waves * tiles > 64)) p.waves /= 2;
+inline W4Plan w4_few_plan(int rows, int n, int depth, bool gated, bool eight) {
+    W4Plan p{rows <= 16 ? 16 : 32, 4, rows <= 32 ? 1 : 2, 8};
+    if (p.side == 32) p.column_tiles = gated && p.row_tiles == 2 ? 1 : 2;
+    // 8-bit results: a row's group of 32 lies in one block.
+    const int least = eight && p.side == 16 ? 2 : 1;
+    while (p.column_tiles > least && w4_groups(p, rows, n) < 512) p.column_tiles /= 2;
+    const int64_t blocks = w4_ceil(depth, p.side == 16 ? 128 : 64);
+    while (p.waves > 1 && (p.waves > blocks || w4_few_shared(p, gated) > 65536)) p.waves /= 2;
     return p;
 }
 
-// Many rows: work-groups of 128 rows by 256 columns (128 of each matrix of a
-// gated pair), the rows laid out before in blocks of 128 rows and 64 columns:
-// 8-bit rows as two planes of E2M3 numbers, 24 bytes a lane each, and their
-// scales; float rows as 1 to 3 parts of 16 KB.
-constexpr int kW4FewRows = 64, kTileRows = 128, kTileColumns = 256, kTileDepth = 64;
+// More rows, by tiles that work-groups bring their rows to LDS for: 128 rows by
+// 256 columns (128 of each matrix of a gated pair), or 64 by 128, 64 columns of
+// depth at a time. For the large ones 8-bit rows are laid out before, in blocks of
+// 128 rows and 64 columns: two planes of 24 bytes a lane, and their scales.
+constexpr int kTileRows = 128, kTileColumns = 256, kTileDepth = 64;
+constexpr int kSmallTileRows = 64, kSmallTileColumns = 128;
 constexpr int kPlaneBytes = 64 * 24, kEightTile = 2 * kPlaneBytes + 256;  // of 32 rows
-constexpr int kEightBlock = 4 * kEightTile, kPartBlock = kTileRows * kTileDepth * 2;
+constexpr int kEightBlock = 4 * kEightTile;
 
-constexpr int w4_block_bytes(int type) {
-    return type == 3 ? kEightBlock : kPartBlock * (type == 0 ? 3 : type == 2 ? 2 : 1);  // MP_TYPE_*
+enum W4Way { kW4Few, kW4SmallTiles, kW4LargeTiles };
+
+constexpr int64_t w4_tile_groups(int64_t rows, int64_t n, bool gated, bool large) {
+    return large ? w4_ceil(rows, kTileRows) * w4_ceil(n, gated ? kTileColumns / 2 : kTileColumns)
+                 : w4_ceil(rows, kSmallTileRows) * w4_ceil(n, gated ? kSmallTileColumns / 2 : kSmallTileColumns);
 }
-constexpr size_t w4_tiles_workspace(int64_t rows, int64_t depth, int type) {
-    return (size_t)(w4_ceil(rows, kTileRows) * w4_ceil(depth, kTileDepth)) * w4_block_bytes(type);
+constexpr W4Way w4_way(int rows, int n, bool gated) {
+    return rows > 64 && w4_tile_groups(rows, n, gated, true) >= 256 ? kW4LargeTiles
+           : rows > 32 && w4_tile_groups(rows, n, gated, false) >= 256 ? kW4SmallTiles
+                                                                      : kW4Few;
 }
-constexpr int64_t w4_tiles_groups(int64_t rows, int64_t n, bool gated) {
-    return w4_ceil(rows, kTileRows) * w4_ceil(n, gated ? kTileColumns / 2 : kTileColumns);
-}
-// Where tiles pay.
-constexpr bool w4_tiled(int rows, int n, bool gated) {
-    return rows > kW4FewRows && w4_tiles_groups(rows, n, gated) >= 128;
+
+constexpr size_t w4_planes_bytes(int64_t rows, int64_t depth) {
+    return (size_t)(w4_ceil(rows, kTileRows) * w4_ceil(depth, kTileDepth)) * kEightBlock;
 }
 
 }  // namespace mphip

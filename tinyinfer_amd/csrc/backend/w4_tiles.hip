@@ -8,287 +8,325 @@ typedef int v8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int kThreads = 256;
-constexpr int kBlockRowTiles = kTileRows / 32;
 
-// ---- rows as operands -----------------------------------------------------------
+// ---- what the work-groups share ------------------------------------------------------
 
-// Lays rows out in blocks of 128 rows and 64 columns, [rows/128][columns/64][block]:
-// a lane (r = l%32, h = l/32) of a tile of 32 rows has row r at columns 32h ..+31.
-//
-// Float rows: [part][tile][8 columns][lane][16 bytes], BF16 numbers.
-//
-// 8-bit rows: a whole number up to 127 (or -128) is 16 times one up to 15 plus
-// another, and whole numbers up to 15 times 1/8 are E2M3 numbers whose code is
-// that number: two planes of 6-bit codes, both with the element's sign. The matrix
-// cores take E2M3 times E2M1 at twice the rate of 8-bit formats and sum such
-// products exactly before they join the FP32 sum, where an E4M3 row would lose
-// what lies 2^-13 below the largest of eight products. Per tile: the low plane
-// ([lane][16 bytes], [lane][8 bytes]), the high one, a word a lane with the scale
-// bytes of both.
-template <int KIND>
-__global__ void __launch_bounds__(kThreads) w4_layout_kernel(ProductArgs a, uint8_t* laid) {
-    const int tile = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-    const int blocks = (int)w4_ceil(a.depth, kTileDepth);
-    const int64_t row = (int64_t)(blockIdx.x / blocks) * kTileRows + tile * 32 + r;
-    const int column = blockIdx.x % blocks * kTileDepth + 32 * h;
-    const bool there = row < a.rows && column < a.depth;
-    uint8_t* const block = laid + (size_t)blockIdx.x * w4_block_bytes(KIND);
-    const int64_t at = row * a.x.stride + column;
-    if constexpr (KIND == MP_TYPE_I8) {
-        u4 codes[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-        uint32_t scale = 127;
-        if (there) {
-            const u4* const from = reinterpret_cast<const u4*>(static_cast<const uint8_t*>(a.x.data) + at);
-            codes[0] = from[0], codes[1] = from[1];
-            scale = a.x.scales[row * a.x.scale_stride + column / kW4Group];
-        }
-        uint64_t low[3] = {0, 0, 0}, high[3] = {0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-            const int x = (int8_t)(codes[k / 16][k % 16 / 4] >> (8 * (k % 4)));
-            const uint32_t m = (uint32_t)(x < 0 ? -x : x), sign = x < 0 ? 32u : 0u;
-            const uint64_t l = sign | (m & 15), u = sign | (m >> 4);
-            const int bit = 6 * k, word = bit / 64, shift = bit % 64;
-            low[word] |= l << shift, high[word] |= u << shift;
-            if (shift > 58) low[word + 1] |= l >> (64 - shift), high[word + 1] |= u >> (64 - shift);
-        }
-        uint8_t* const to = block + tile * kEightTile;
-        reinterpret_cast<ulonglong2*>(to)[lane] = make_ulonglong2(low[0], low[1]);
-        reinterpret_cast<uint64_t*>(to + 1024)[lane] = low[2];
-        reinterpret_cast<ulonglong2*>(to + kPlaneBytes)[lane] = make_ulonglong2(high[0], high[1]);
-        reinterpret_cast<uint64_t*>(to + kPlaneBytes + 1024)[lane] = high[2];
-        const bool nan = scale > kMostScale;
-        reinterpret_cast<uint32_t*>(to + 2 * kPlaneBytes)[lane] = nan ? 0xFFFFu : (scale + 3) | (scale + 7) << 8;
-    } else {
-        u4* const to = reinterpret_cast<u4*>(block + tile * (kPartBlock / kBlockRowTiles));
-        constexpr int kPart = kPartBlock / 16;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            u4 part[parts_of(KIND)];
-            if constexpr (KIND == MP_TYPE_BF16) {
-                part[0] = u4{0, 0, 0, 0};
-                if (there) {
-                    const uint16_t* const from = static_cast<const uint16_t*>(a.x.data) + at + 8 * d;
-                    if (a.x_wide) {
-                        part[0] = *reinterpret_cast<const u4*>(from);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) part[0][k] = from[2 * k] | (uint32_t)from[2 * k + 1] << 16;
-                    }
-                }
-            } else {
-                float x[8] = {};
-                if (there) load_row(a.x.data, KIND, a.x_wide, at + 8 * d, x);
-#pragma unroll
-                for (int k = 0; k < 8; k += 2) {
-                    float u = x[k], v = x[k + 1];
-#pragma unroll
-                    for (int p = 0; p < parts_of(KIND); ++p) {
-                        part[p][k / 2] = upper_halves(u, v);
-                        u -= __uint_as_float(__float_as_uint(u) & 0xFFFF0000u);
-                        v -= __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
-                    }
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < parts_of(KIND); ++p) to[p * kPart + d * 64 + lane] = part[p];
-        }
-    }
-}
-
-// ---- tiles --------------------------------------------------------------------------
-
-struct TileArgs {
-    ProductArgs p;
-    const uint8_t* laid;
-};
-
-// Results of 32 rows by 32 columns: lane (r, h) has row r at columns 8q + 4h ..+3.
-__device__ __forceinline__ void store_tile(const ProductArgs& a, int64_t row, int n, int h, const f16v& v) {
-    if (a.out.type == MP_TYPE_I8) {
-        uint32_t amax = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) amax = max(amax, magnitude(v[i]));
-        const auto both = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
-        const uint32_t byte = scale_byte8(max((uint32_t)both[0], (uint32_t)both[1]));
-        if (row >= a.rows || n >= a.n) return;
-        const float inverse = scale_inverse(byte);
-        uint8_t* const codes = static_cast<uint8_t*>(a.out.data) + row * a.out.stride + n + 4 * h;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint32_t*>(codes + 8 * q) =
-                to_codes8(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], inverse);
-        if (h == 0) a.out.scales[row * a.out.scale_stride + n / kW4Group] = (uint8_t)byte;
-    } else if (row < a.rows) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (n + 8 * q + 4 * h < a.n)
-                store_result(a, row, n + 8 * q + 4 * h, f4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
-    }
-}
-
-// A work-group of 2 x 2 wavefronts: 256 columns (of a gated pair 128 of each
-// matrix) by 128 rows. A wavefront has 4 tiles of 32 columns, whose codes come from
-// memory to its registers as they lie, and 2 tiles of 32 rows, which the work-group
-// brings to LDS, the next block while this one is multiplied.
-template <int KIND, bool GATED>
-__global__ void __launch_bounds__(kThreads, 2) w4_tiles_kernel(TileArgs t) {
-    constexpr bool EIGHT = KIND == MP_TYPE_I8;
-    constexpr int PARTS = parts_of(KIND), BLOCK = EIGHT ? kEightBlock : kPartBlock;
-    constexpr int PIECES = (BLOCK / 16 + kThreads - 1) / kThreads;  // of 16 bytes, a thread
-    __shared__ u4 rows_s[2][BLOCK / 16];
-    const ProductArgs& a = t.p;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
-    const int wave_columns = wave >> 1, wave_rows = wave & 1;
-    // Work-groups that an XCD runs together share columns and rows: each XCD has a
-    // run of blocks that goes down 8 blocks of rows before the next columns.
+// Work-groups that an XCD runs together share columns and rows: each XCD has a
+// run of blocks that goes down 8 blocks of rows before the next columns.
+__device__ __forceinline__ void find_block(const ProductArgs& a, int* row_block, int* column_block) {
     const int all = gridDim.x, xcd = blockIdx.x % 8, inside = blockIdx.x / 8;
     const int index = xcd * (all / 8) + min(xcd, all % 8) + inside;
     const int band = index / (8 * a.column_blocks), in_band = index % (8 * a.column_blocks);
     const int band_rows = min(8, a.row_blocks - 8 * band);
-    const int row_block = 8 * band + in_band % band_rows, column_block = in_band / band_rows;
-    const int steps = (int)w4_steps(a.depth), words = (int)w4_words(a.depth), blocks = (int)w4_ceil(a.depth, kTileDepth);
-    const int tiles = (int)w4_tiles(a.n);
-    // Tile i of 32 columns: of the matrix, or two of it and the same two of the gate.
-    int column[4];
-    const u4* codes[4];
-    const uint32_t* scales[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        column[i] = GATED ? column_block * 128 + wave_columns * 64 + i % 2 * 32
-                          : column_block * kTileColumns + wave_columns * 128 + i * 32;
-        // Columns behind the end are those at the end again, and not stored.
-        const int64_t tile = min(column[i] / kW4Rows + lane % 32 / 16, tiles - 1);
-        const W4View& m = a.m[GATED ? i / 2 : 0];
-        codes[i] = m.codes + tile * steps * 64 + h * 16 + lane % 16;
-        scales[i] = m.scales + tile * words * 64 + h * 16 + lane % 16;
-    }
-    const u4* const laid = reinterpret_cast<const u4*>(t.laid) + (size_t)row_block * blocks * PARTS * (BLOCK / 16);
-    f16v sum[4][2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) sum[i][j][k] = 0.0f;
+    *row_block = 8 * band + in_band % band_rows, *column_block = in_band / band_rows;
+}
 
-    u4 piece[PIECES], w[4], w_next[4];
-    uint32_t scale[4], scale_next[4];
+// A wavefront's N tiles of 32 columns from `first` on: of the matrix, or half of
+// them of it and the same of the gate. Codes come from memory to the registers as
+// they lie, lane (c, h) with row c at columns 32h ..+31 of a block of 64.
+template <int N, bool GATED>
+struct Weights {
+    static constexpr int EACH = GATED ? N / 2 : N;
+    const u4* codes_at[N];
+    const uint32_t* scales_at[N];
+    u4 codes[N];
+    uint32_t scale[N];
+    __device__ __forceinline__ void begin(const ProductArgs& a, int first) {
+        const int lane = threadIdx.x & 63, tiles = (int)w4_tiles(a.n);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            // Columns behind the end are those at the end again, and not stored.
+            const int64_t tile = min((first + i % EACH * 32) / kW4Rows + lane % 32 / 16, tiles - 1);
+            const W4View& m = a.m[i / EACH];
+            codes_at[i] = m.codes + tile * w4_steps(a.depth) * 64 + lane / 32 * 16 + lane % 16;
+            scales_at[i] = m.scales + tile * w4_words(a.depth) * 64 + lane / 32 * 16 + lane % 16;
+        }
+    }
+    __device__ __forceinline__ void load(int block) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            codes[i] = codes_at[i][block / 2 * 64 + block % 2 * 32];
+            scale[i] = scales_at[i][block / 2 / kW4Word * 64 + block % 2 * 32];
+        }
+    }
+    // The scale's byte for a block, in the lowest place.
+    static __device__ __forceinline__ uint32_t byte_of(uint32_t scale, int block) { return scale >> (8 * (block / 2 % kW4Word)); }
+};
+
+// Results of 32 rows by 32 columns: lane (r, h) has row r at columns 8q + 4h ..+3.
+__device__ __forceinline__ void store_tile(const ProductArgs& a, int64_t row, int n, int h, const f16v& v) {
+    f4 quad[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) quad[q] = f4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+    if (a.out.type == MP_TYPE_I8) {
+        store_result8<32>(a, row, n, h, quad, row < a.rows && n < a.n);
+    } else if (row < a.rows) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (n + 8 * q + 4 * h < a.n) store_result(a, row, n + 8 * q + 4 * h, quad[q]);
+    }
+}
+
+template <int N, int RT, bool GATED>
+__device__ __forceinline__ void store_tiles(const ProductArgs& a, int64_t first_row, int first_column,
+                                            const f16v (&sum)[N][RT]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (int i = 0; i < Weights<N, GATED>::EACH; ++i) {
+            f16v v = sum[i][j];
+            if constexpr (GATED) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = gated(sum[i + N / 2][j][k], v[k]);
+            }
+            store_tile(a, first_row + j * 32 + lane % 32, first_column + i * 32, lane / 32, v);
+        }
+}
+
+// ---- rows as BF16 numbers --------------------------------------------------------------
+
+// A work-group of WN x WR wavefronts has 32 N WN columns (half of them of each
+// matrix of a gated pair) by 32 RT WR rows. It brings 64 columns of its rows to
+// LDS, as the BF16 numbers whose sums they are, while the columns before are
+// multiplied.
+template <int KIND, bool GATED, int N, int RT, int WN, int WR>
+__global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a) {
+    constexpr int PARTS = parts_of(KIND), THREADS = 64 * WN * WR, TILES = RT * WR, ROWS = 32 * TILES;
+    constexpr int EACH = ROWS * 8 / THREADS;  // runs of 8 columns a thread
+    constexpr int SIZE = PARTS * TILES * 256, BUFFERS = 2 * SIZE * 16 <= 65536 ? 2 : 1;
+    __shared__ u4 rows_s[BUFFERS][SIZE];  // [part][tile][8 columns][lane]
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wave_columns = wave / WR, wave_rows = wave % WR;
+    int row_block, column_block;
+    find_block(a, &row_block, &column_block);
+    constexpr int COLUMNS = Weights<N, GATED>::EACH * 32;  // of a wavefront
+    const int first_column = (column_block * WN + wave_columns) * COLUMNS;
+    const int64_t first_row = (int64_t)row_block * ROWS;
+    Weights<N, GATED> w;
+    w.begin(a, first_column);
+    const int blocks = (int)w4_ceil(a.depth, kTileDepth);
+    f16v sum[N][RT] = {};
+
+    Run8<KIND> run[EACH];
+    // Run i of a thread: row r of a tile, columns 8e ..+7 of the block.
+    const int r = threadIdx.x % 32, e0 = threadIdx.x / 32;
+    constexpr int STEP = THREADS / 32;
+    auto load_rows = [&](int block) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int e = (e0 + i * STEP) % 8, tile = (e0 + i * STEP) / 8;
+            run[i].load(a, first_row + tile * 32 + r, block * kTileDepth + 8 * e);
+        }
+    };
+    auto keep_rows = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int e = (e0 + i * STEP) % 8, tile = (e0 + i * STEP) / 8;
+            u4 part[PARTS];
+            run[i].split(part);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                rows_s[buffer][((p * TILES + tile) * 4 + e % 4) * 64 + e / 4 * 32 + r] = part[p];
+        }
+    };
+    load_rows(0);
+    w.load(0);
+    keep_rows(0);
+    __syncthreads();
+    for (int block = 0; block < blocks; ++block) {
+        const int buffer = BUFFERS == 2 ? block & 1 : 0;
+        const bool more = block + 1 < blocks;
+        u4 codes[N];
+        float power[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            codes[i] = w.codes[i];
+            power[i] = scale_power(w.byte_of(w.scale[i], block) & 0xFF);
+        }
+        if (more) {
+            load_rows(block + 1);
+            w.load(block + 1);
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            b8 c[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) c[i] = weights8(codes[i][d], power[i]);
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    const b8 x = __builtin_bit_cast(
+                        b8, rows_s[buffer][((p * TILES + wave_rows * RT + j) * 4 + d) * 64 + lane]);
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[i], x, sum[i][j], 0, 0, 0);
+                }
+        }
+        if (BUFFERS == 1) __syncthreads();
+        if (more) keep_rows(BUFFERS == 2 ? buffer ^ 1 : 0);
+        __syncthreads();
+    }
+    store_tiles<N, RT, GATED>(a, first_row + wave_rows * RT * 32, first_column, sum);
+}
+
+// ---- 8-bit rows as planes of 6-bit numbers ------------------------------------------------
+
+// Lays rows out in blocks of 128 rows and 64 columns, [rows/128][columns/64][block]:
+// a lane (r = l%32, h = l/32) of a tile of 32 rows has row r at columns 32h ..+31.
+// A whole number up to 127 (or -128) is 16 times one up to 15 plus another, and
+// whole numbers up to 15 times 1/8 are E2M3 numbers whose code is that number: two
+// planes of 6-bit codes, both with the element's sign. The matrix cores take E2M3
+// times E2M1 at twice the rate of 8-bit formats and sum such products exactly
+// before they join the FP32 sum, where 8-bit formats lose what lies 2^-13 below the
+// largest of eight products. Per tile: the low plane ([lane][16 bytes], [lane][8
+// bytes]), the high one, a word a lane with the scale bytes of both.
+__global__ void __launch_bounds__(kThreads) w4_planes_layout_kernel(ProductArgs a, uint8_t* laid) {
+    const int tile = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int blocks = (int)w4_ceil(a.depth, kTileDepth);
+    const int64_t row = (int64_t)(blockIdx.x / blocks) * kTileRows + tile * 32 + r;
+    const int column = blockIdx.x % blocks * kTileDepth + 32 * h;
+    u4 codes[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    uint32_t scale = 127;
+    if (row < a.rows && column < a.depth) {
+        const u4* const from =
+            reinterpret_cast<const u4*>(static_cast<const uint8_t*>(a.x.data) + row * a.x.stride + column);
+        codes[0] = from[0], codes[1] = from[1];
+        scale = a.x.scales[row * a.x.scale_stride + column / kW4Group];
+    }
+    uint64_t low[3] = {0, 0, 0}, high[3] = {0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+        const int x = (int8_t)(codes[k / 16][k % 16 / 4] >> (8 * (k % 4)));
+        const uint32_t m = (uint32_t)(x < 0 ? -x : x), sign = x < 0 ? 32u : 0u;
+        const uint64_t l = sign | (m & 15), u = sign | (m >> 4);
+        const int bit = 6 * k, word = bit / 64, shift = bit % 64;
+        low[word] |= l << shift, high[word] |= u << shift;
+        if (shift > 58) low[word + 1] |= l >> (64 - shift), high[word + 1] |= u >> (64 - shift);
+    }
+    uint8_t* const to = laid + (size_t)blockIdx.x * kEightBlock + tile * kEightTile;
+    reinterpret_cast<ulonglong2*>(to)[lane] = make_ulonglong2(low[0], low[1]);
+    reinterpret_cast<uint64_t*>(to + 1024)[lane] = low[2];
+    reinterpret_cast<ulonglong2*>(to + kPlaneBytes)[lane] = make_ulonglong2(high[0], high[1]);
+    reinterpret_cast<uint64_t*>(to + kPlaneBytes + 1024)[lane] = high[2];
+    const bool nan = scale > kMostScale;
+    reinterpret_cast<uint32_t*>(to + 2 * kPlaneBytes)[lane] = nan ? 0xFFFFu : (scale + 3) | (scale + 7) << 8;
+}
+
+// A work-group of 2 x 2 wavefronts: 256 columns (of a gated pair 128 of each
+// matrix) by 128 rows. A wavefront has 4 tiles of columns and 2 of rows, which the
+// work-group brings to LDS, the next block while this one is multiplied.
+template <bool GATED>
+__global__ void __launch_bounds__(kThreads, 2) w4_planes_kernel(ProductArgs a, const uint8_t* laid_rows) {
+    constexpr int PIECES = (kEightBlock / 16 + kThreads - 1) / kThreads;  // of 16 bytes, a thread
+    __shared__ u4 rows_s[2][kEightBlock / 16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wave_columns = wave >> 1, wave_rows = wave & 1;
+    int row_block, column_block;
+    find_block(a, &row_block, &column_block);
+    constexpr int COLUMNS = Weights<4, GATED>::EACH * 32;
+    const int first_column = (column_block * 2 + wave_columns) * COLUMNS;
+    Weights<4, GATED> w;
+    w.begin(a, first_column);
+    const int blocks = (int)w4_ceil(a.depth, kTileDepth);
+    const u4* const laid = reinterpret_cast<const u4*>(laid_rows) + (size_t)row_block * blocks * (kEightBlock / 16);
+    f16v sum[4][2] = {};
+
+    u4 piece[PIECES];
     auto load_rows = [&](int block) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int at = i * kThreads + threadIdx.x;
-            if ((i + 1) * kThreads <= BLOCK / 16 || at < BLOCK / 16) piece[i] = laid[(size_t)block * (BLOCK / 16) + at];
+            if ((i + 1) * kThreads <= kEightBlock / 16 || at < kEightBlock / 16)
+                piece[i] = laid[(size_t)block * (kEightBlock / 16) + at];
         }
     };
     auto keep_rows = [&](int buffer) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int at = i * kThreads + threadIdx.x;
-            if ((i + 1) * kThreads <= BLOCK / 16 || at < BLOCK / 16) rows_s[buffer][at] = piece[i];
-        }
-    };
-    auto load_weights = [&](int block) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w_next[i] = codes[i][block / 2 * 64 + block % 2 * 32];
-            scale_next[i] = scales[i][block / 2 / kW4Word * 64 + block % 2 * 32];
+            if ((i + 1) * kThreads <= kEightBlock / 16 || at < kEightBlock / 16) rows_s[buffer][at] = piece[i];
         }
     };
     load_rows(0);
-    load_weights(0);
+    w.load(0);
     keep_rows(0);
     __syncthreads();
-    int buffer = 0;
     for (int block = 0; block < blocks; ++block) {
+        const bool more = block + 1 < blocks;
+        u4 codes[4];
+        int scale[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = w_next[i];
-            scale[i] = scale_next[i] >> (8 * (block / 2 % kW4Word));
+            codes[i] = w.codes[i];
+            scale[i] = (int)w.byte_of(w.scale[i], block);
         }
-#pragma unroll 1
-        for (int p = 0; p < PARTS; ++p) {
-            const bool more = block + 1 < blocks || p + 1 < PARTS;
-            if (more) load_rows(block * PARTS + p + 1);
-            if (p == 0 && block + 1 < blocks) load_weights(block + 1);
-            const uint8_t* const from = reinterpret_cast<const uint8_t*>(rows_s[buffer]);
-            if constexpr (EIGHT) {
+        if (more) {
+            load_rows(block + 1);
+            w.load(block + 1);
+        }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint8_t* const tile = from + (wave_rows * 2 + j) * kEightTile;
-                    const int power = reinterpret_cast<const int*>(tile + 2 * kPlaneBytes)[lane];
+        for (int j = 0; j < 2; ++j) {
+            const uint8_t* const tile =
+                reinterpret_cast<const uint8_t*>(rows_s[block & 1]) + (wave_rows * 2 + j) * kEightTile;
+            const int power = reinterpret_cast<const int*>(tile + 2 * kPlaneBytes)[lane];
 #pragma unroll
-                    for (int plane = 0; plane < 2; ++plane) {
-                        const u4 x = reinterpret_cast<const u4*>(tile + plane * kPlaneBytes)[lane];
-                        const uint2 y = reinterpret_cast<const uint2*>(tile + plane * kPlaneBytes + 1024)[lane];
-                        const v8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y.x, (int)y.y, 0, 0};
+            for (int plane = 0; plane < 2; ++plane) {
+                const u4 x = reinterpret_cast<const u4*>(tile + plane * kPlaneBytes)[lane];
+                const uint2 y = reinterpret_cast<const uint2*>(tile + plane * kPlaneBytes + 1024)[lane];
+                const v8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y.x, (int)y.y, 0, 0};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const v8 c = {(int)w[i][0], (int)w[i][1], (int)w[i][2], (int)w[i][3], 0, 0, 0, 0};
-                            // Formats 4 and 2: E2M1 and E2M3.
-                            sum[i][j] = plane == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                                                         c, b, sum[i][j], 4, 2, 0, (int)scale[i], 0, power)
-                                                   : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                                                         c, b, sum[i][j], 4, 2, 0, (int)scale[i], 1, power);
-                        }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    b8 x[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        x[j] = reinterpret_cast<const b8*>(from)[((wave_rows * 2 + j) * 4 + d) * 64 + lane];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const b8 c = weights8(w[i][d], scale_power(scale[i] & 0xFF));
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-                            sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c, x[j], sum[i][j], 0, 0, 0);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const v8 c = {(int)codes[i][0], (int)codes[i][1], (int)codes[i][2], (int)codes[i][3], 0, 0, 0, 0};
+                    // Formats 4 and 2: E2M1 and E2M3; the scales' bytes 0, and 0 or 1.
+                    sum[i][j] = plane == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(c, b, sum[i][j], 4, 2, 0,
+                                                                                             scale[i], 0, power)
+                                           : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(c, b, sum[i][j], 4, 2, 0,
+                                                                                             scale[i], 1, power);
                 }
             }
-            if (more) keep_rows(buffer ^ 1);
-            __syncthreads();
-            buffer ^= 1;
         }
+        if (more) keep_rows((block & 1) ^ 1);
+        __syncthreads();
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t row = (int64_t)row_block * kTileRows + wave_rows * 64 + j * 32 + lane % 32;
-#pragma unroll
-        for (int i = 0; i < (GATED ? 2 : 4); ++i) {
-            f16v v = sum[i][j];
-            if constexpr (GATED) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = gated(sum[i + 2][j][k], v[k]);
-            }
-            store_tile(a, row, column[i], h, v);
-        }
-    }
+    store_tiles<4, 2, GATED>(a, (int64_t)row_block * kTileRows + wave_rows * 64, first_column, sum);
 }
 
+void blocks_of(ProductArgs* a, int rows, int columns) {
+    a->row_blocks = (int)w4_ceil(a->rows, rows);
+    a->column_blocks = (int)w4_ceil(a->n, columns);
+}
+
+template <int KIND, bool GATED>
+void tiles(ProductArgs a, bool large, hipStream_t s) {
+    blocks_of(&a, large ? kTileRows : kSmallTileRows, (large ? kTileColumns : kSmallTileColumns) / (GATED ? 2 : 1));
+    const unsigned groups = (unsigned)(a.row_blocks * (int64_t)a.column_blocks);
+    if constexpr (KIND != MP_TYPE_I8) {  // whose large tiles have planes
+        if (large) return w4_tiles_kernel<KIND, GATED, 4, 2, 2, 2><<<groups, 256, 0, s>>>(a);
+    }
+    w4_tiles_kernel<KIND, GATED, 2, 1, 2, 2><<<groups, 256, 0, s>>>(a);
+}
 template <int KIND>
-void tiles(const TileArgs& t, bool gate, uint8_t* laid, hipStream_t s) {
-    const unsigned blocks = (unsigned)(t.p.row_blocks * w4_ceil(t.p.depth, kTileDepth));
-    w4_layout_kernel<KIND><<<blocks, kThreads, 0, s>>>(t.p, laid);
-    const unsigned groups = (unsigned)(t.p.row_blocks * (int64_t)t.p.column_blocks);
-    if (gate) w4_tiles_kernel<KIND, true><<<groups, kThreads, 0, s>>>(t);
-    else w4_tiles_kernel<KIND, false><<<groups, kThreads, 0, s>>>(t);
+void tiles(const ProductArgs& a, bool gate, bool large, hipStream_t s) {
+    if (gate) tiles<KIND, true>(a, large, s);
+    else tiles<KIND, false>(a, large, s);
+}
+template <bool GATED>
+void planes(ProductArgs a, uint8_t* laid, hipStream_t s) {
+    blocks_of(&a, kTileRows, kTileColumns / (GATED ? 2 : 1));
+    w4_planes_layout_kernel<<<(unsigned)(a.row_blocks * w4_ceil(a.depth, kTileDepth)), kThreads, 0, s>>>(a, laid);
+    w4_planes_kernel<GATED><<<(unsigned)(a.row_blocks * (int64_t)a.column_blocks), kThreads, 0, s>>>(a, laid);
 }
 
 }  // namespace
 
-void w4_tiles(const ProductArgs& a, int kind, bool gate, void* workspace, hipStream_t s) {
-    TileArgs t{a, static_cast<const uint8_t*>(workspace)};
-    t.p.row_blocks = (int)w4_ceil(a.rows, kTileRows);
-    t.p.column_blocks = (int)w4_ceil(a.n, gate ? kTileColumns / 2 : kTileColumns);
+void w4_tiles(const ProductArgs& a, int kind, bool gate, bool large, void* workspace, hipStream_t s) {
     uint8_t* const laid = static_cast<uint8_t*>(workspace);
-    if (kind == MP_TYPE_F32) tiles<MP_TYPE_F32>(t, gate, laid, s);
-    else if (kind == MP_TYPE_BF16) tiles<MP_TYPE_BF16>(t, gate, laid, s);
-    else if (kind == MP_TYPE_F16) tiles<MP_TYPE_F16>(t, gate, laid, s);
-    else tiles<MP_TYPE_I8>(t, gate, laid, s);
+    if (kind == MP_TYPE_F32) tiles<MP_TYPE_F32>(a, gate, large, s);
+    else if (kind == MP_TYPE_BF16) tiles<MP_TYPE_BF16>(a, gate, large, s);
+    else if (kind == MP_TYPE_F16) tiles<MP_TYPE_F16>(a, gate, large, s);
+    else if (!large) tiles<MP_TYPE_I8>(a, gate, false, s);
+    else if (gate) planes<true>(a, laid, s);
+    else planes<false>(a, laid, s);
 }
 
 }  // namespace mphip
