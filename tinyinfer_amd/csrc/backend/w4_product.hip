@@ -5,16 +5,6 @@
 namespace mphip {
 namespace {
 
-// 32 columns of a row.
-template <int KIND>
-struct Columns {
-    Run8<KIND> run[4];
-    __device__ __forceinline__ void load(const ProductArgs& a, int64_t row, int column) {
-#pragma unroll
-        for (int d = 0; d < 4; ++d) run[d].load(a, row, column + 8 * d);
-    }
-};
-
 // Tiles of 16 by 16 (128 columns of depth a step, lane (c, g) of a tile with row
 // c at columns 32g ..+31), and of 32 by 32 (64 columns, lane (r, h) with row r at
 // columns 32h ..+31), which take less time an operation.
@@ -41,22 +31,27 @@ struct Tile<32> {
     }
 };
 
-// A work-group has NT tiles of columns and RT of rows; its wavefronts deal the
+// A work-group has NT tiles of columns and one of rows; its wavefronts deal the
 // depth among themselves, each with all of the block's sums, which meet in LDS at
-// the end, in the wavefronts' order. What the next step needs is on its way while
-// this one is multiplied.
-template <int KIND, int SIDE, int NT, int RT, bool GATED>
+// the end, in the wavefronts' order.
+//
+// A wavefront reads its rows along their columns, whole lines of memory at a time
+// (16 bytes of 64 rows take four times as long), and turns them into operands on
+// the way through LDS of its own, so that wavefronts do not wait for each other.
+// Of a tile that is not full only the rows that are there are kept. What the next
+// block of depth needs is on its way while this one is multiplied.
+template <int KIND, int SIDE, int NT, bool GATED>
 __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
     typedef Tile<SIDE> T;
-    constexpr int M = GATED ? 2 : 1, Q = T::QUADS, UNITS = M * NT * RT * Q, PARTS = parts_of(KIND);
-    extern __shared__ f4 parts_s[];  // [wavefront][matrix][column tile][row tile][quad][lane]
+    constexpr int M = GATED ? 2 : 1, Q = T::QUADS, UNITS = M * NT * Q, PARTS = parts_of(KIND);
+    constexpr int RUNS = T::DEPTH / 8, EACH = SIDE * RUNS / 64, ROWS_EACH = 64 / RUNS;
+    extern __shared__ u4 shared_s[];  // [wavefront][part][run][row]; at the end [wavefront][matrix][tile][quad][lane]
     const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane % SIDE, g = lane / SIDE;
     const int column_block = blockIdx.x / a.row_blocks, row_block = blockIdx.x % a.row_blocks;
     const int tiles = (int)w4_tiles(a.n), steps = (int)w4_steps(a.depth), words = (int)w4_words(a.depth);
-    // Tiles and rows behind the end are those at the end again, and not stored.
+    // Columns behind the end are those at the end again, and not stored.
     const u4* codes_at[M][NT];
     const uint32_t* scales_at[M][NT];
-    int64_t row[RT];
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -65,68 +60,91 @@ __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
             codes_at[m][i] = a.m[m].codes + tile * steps * 64 + g * 16 + c % 16;
             scales_at[m][i] = a.m[m].scales + tile * words * 64 + g * 16 + c % 16;
         }
-#pragma unroll
-    for (int j = 0; j < RT; ++j) row[j] = min((row_block * RT + j) * SIDE + c, a.rows - 1);
-    typename T::Sum sum[M][NT][RT] = {};
+    typename T::Sum sum[M][NT] = {};
     // Blocks of DEPTH columns: halves of a step with tiles of 32.
     constexpr int HALVES = kW4Step / T::DEPTH;
     const int blocks = (int)w4_ceil(a.depth, T::DEPTH);
     const int first = blocks * wave / waves, last = blocks * (wave + 1) / waves;
-    struct Block {
-        u4 codes[M][NT];
-        uint32_t scale[M][NT];
-        Columns<KIND> x[RT];
-    } next;
+    // Rows of this tile, and the power of two that their places in LDS take:
+    // row r of run e lies at r ^ e, so that neither rows nor runs share banks.
+    const int rows = min(a.rows - row_block * SIDE, SIDE), places = w4_places(rows), mask = places - 1;
+    u4* const mine = shared_s + wave * (PARTS * RUNS) * places;
+    const int run_of = lane % RUNS, row_of = lane / RUNS;
+    u4 codes[M][NT];
+    uint32_t scale[M][NT];
+    Run8<KIND> run[EACH];
     auto load = [&](int block) {
         const int step = block / HALVES, half = block % HALVES;
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                next.codes[m][i] = codes_at[m][i][step * 64 + half * 32];
-                next.scale[m][i] = scales_at[m][i][step / kW4Word * 64 + half * 32];
+                codes[m][i] = codes_at[m][i][step * 64 + half * 32];
+                scale[m][i] = scales_at[m][i][step / kW4Word * 64 + half * 32];
             }
 #pragma unroll
-        for (int j = 0; j < RT; ++j) next.x[j].load(a, row[j], block * T::DEPTH + 32 * g);
+        for (int i = 0; i < EACH; ++i)
+            if (i * ROWS_EACH < rows)
+                run[i].load(a, (int64_t)row_block * SIDE + i * ROWS_EACH + row_of, block * T::DEPTH + 8 * run_of);
     };
     if (first < last) load(first);
     for (int block = first; block < last; ++block) {
-        const Block now = next;
-        if (block + 1 < last) load(block + 1);
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int r = i * ROWS_EACH + row_of;
+            if (i * ROWS_EACH < rows && r < places) {
+                u4 part[PARTS];
+                run[i].split(part);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) mine[(p * RUNS + run_of) * places + (r ^ (run_of & mask))] = part[p];
+            }
+        }
+        wave_sync();
+        u4 now[M][NT];
+        float power[M][NT];
         const int shift = 8 * (block / HALVES % kW4Word);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            u4 x[RT][PARTS];
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int j = 0; j < RT; ++j) now.x[j].run[d].split(x[j]);
+            for (int i = 0; i < NT; ++i) {
+                now[m][i] = codes[m][i];
+                power[m][i] = scale_power(scale[m][i] >> shift & 0xFF);
+            }
+        if (block + 1 < last) load(block + 1);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            b8 x[PARTS];
+            const int e = 4 * g + d;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                x[p] = __builtin_bit_cast(b8, mine[(p * RUNS + e) * places + ((c ^ e) & mask)]);
 #pragma unroll
             for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    const b8 w = weights8(now.codes[m][i][d], scale_power(now.scale[m][i] >> shift & 0xFF));
+                    const b8 w = weights8(now[m][i][d], power[m][i]);
 #pragma unroll
-                    for (int j = 0; j < RT; ++j)
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p) T::add(w, __builtin_bit_cast(b8, x[j][p]), &sum[m][i][j]);
+                    for (int p = 0; p < PARTS; ++p) T::add(w, x[p], &sum[m][i]);
                 }
         }
     }
+    f4* const parts_s = reinterpret_cast<f4*>(shared_s);
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int j = 0; j < RT; ++j)
-#pragma unroll
-                for (int q = 0; q < Q; ++q)
-                    parts_s[(wave * UNITS + ((m * NT + i) * RT + j) * Q + q) * 64 + lane] = T::quad(sum[m][i][j], q);
+            for (int q = 0; q < Q; ++q)
+                parts_s[(wave * UNITS + (m * NT + i) * Q + q) * 64 + lane] = T::quad(sum[m][i], q);
     __syncthreads();
-    auto joined = [&](int i, int j, int q) {
+    auto joined = [&](int i, int q) {
         f4 v[M];
 #pragma unroll
         for (int m = 0; m < M; ++m) {
             v[m] = f4{0.f, 0.f, 0.f, 0.f};
-            for (int w = 0; w < waves; ++w) v[m] += parts_s[(w * UNITS + ((m * NT + i) * RT + j) * Q + q) * 64 + lane];
+            for (int w = 0; w < waves; ++w) v[m] += parts_s[(w * UNITS + (m * NT + i) * Q + q) * 64 + lane];
         }
         if constexpr (GATED) {
 #pragma unroll
@@ -134,56 +152,49 @@ __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
         }
         return v[0];
     };
+    const int64_t row = (int64_t)row_block * SIDE + c;
     if (a.out.type == MP_TYPE_I8) {
         // A row's group of 32: two tiles of 16 columns, or one of 32.
         if constexpr (SIDE == 32) {
-            for (int unit = wave; unit < NT * RT; unit += waves) {
-                const int i = unit / RT, j = unit % RT, r = (row_block * RT + j) * SIDE + c;
+            for (int i = wave; i < NT; i += waves) {
                 const int n = (column_block * NT + i) * SIDE;
                 f4 v[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) v[q] = joined(i, j, q);
-                store_result8<32>(a, r, n, g, v, r < a.rows && n < a.n);
+                for (int q = 0; q < 4; ++q) v[q] = joined(i, q);
+                store_result8<32>(a, row, n, g, v, c < rows && n < a.n);
             }
         } else if constexpr (NT % 2 == 0) {
-            for (int unit = wave; unit < NT / 2 * RT; unit += waves) {
-                const int i = unit / RT * 2, j = unit % RT, r = (row_block * RT + j) * SIDE + c;
+            for (int i = 2 * wave; i < NT; i += 2 * waves) {
                 const int n = (column_block * NT + i) * SIDE;
-                const f4 v[2] = {joined(i, j, 0), joined(i + 1, j, 0)};
-                store_result8<16>(a, r, n, g, v, r < a.rows && n < a.n);
+                const f4 v[2] = {joined(i, 0), joined(i + 1, 0)};
+                store_result8<16>(a, row, n, g, v, c < rows && n < a.n);
             }
         }
     } else {
-        for (int unit = wave; unit < NT * RT * Q; unit += waves) {
-            const int q = unit % Q, j = unit / Q % RT, i = unit / Q / RT, r = (row_block * RT + j) * SIDE + c;
-            const int n = (column_block * NT + i) * SIDE + 8 * q + 4 * g;
-            const f4 v = joined(i, j, q);
-            if (r < a.rows && n < a.n) store_result(a, r, n, v);
+        for (int unit = wave; unit < NT * Q; unit += waves) {
+            const int n = (column_block * NT + unit / Q) * SIDE + 8 * (unit % Q) + 4 * g;
+            const f4 v = joined(unit / Q, unit % Q);
+            if (c < rows && n < a.n) store_result(a, row, n, v);
         }
     }
 }
 
-template <int KIND, int SIDE, int NT, int RT>
+template <int KIND, int SIDE, int NT>
 void few(const ProductArgs& a, const W4Plan& p, bool gate, hipStream_t s) {
     const unsigned groups = (unsigned)(a.column_blocks * (int64_t)a.row_blocks);
-    const size_t shared = w4_few_shared(p, gate);
-    if constexpr (NT * RT < 4 || SIDE == 16) {
-        if (gate) return w4_few_kernel<KIND, SIDE, NT, RT, true><<<groups, 64 * p.waves, shared, s>>>(a);
-    }
-    w4_few_kernel<KIND, SIDE, NT, RT, false><<<groups, 64 * p.waves, shared, s>>>(a);
+    const size_t shared = w4_few_shared(p, a.rows, parts_of(KIND), gate);
+    if (gate) w4_few_kernel<KIND, SIDE, NT, true><<<groups, 64 * p.waves, shared, s>>>(a);
+    else w4_few_kernel<KIND, SIDE, NT, false><<<groups, 64 * p.waves, shared, s>>>(a);
 }
 template <int KIND>
 void few_tiles(const ProductArgs& a, const W4Plan& p, bool gate, hipStream_t s) {
-    if (p.side == 16) {
-        if (p.column_tiles == 1) few<KIND, 16, 1, 1>(a, p, gate, s);
-        else if (p.column_tiles == 2) few<KIND, 16, 2, 1>(a, p, gate, s);
-        else few<KIND, 16, 4, 1>(a, p, gate, s);
-    } else if (p.row_tiles == 1) {
-        if (p.column_tiles == 1) few<KIND, 32, 1, 1>(a, p, gate, s);
-        else few<KIND, 32, 2, 1>(a, p, gate, s);
+    if (p.side == 32) {
+        if (p.column_tiles == 1) few<KIND, 32, 1>(a, p, gate, s);
+        else few<KIND, 32, 2>(a, p, gate, s);
     } else {
-        if (p.column_tiles == 1) few<KIND, 32, 1, 2>(a, p, gate, s);
-        else few<KIND, 32, 2, 2>(a, p, gate, s);
+        if (p.column_tiles == 1) few<KIND, 16, 1>(a, p, gate, s);
+        else if (p.column_tiles == 2) few<KIND, 16, 2>(a, p, gate, s);
+        else few<KIND, 16, 4>(a, p, gate, s);
     }
 }
 
@@ -229,7 +240,7 @@ extern "C" int mp_hip_w4_product(const mp_w4_matrix* w, const mp_w4_matrix* gate
             return refuse_call("4-bit product: the workspace is smaller than mp_hip_w4_product_workspace says");
         if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
             return refuse_call("4-bit product: the workspace must be 16-byte aligned");
-        const W4Plan p = w4_few_plan(rows, w->rows, w->depth, gate != nullptr, out->type == MP_TYPE_I8);
+        const W4Plan p = w4_few_plan(rows, w->rows, w->depth, parts_of(x->type), gate != nullptr, out->type == MP_TYPE_I8);
         const int64_t groups = way == kW4Few ? w4_groups(p, rows, w->rows)
                                              : w4_tile_groups(rows, w->rows, gate != nullptr, way == kW4LargeTiles);
         if (groups > kW4MostGroups || (planes && need / kEightBlock > kW4MostGroups))
@@ -241,7 +252,7 @@ extern "C" int mp_hip_w4_product(const mp_w4_matrix* w, const mp_w4_matrix* gate
         a.x = rows_view(*x), a.out = rows_view(*out);
         a.x_wide = rows_wide(*x), a.out_wide = rows_wide(*out);
         a.column_blocks = (int)w4_ceil(a.n, p.side * p.column_tiles);
-        a.row_blocks = (int)w4_ceil(rows, p.side * p.row_tiles);
+        a.row_blocks = (int)w4_ceil(rows, p.side);
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const StreamDevice device(s);
         if (device.status != hipSuccess) return call_done(device.status, "4-bit product: device of the stream");

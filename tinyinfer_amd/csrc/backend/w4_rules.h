@@ -24,30 +24,36 @@ constexpr size_t w4_scale_bytes(int64_t rows, int64_t depth) { return (size_t)(w
 constexpr int64_t kRowsMostElements = (int64_t)1 << 33;
 
 // A product by wavefronts that share a block of columns and deal the depth
-// among themselves: `column_tiles` and `row_tiles` of `side` a wavefront, `waves`
-// of them a work-group.
+// among themselves: `column_tiles` tiles of `side` columns and rows a wavefront,
+// `waves` of them a work-group.
 struct W4Plan {
-    int side, column_tiles, row_tiles, waves;
+    int side, column_tiles, waves;
 };
 
 constexpr int64_t w4_groups(const W4Plan& p, int rows, int n) {
-    return w4_ceil(n, p.side * p.column_tiles) * w4_ceil(rows, p.side * p.row_tiles);
+    return w4_ceil(n, p.side * p.column_tiles) * w4_ceil(rows, p.side);
 }
-// Bytes of LDS in which a work-group's sums meet.
-constexpr size_t w4_few_shared(const W4Plan& p, bool gated) {
-    return (size_t)p.waves * p.column_tiles * p.row_tiles * (gated ? 2 : 1) * p.side * p.side * 4;
+// Places that a tile's rows take in LDS: a power of two, and all 8 runs of a
+// tile of 32 rows have one of their own.
+constexpr int w4_places(int rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+// Bytes of LDS: a wavefront's rows as operands (`parts` BF16 numbers an element),
+// at the end the sums that meet.
+constexpr size_t w4_few_shared(const W4Plan& p, int rows, int parts, bool gated) {
+    const int side = p.side, inside = rows < side ? rows : side;
+    const size_t operands = (size_t)p.waves * parts * (side == 16 ? 16 : 8) * w4_places(inside) * 16;
+    const size_t sums = (size_t)p.waves * p.column_tiles * (gated ? 2 : 1) * side * side * 4;
+    return operands > sums ? operands : sums;
 }
 
 constexpr int64_t kW4MostGroups = 1 << 22;  // 2^31 threads of 512
 
-inline W4Plan w4_few_plan(int rows, int n, int depth, bool gated, bool eight) {
-    W4Plan p{rows <= 16 ? 16 : 32, 4, rows <= 32 ? 1 : 2, 8};
-    if (p.side == 32) p.column_tiles = gated && p.row_tiles == 2 ? 1 : 2;
+inline W4Plan w4_few_plan(int rows, int n, int depth, int parts, bool gated, bool eight) {
+    W4Plan p{rows <= 16 ? 16 : 32, rows <= 16 ? 4 : 2, 8};
     // 8-bit results: a row's group of 32 lies in one block.
     const int least = eight && p.side == 16 ? 2 : 1;
     while (p.column_tiles > least && w4_groups(p, rows, n) < 512) p.column_tiles /= 2;
     const int64_t blocks = w4_ceil(depth, p.side == 16 ? 128 : 64);
-    while (p.waves > 1 && (p.waves > blocks || w4_few_shared(p, gated) > 65536)) p.waves /= 2;
+    while (p.waves > 1 && (p.waves > blocks || w4_few_shared(p, rows, parts, gated) > 65536)) p.waves /= 2;
     return p;
 }
 

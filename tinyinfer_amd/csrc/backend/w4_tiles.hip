@@ -95,8 +95,9 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a
     constexpr int PARTS = parts_of(KIND), THREADS = 64 * WN * WR, TILES = RT * WR, ROWS = 32 * TILES;
     constexpr int EACH = ROWS * 8 / THREADS;  // runs of 8 columns a thread
     constexpr int SIZE = PARTS * TILES * 256, BUFFERS = 2 * SIZE * 16 <= 65536 ? 2 : 1;
-    __shared__ u4 rows_s[BUFFERS][SIZE];  // [part][tile][8 columns][lane]
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wave_columns = wave / WR, wave_rows = wave % WR;
+    __shared__ u4 rows_s[BUFFERS][SIZE];  // [part][tile][run of 8 columns][row]
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane / 32;
+    const int wave_columns = wave / WR, wave_rows = wave % WR;
     int row_block, column_block;
     find_block(a, &row_block, &column_block);
     constexpr int COLUMNS = Weights<N, GATED>::EACH * 32;  // of a wavefront
@@ -108,25 +109,23 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a
     f16v sum[N][RT] = {};
 
     Run8<KIND> run[EACH];
-    // Run i of a thread: row r of a tile, columns 8e ..+7 of the block.
-    const int r = threadIdx.x % 32, e0 = threadIdx.x / 32;
-    constexpr int STEP = THREADS / 32;
+    // Run i of a thread: columns 8e ..+7 of the block of a row, so that neighbours
+    // read a line of memory. In LDS row r of run e lies at r ^ e: neither rows nor
+    // runs share banks.
+    const int e = threadIdx.x % 8, r0 = threadIdx.x / 8;
     auto load_rows = [&](int block) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int e = (e0 + i * STEP) % 8, tile = (e0 + i * STEP) / 8;
-            run[i].load(a, first_row + tile * 32 + r, block * kTileDepth + 8 * e);
-        }
+        for (int i = 0; i < EACH; ++i) run[i].load(a, first_row + r0 + i * (THREADS / 8), block * kTileDepth + 8 * e);
     };
     auto keep_rows = [&](int buffer) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int e = (e0 + i * STEP) % 8, tile = (e0 + i * STEP) / 8;
+            const int r = r0 + i * (THREADS / 8);
             u4 part[PARTS];
             run[i].split(part);
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
-                rows_s[buffer][((p * TILES + tile) * 4 + e % 4) * 64 + e / 4 * 32 + r] = part[p];
+                rows_s[buffer][((p * TILES + r / 32) * 8 + e) * 32 + (r % 32 ^ e)] = part[p];
         }
     };
     load_rows(0);
@@ -157,7 +156,7 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                     const b8 x = __builtin_bit_cast(
-                        b8, rows_s[buffer][((p * TILES + wave_rows * RT + j) * 4 + d) * 64 + lane]);
+                        b8, rows_s[buffer][((p * TILES + wave_rows * RT + j) * 8 + h * 4 + d) * 32 + (lane % 32 ^ (h * 4 + d))]);
 #pragma unroll
                     for (int i = 0; i < N; ++i)
                         sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[i], x, sum[i][j], 0, 0, 0);
