@@ -72,7 +72,7 @@ static void ways() {
                 large = now;
             }
         }
-    expect(w4_planes_bytes(129, 65) == (size_t)4 * kEightBlock && kEightBlock == 13312, "planes");
+    expect(w4_planes_bytes(129, 65) == (size_t)4 * 12288 + 2 * 1024 && kPlanesBlock == 12288, "planes");
 }
 
 int main() {

@@ -276,10 +276,10 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(NormArgs a, int waves) {
 
 template <int TYPE, int OUT, bool RESIDUAL, bool WIDE>
 hipError_t norm(const NormArgs& a, hipStream_t s) {
-    // Up to 1,024 elements a wavefront of its own, four rows a work-group.
-    if (a.width <= 512) rms_norm_kernel<TYPE, OUT, RESIDUAL, WIDE, 1><<<(a.rows + 3) / 4, 256, 0, s>>>(a, 1);
-    else if (a.width <= 1024) rms_norm_kernel<TYPE, OUT, RESIDUAL, WIDE, 2><<<(a.rows + 3) / 4, 256, 0, s>>>(a, 1);
-    else if (a.width <= 4096) rms_norm_kernel<TYPE, OUT, RESIDUAL, WIDE, 2><<<a.rows, 256, 0, s>>>(a, 4);
+    // A wavefront for 512 elements, up to 16 of them; short rows four a work-group.
+    const int waves = (int)w4_ceil(a.width, 64 * kEach);
+    if (waves == 1) rms_norm_kernel<TYPE, OUT, RESIDUAL, WIDE, 1><<<(a.rows + 3) / 4, 256, 0, s>>>(a, 1);
+    else if (waves <= 16) rms_norm_kernel<TYPE, OUT, RESIDUAL, WIDE, 1><<<a.rows, 64 * waves, 0, s>>>(a, waves);
     else rms_norm_kernel<TYPE, OUT, RESIDUAL, WIDE, 2><<<a.rows, 1024, 0, s>>>(a, 16);
     return hipGetLastError();
 }

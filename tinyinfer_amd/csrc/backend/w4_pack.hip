@@ -17,76 +17,73 @@ struct PackArgs {
     bool wide;
 };
 
-// A wavefront takes 16 rows by 512 columns, four tiles and the words of their
-// scales. It reads each row's groups by 16 bytes a lane (8 lanes a group in
-// FP32, 4 in 16 bits; whole lines of memory), and turns the codes round through
-// LDS: there a lane of the result finds the 16 bytes of its row and group.
+// A wavefront takes a tile, 16 rows by 128 columns. It reads each row's groups by
+// 16 bytes a lane (8 lanes a group in FP32, 4 in 16 bits; whole lines of memory),
+// and turns the codes round through LDS: there a lane of the result finds the 16
+// bytes of its row and group.
 //
 // Reads 4 (or 2) bytes an element and writes 17/32, which bounds it.
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads) w4_pack_kernel(PackArgs a) {
     constexpr int V = TYPE == MP_TYPE_F32 ? 4 : 8, L = kW4Group / V, RPI = 64 / L;  // elements, lanes a group, rows a load
     __shared__ u4 codes_s[kThreads / 64][64];
-    __shared__ uint32_t scales_s[kThreads / 64][64];
+    __shared__ uint8_t scales_s[kThreads / 64][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15;
     const int words = (int)w4_words(a.depth), steps = (int)w4_steps(a.depth);
     const int64_t item = (int64_t)blockIdx.x * (kThreads / 64) + wave;
-    const int tile = (int)(item / words) + a.first / kW4Rows, word = (int)(item % words);
+    const int tile = (int)(item / steps) + a.first / kW4Rows, step = (int)(item % steps);
     const int last = a.first + a.count;
     if (tile * kW4Rows >= last) return;  // a wavefront behind the end: nothing here waits for it
     uint8_t* const code_bytes = reinterpret_cast<uint8_t*>(codes_s[wave]);
-    uint8_t* const scale_bytes = reinterpret_cast<uint8_t*>(scales_s[wave]);
-    // Rows that fill the last tile up are written with the matrix's last row, as zeros.
-    const int row = tile * kW4Rows + c;
-    const bool writes = row >= a.first && (row < last || last == a.rows);
-    scales_s[wave][lane] = 0;
+    float x[4][kW4Rows / RPI][V];
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int h = 0; h < kW4Rows / RPI; ++h) {
+            const int r = tile * kW4Rows + h * RPI + lane / L, column = step * kW4Step + b * kW4Group;
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[b][h][i] = 0.0f;
+            if (r >= a.first && r < last && column < a.depth)
+                load_row(a.x, TYPE, a.wide, (r - a.first) * a.x_stride + column + V * (lane % L), x[b][h]);
+        }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int h = 0; h < kW4Rows / RPI; ++h) {
+            const int inside = h * RPI + lane / L;
+            uint32_t amax = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) amax = max(amax, magnitude(x[b][h][i]));
+            amax = max(amax, dpp_u<kDppQuadXor1>(amax));
+            amax = max(amax, dpp_u<kDppQuadXor2>(amax));
+            if (L == 8) amax = max(amax, dpp_u<kDppHalfMirror>(amax));
+            const uint32_t byte = scale_byte4(amax);
+            const float scale = scale_power(byte);
+            uint32_t code = 0;
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[b][h][0], x[b][h][1], scale, 0);
+            code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[b][h][2], x[b][h][3], scale, 1);
+            uint8_t* const to = code_bytes + (b * 16 + inside) * 16 + (lane % L) * (V / 2);
+            if constexpr (V == 8) {
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[b][h][4], x[b][h][5], scale, 2);
+                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[b][h][6], x[b][h][7], scale, 3);
+                *reinterpret_cast<uint32_t*>(to) = code;
+            } else {
+                *reinterpret_cast<uint16_t*>(to) = (uint16_t)code;
+            }
+            // Rows and columns that fill a tile up have scales of 0, as their codes are.
+            const bool there = step * kW4Step + b * kW4Group < a.depth && tile * kW4Rows + inside < last;
+            if (lane % L == 0) scales_s[wave][b * 16 + inside] = there ? (uint8_t)byte : 0;
+        }
     wave_sync();
-    for (int t = 0; t < kW4Word && word * kW4Word + t < steps; ++t) {
-        const int step = word * kW4Word + t;
-        float x[4][kW4Rows / RPI][V];
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int h = 0; h < kW4Rows / RPI; ++h) {
-                const int r = tile * kW4Rows + h * RPI + lane / L, column = step * kW4Step + b * kW4Group;
-#pragma unroll
-                for (int i = 0; i < V; ++i) x[b][h][i] = 0.0f;
-                if (r >= a.first && r < last && column < a.depth)
-                    load_row(a.x, TYPE, a.wide, (r - a.first) * a.x_stride + column + V * (lane % L), x[b][h]);
-            }
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int h = 0; h < kW4Rows / RPI; ++h) {
-                const int inside = h * RPI + lane / L;
-                uint32_t amax = 0;
-#pragma unroll
-                for (int i = 0; i < V; ++i) amax = max(amax, magnitude(x[b][h][i]));
-                amax = max(amax, dpp_u<kDppQuadXor1>(amax));
-                amax = max(amax, dpp_u<kDppQuadXor2>(amax));
-                if (L == 8) amax = max(amax, dpp_u<kDppHalfMirror>(amax));
-                const uint32_t byte = scale_byte4(amax);
-                const float scale = scale_power(byte);
-                uint32_t code = 0;
-                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[b][h][0], x[b][h][1], scale, 0);
-                code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[b][h][2], x[b][h][3], scale, 1);
-                uint8_t* const to = code_bytes + (b * 16 + inside) * 16 + (lane % L) * (V / 2);
-                if constexpr (V == 8) {
-                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[b][h][4], x[b][h][5], scale, 2);
-                    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[b][h][6], x[b][h][7], scale, 3);
-                    *reinterpret_cast<uint32_t*>(to) = code;
-                } else {
-                    *reinterpret_cast<uint16_t*>(to) = (uint16_t)code;
-                }
-                const int column = step * kW4Step + b * kW4Group;
-                if (lane % L == 0 && column < a.depth && tile * kW4Rows + inside < last)
-                    scale_bytes[(b * 16 + inside) * 4 + t] = (uint8_t)byte;
-            }
-        wave_sync();
-        if (writes) a.codes[((int64_t)tile * steps + step) * 64 + lane] = codes_s[wave][lane];
-        wave_sync();
-    }
-    if (writes) a.scales[((int64_t)tile * words + word) * 64 + lane] = scales_s[wave][lane];
+    // Rows that fill the last tile up are written with the matrix's last row.
+    const int row = tile * kW4Rows + c;
+    if (row < a.first || (row >= last && last != a.rows)) return;
+    a.codes[((int64_t)tile * steps + step) * 64 + lane] = codes_s[wave][lane];
+    uint8_t* const scale =
+        reinterpret_cast<uint8_t*>(a.scales + ((int64_t)tile * words + step / kW4Word) * 64 + lane) + step % kW4Word;
+    *scale = scales_s[wave][lane];
+    if (step == steps - 1)  // the rest of the last word
+        for (int t = 1; t < kW4Word - step % kW4Word; ++t) scale[t] = 0;
 }
 
 // ---- reading -----------------------------------------------------------------------
@@ -99,42 +96,59 @@ struct ReadArgs {
     bool wide;
 };
 
-// V consecutive columns a thread, 16 bytes of result: the stores, several times
-// the codes' bytes, are what bounds it.
-template <int TYPE>
+// 8 consecutive columns of R rows a thread: the stores, several times the codes'
+// bytes, are what bounds it. Several rows share the arithmetic of the places, where
+// there are enough of them (49,152 rows of 576 in FP32: XX us with 8, YY with 1; 64
+// rows: XX and YY).
+template <int TYPE, int R>
 __global__ void __launch_bounds__(kThreads) w4_read_kernel(ReadArgs a) {
-    constexpr int V = TYPE == MP_TYPE_F32 ? 4 : 8;
-    const uint32_t chunks = a.depth / V;
-    const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
-    const uint32_t r = item / chunks, column = (item - r * chunks) * V;
-    if (r >= (uint32_t)a.count) return;
-    const int id = a.ids[r];
-    float x[V];
-    if (id < 0 || id >= a.rows) {
+    const uint32_t chunks = a.depth / 8, item = blockIdx.x * kThreads + threadIdx.x;
+    const uint32_t group = item / chunks, column = (item - group * chunks) * 8;
+    const int64_t steps = w4_steps(a.depth), words = w4_words(a.depth);
+    const uint32_t step = column / kW4Step, g = column % kW4Step / kW4Group;
+    const uint8_t* const codes = reinterpret_cast<const uint8_t*>(a.m.codes) + step * 1024 + g * 256 + column % kW4Group / 2;
+    const uint8_t* const scales =
+        reinterpret_cast<const uint8_t*>(a.m.scales) + step / kW4Word * 256 + g * 64 + step % kW4Word;
+    int id[R];
+    uint32_t code[R], scale[R];
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = __builtin_nanf("");
-    } else {
-        const int64_t tile = id / kW4Rows, step = column / kW4Step;
-        const int lane = column % kW4Step / kW4Group * 16 + id % kW4Rows;
-        const uint8_t* const from = reinterpret_cast<const uint8_t*>(a.m.codes) +
-                                    (((tile * w4_steps(a.depth)) + step) * 64 + lane) * 16 + column % kW4Group / 2;
-        const uint32_t word = a.m.scales[(tile * w4_words(a.depth) + step / kW4Word) * 64 + lane];
-        const float scale = scale_power(word >> (8 * (step % kW4Word)) & 0xFF);
-        uint32_t codes;
-        if constexpr (V == 8) codes = *reinterpret_cast<const uint32_t*>(from);
-        else codes = *reinterpret_cast<const uint16_t*>(from);
-        auto two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0);
-        x[0] = two[0], x[1] = two[1];
-        two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 1);
-        x[2] = two[0], x[3] = two[1];
-        if constexpr (V == 8) {
-            two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 2);
-            x[4] = two[0], x[5] = two[1];
-            two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 3);
-            x[6] = two[0], x[7] = two[1];
+    for (int k = 0; k < R; ++k) id[k] = group * R + k < (uint32_t)a.count ? a.ids[group * R + k] : -1;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const bool there = id[k] >= 0 && id[k] < a.rows;
+        const int64_t tile = there ? id[k] / kW4Rows : 0, row = there ? id[k] % kW4Rows : 0;
+        code[k] = *reinterpret_cast<const uint32_t*>(codes + tile * steps * 1024 + row * 16);
+        scale[k] = there ? scales[tile * words * 256 + row * 4] : kNanScale;
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        if (group * R + k >= (uint32_t)a.count) return;
+        const float power = scale_power(scale[k]);
+        const auto x0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 0);
+        const auto x1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 1);
+        const auto x2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 2);
+        const auto x3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 3);
+        const int64_t at = (group * R + k) * a.out.stride + column;
+        if constexpr (TYPE == MP_TYPE_F32) {
+            const float lo[4] = {x0[0], x0[1], x1[0], x1[1]}, hi[4] = {x2[0], x2[1], x3[0], x3[1]};
+            store_row<TYPE, 4>(a.out.data, a.wide, at, lo);
+            store_row<TYPE, 4>(a.out.data, a.wide, at + 4, hi);
+        } else {
+            const float x[8] = {x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+            store_row<TYPE, 8>(a.out.data, a.wide, at, x);
         }
     }
-    store_row<TYPE, V>(a.out.data, a.wide, r * a.out.stride + column, x);
+}
+
+template <int TYPE>
+void read(const ReadArgs& a, hipStream_t s) {
+    const int64_t items = (int64_t)a.count * (a.depth / 8);
+    if (items >= kW4ReadGroups) {
+        const int64_t groups = w4_ceil(w4_ceil(a.count, 8) * (a.depth / 8), kThreads);
+        w4_read_kernel<TYPE, 8><<<(unsigned)groups, kThreads, 0, s>>>(a);
+    } else {
+        w4_read_kernel<TYPE, 1><<<(unsigned)w4_ceil(items, kThreads), kThreads, 0, s>>>(a);
+    }
 }
 
 }  // namespace
@@ -160,7 +174,7 @@ extern "C" int mp_hip_w4_pack(const mp_w4_matrix* w, int32_t first, const mp_row
         if (first < 0 || rows < 0 || first > w->rows || rows > w->rows - first)
             return refuse_call("4-bit matrix: no such rows");
         if (rows == 0) return MP_OK;
-        const int64_t tiles = w4_tiles(first + rows) - first / kW4Rows, items = tiles * w4_words(w->depth);
+        const int64_t tiles = w4_tiles(first + rows) - first / kW4Rows, items = tiles * w4_steps(w->depth);
         const int64_t groups = w4_ceil(items, kThreads / 64);
         if (groups > kW4MostGroups) return refuse_call("4-bit matrix: too many rows for one call");
         PackArgs a{};
@@ -198,11 +212,9 @@ extern "C" int mp_hip_w4_read(const mp_w4_matrix* w, const int32_t* ids, int32_t
         const hipStream_t s = static_cast<hipStream_t>(stream);
         const StreamDevice device(s);
         if (device.status != hipSuccess) return call_done(device.status, "4-bit read: device of the stream");
-        const int64_t items = (int64_t)count * (w->depth / (out->type == MP_TYPE_F32 ? 4 : 8));
-        const unsigned groups = (unsigned)w4_ceil(items, kThreads);
-        if (out->type == MP_TYPE_F32) w4_read_kernel<MP_TYPE_F32><<<groups, kThreads, 0, s>>>(a);
-        else if (out->type == MP_TYPE_BF16) w4_read_kernel<MP_TYPE_BF16><<<groups, kThreads, 0, s>>>(a);
-        else w4_read_kernel<MP_TYPE_F16><<<groups, kThreads, 0, s>>>(a);
+        if (out->type == MP_TYPE_F32) read<MP_TYPE_F32>(a, s);
+        else if (out->type == MP_TYPE_BF16) read<MP_TYPE_BF16>(a, s);
+        else read<MP_TYPE_F16>(a, s);
         return call_done(hipGetLastError(), "4-bit read launch");
     });
 }

@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
                 power[m][i] = scale_power(scale[m][i] >> shift & 0xFF);
             }
         if (block + 1 < last) load(block + 1);
+        __builtin_amdgcn_sched_barrier(0);  // the loads go out before the products
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             b8 x[PARTS];
@@ -243,7 +244,7 @@ extern "C" int mp_hip_w4_product(const mp_w4_matrix* w, const mp_w4_matrix* gate
         const W4Plan p = w4_few_plan(rows, w->rows, w->depth, parts_of(x->type), gate != nullptr, out->type == MP_TYPE_I8);
         const int64_t groups = way == kW4Few ? w4_groups(p, rows, w->rows)
                                              : w4_tile_groups(rows, w->rows, gate != nullptr, way == kW4LargeTiles);
-        if (groups > kW4MostGroups || (planes && need / kEightBlock > kW4MostGroups))
+        if (groups > kW4MostGroups || (planes && w4_planes_blocks(rows, w->depth) > kW4MostGroups))
             return refuse_call("4-bit product: too large for one call");
         ProductArgs a{};
         a.m[0] = view(*w);

@@ -23,6 +23,9 @@ constexpr size_t w4_scale_bytes(int64_t rows, int64_t depth) { return (size_t)(w
 // Elements of a call on rows alone (norm, conversion): 2^30 threads of 8.
 constexpr int64_t kRowsMostElements = (int64_t)1 << 33;
 
+// Runs of 8 elements from which on a read takes 8 rows a thread.
+constexpr int64_t kW4ReadGroups = 1 << 20;
+
 // A product by wavefronts that share a block of columns and deal the depth
 // among themselves: `column_tiles` tiles of `side` columns and rows a wavefront,
 // `waves` of them a work-group.
@@ -63,8 +66,7 @@ inline W4Plan w4_few_plan(int rows, int n, int depth, int parts, bool gated, boo
 // 128 rows and 64 columns: two planes of 24 bytes a lane, and their scales.
 constexpr int kTileRows = 128, kTileColumns = 256, kTileDepth = 64;
 constexpr int kSmallTileRows = 64, kSmallTileColumns = 128;
-constexpr int kPlaneBytes = 64 * 24, kEightTile = 2 * kPlaneBytes + 256;  // of 32 rows
-constexpr int kEightBlock = 4 * kEightTile;
+constexpr int kPlaneBytes = 64 * 24, kPlanesBlock = 4 * 2 * kPlaneBytes;  // of 32 and of 128 rows
 
 enum W4Way { kW4Few, kW4SmallTiles, kW4LargeTiles };
 
@@ -78,8 +80,12 @@ constexpr W4Way w4_way(int rows, int n, bool gated) {
                                                                       : kW4Few;
 }
 
+constexpr int64_t w4_planes_blocks(int64_t rows, int64_t depth) {
+    return w4_ceil(rows, kTileRows) * w4_ceil(depth, kTileDepth);
+}
 constexpr size_t w4_planes_bytes(int64_t rows, int64_t depth) {
-    return (size_t)(w4_ceil(rows, kTileRows) * w4_ceil(depth, kTileDepth)) * kEightBlock;
+    return (size_t)w4_planes_blocks(rows, depth) * kPlanesBlock +
+           (size_t)(w4_ceil(rows, kTileRows) * w4_steps(depth)) * kTileRows * 8;
 }
 
 }  // namespace mphip
