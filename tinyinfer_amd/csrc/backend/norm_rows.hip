@@ -151,6 +151,7 @@ struct NormArgs {
     const float* weight;
     float epsilon;
     int rows, width;
+    double share;  // 1 / width
 };
 
 // The sum over a wavefront's lanes, in every lane.
@@ -195,6 +196,17 @@ __device__ __forceinline__ float to_type(double y) {
     return TYPE == MP_TYPE_F32 ? (float)y : to_odd(y);
 }
 
+// 1 / sqrt(v) to the last bit or two: an estimate of half the bits and two steps of
+// Newton's method, a fourth of the instructions of a root and a division. Infinity
+// gives 0.
+__device__ __forceinline__ double inverse_root(double v) {
+    const double estimate = __builtin_amdgcn_rsq(v);
+    double y = estimate;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = __builtin_fma(0.5 * y, __builtin_fma(-v * y, y, 1.0), y);
+    return v == __builtin_inf() ? estimate : y;
+}
+
 // A row by `waves` wavefronts (a work-group, or one of a work-group's
 // wavefronts), C chunks of 8 elements a lane in registers between the sum of
 // squares and the result; longer rows are read a second time.
@@ -216,6 +228,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(NormArgs a, int waves) {
     const int step = WIDE ? 1 : lanes;
     auto place = [&](int base, int c) { return base + c * lanes * kEach + (WIDE ? me * kEach : me); };
     double t[C][kEach];
+    float w[C][kEach];
     auto load = [&](int base) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -229,9 +242,23 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(NormArgs a, int waves) {
             for (int k = 0; k < kEach; ++k) t[c][k] = RESIDUAL ? (double)x[k] + (double)r[k] : (double)x[k];
         }
     };
+    // On their way while the row's sums meet.
+    auto load_weight = [&](int base) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int i = place(base, c);
+            if constexpr (WIDE) {
+                if (i < a.width) load_row(a.weight, MP_TYPE_F32, true, i, w[c]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) w[c][k] = i + k * step < a.width ? a.weight[i + k * step] : 0.0f;
+            }
+        }
+    };
     double squares = 0.0;
     for (int base = 0; base < a.width; base += block) {
         load(base);
+        if (block >= a.width) load_weight(base);
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -244,21 +271,18 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(NormArgs a, int waves) {
         squares = 0.0;
         for (int w = 0; w < waves; ++w) squares += sums[w];
     }
-    const double inverse = 1.0 / __builtin_sqrt(squares / a.width + (double)a.epsilon);
+    const double inverse = inverse_root(__builtin_fma(squares, a.share, (double)a.epsilon));
     for (int base = 0; base < a.width; base += block) {
-        if (block < a.width) load(base);
+        if (block < a.width) {
+            load(base);
+            load_weight(base);
+        }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int i = place(base, c);
             // A quad or 32 lanes whose group is there stay together.
-            float y[kEach] = {}, w[kEach] = {};
+            float y[kEach] = {};
             if (i < a.width) {
-                if constexpr (WIDE) {
-                    load_row(a.weight, MP_TYPE_F32, true, i, w);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < kEach; ++k) w[k] = i + k * step < a.width ? a.weight[i + k * step] : 0.0f;
-                }
                 if constexpr (RESIDUAL) {
                     if (a.sum.data) {
 #pragma unroll
@@ -267,7 +291,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(NormArgs a, int waves) {
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < kEach; ++k) y[k] = to_type<OUT>(t[c][k] * inverse * (double)w[k]);
+                for (int k = 0; k < kEach; ++k) y[k] = to_type<OUT>(t[c][k] * inverse * (double)w[c][k]);
                 store_each<OUT, WIDE>(a.out, row, i, step, a.width, y);
             }
         }
@@ -355,7 +379,7 @@ extern "C" int mp_hip_rms_norm(const mp_rows* x, const mp_rows* residual, const 
         a.x = rows_view(*x), a.out = rows_view(*out);
         if (residual) a.residual = rows_view(*residual);
         if (sum) a.sum = rows_view(*sum);
-        a.weight = weight, a.epsilon = epsilon, a.rows = rows, a.width = width;
+        a.weight = weight, a.epsilon = epsilon, a.rows = rows, a.width = width, a.share = 1.0 / width;
         const bool wide = width % kEach == 0 && rows_wide(*x) && rows_wide(*out) && (!residual || rows_wide(*residual)) &&
                           (!sum || rows_wide(*sum)) && reinterpret_cast<uintptr_t>(weight) % 16 == 0;
         const hipStream_t s = static_cast<hipStream_t>(stream);

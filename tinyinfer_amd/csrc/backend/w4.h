@@ -66,11 +66,16 @@ __device__ __forceinline__ float scale_inverse(uint32_t byte) { return __uint_as
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-// A number over its group's scale, rounded to nearest, ties to even; what a
-// group whose scale is NaN holds does not matter.
-__device__ __forceinline__ uint32_t to_code8(float x, float inverse) { return (uint32_t)(int)rintf(x * inverse) & 0xFF; }
+// A number over its group's scale in the low byte, rounded to nearest, ties to
+// even: next to 1.5 * 2^23 an FP32 number's last bit is 1. What a group whose scale
+// is NaN holds does not matter.
+__device__ __forceinline__ uint32_t to_code8(float x, float inverse) {
+    return __float_as_uint(__builtin_fmaf(x, inverse, 12582912.0f));
+}
 __device__ __forceinline__ uint32_t to_codes8(float a, float b, float c, float d, float inverse) {
-    return to_code8(a, inverse) | to_code8(b, inverse) << 8 | to_code8(c, inverse) << 16 | to_code8(d, inverse) << 24;
+    const uint32_t lo = __builtin_amdgcn_perm(to_code8(b, inverse), to_code8(a, inverse), 0x0C0C0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(to_code8(d, inverse), to_code8(c, inverse), 0x04000C0Cu);
+    return lo | hi;
 }
 // Four codes times a scale.
 __device__ __forceinline__ f4 from_codes8(uint32_t codes, float scale) {

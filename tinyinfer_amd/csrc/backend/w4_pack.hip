@@ -96,14 +96,14 @@ struct ReadArgs {
     bool wide;
 };
 
-// 8 consecutive columns of R rows a thread: the stores, several times the codes'
-// bytes, are what bounds it. Several rows share the arithmetic of the places, where
-// there are enough of them (49,152 rows of 576 in FP32: XX us with 8, YY with 1; 64
-// rows: XX and YY).
+// V consecutive columns of R rows a thread, 16 bytes of result each: the stores,
+// several times the codes' bytes, are what bounds it. Several rows share the
+// arithmetic of the places, where there are enough of them.
 template <int TYPE, int R>
 __global__ void __launch_bounds__(kThreads) w4_read_kernel(ReadArgs a) {
-    const uint32_t chunks = a.depth / 8, item = blockIdx.x * kThreads + threadIdx.x;
-    const uint32_t group = item / chunks, column = (item - group * chunks) * 8;
+    constexpr int V = TYPE == MP_TYPE_F32 ? 4 : 8;
+    const uint32_t chunks = a.depth / V, item = blockIdx.x * kThreads + threadIdx.x;
+    const uint32_t group = item / chunks, column = (item - group * chunks) * V;
     const int64_t steps = w4_steps(a.depth), words = w4_words(a.depth);
     const uint32_t step = column / kW4Step, g = column % kW4Step / kW4Group;
     const uint8_t* const codes = reinterpret_cast<const uint8_t*>(a.m.codes) + step * 1024 + g * 256 + column % kW4Group / 2;
@@ -117,34 +117,35 @@ __global__ void __launch_bounds__(kThreads) w4_read_kernel(ReadArgs a) {
     for (int k = 0; k < R; ++k) {
         const bool there = id[k] >= 0 && id[k] < a.rows;
         const int64_t tile = there ? id[k] / kW4Rows : 0, row = there ? id[k] % kW4Rows : 0;
-        code[k] = *reinterpret_cast<const uint32_t*>(codes + tile * steps * 1024 + row * 16);
+        const uint8_t* const from = codes + tile * steps * 1024 + row * 16;
+        if constexpr (V == 8) code[k] = *reinterpret_cast<const uint32_t*>(from);
+        else code[k] = *reinterpret_cast<const uint16_t*>(from);
         scale[k] = there ? scales[tile * words * 256 + row * 4] : kNanScale;
     }
 #pragma unroll
     for (int k = 0; k < R; ++k) {
         if (group * R + k >= (uint32_t)a.count) return;
         const float power = scale_power(scale[k]);
-        const auto x0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 0);
-        const auto x1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 1);
-        const auto x2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 2);
-        const auto x3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 3);
-        const int64_t at = (group * R + k) * a.out.stride + column;
-        if constexpr (TYPE == MP_TYPE_F32) {
-            const float lo[4] = {x0[0], x0[1], x1[0], x1[1]}, hi[4] = {x2[0], x2[1], x3[0], x3[1]};
-            store_row<TYPE, 4>(a.out.data, a.wide, at, lo);
-            store_row<TYPE, 4>(a.out.data, a.wide, at + 4, hi);
-        } else {
-            const float x[8] = {x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
-            store_row<TYPE, 8>(a.out.data, a.wide, at, x);
+        float x[V];
+        auto two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 0);
+        x[0] = two[0], x[1] = two[1];
+        two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 1);
+        x[2] = two[0], x[3] = two[1];
+        if constexpr (V == 8) {
+            two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 2);
+            x[4] = two[0], x[5] = two[1];
+            two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[k], power, 3);
+            x[6] = two[0], x[7] = two[1];
         }
+        store_row<TYPE, V>(a.out.data, a.wide, (group * R + k) * a.out.stride + column, x);
     }
 }
 
 template <int TYPE>
 void read(const ReadArgs& a, hipStream_t s) {
-    const int64_t items = (int64_t)a.count * (a.depth / 8);
-    if (items >= kW4ReadGroups) {
-        const int64_t groups = w4_ceil(w4_ceil(a.count, 8) * (a.depth / 8), kThreads);
+    const int64_t runs = a.depth / (TYPE == MP_TYPE_F32 ? 4 : 8), items = a.count * runs;
+    if (items >= kW4ReadRuns) {
+        const int64_t groups = w4_ceil(w4_ceil(a.count, 8) * runs, kThreads);
         w4_read_kernel<TYPE, 8><<<(unsigned)groups, kThreads, 0, s>>>(a);
     } else {
         w4_read_kernel<TYPE, 1><<<(unsigned)w4_ceil(items, kThreads), kThreads, 0, s>>>(a);

@@ -23,8 +23,8 @@ constexpr size_t w4_scale_bytes(int64_t rows, int64_t depth) { return (size_t)(w
 // Elements of a call on rows alone (norm, conversion): 2^30 threads of 8.
 constexpr int64_t kRowsMostElements = (int64_t)1 << 33;
 
-// Runs of 8 elements from which on a read takes 8 rows a thread.
-constexpr int64_t kW4ReadGroups = 1 << 20;
+// Runs of 16 bytes from which on a read takes 8 rows a thread.
+constexpr int64_t kW4ReadRuns = 1 << 20;
 
 // A product by wavefronts that share a block of columns and deal the depth
 // among themselves: `column_tiles` tiles of `side` columns and rows a wavefront,
