@@ -11,7 +11,7 @@ struct ProductArgs {
     W4View m[2];  // the matrix, the gate
     int n, depth, rows;
     RowsView x, out;
-    bool x_wide, out_wide;
+    bool out_wide;
     int column_blocks, row_blocks;
 };
 
@@ -77,37 +77,38 @@ __device__ __forceinline__ void store_result8(const ProductArgs& a, int64_t row,
 }
 
 // 8 columns of a row, as they lie and as the BF16 numbers whose sums they are.
+// Loads are of 16 bytes wherever a row begins: the memory takes any alignment of
+// the elements, and aligned rows are as fast.
 template <int KIND>
 struct Run8 {
     static constexpr int BYTES = 8 * (KIND == MP_TYPE_I8 ? 1 : KIND == MP_TYPE_F32 ? 4 : 2), WORDS = BYTES / 4;
     uint32_t raw[WORDS];
     float scale;
-    // Zeros where there is no such row or column.
-    __device__ __forceinline__ void load(const ProductArgs& a, int64_t row, int column) {
-        if (row >= a.rows || column >= a.depth) {
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) raw[i] = 0;
-            scale = 0.0f;
-            return;
+    // A row behind the end is the last again.
+    struct Row {
+        const uint8_t* data;
+        const uint8_t* scales;
+        __device__ __forceinline__ void begin(const ProductArgs& a, int64_t row) {
+            row = min(row, (int64_t)a.rows - 1);
+            data = static_cast<const uint8_t*>(a.x.data) + row * a.x.stride * (BYTES / 8);
+            if constexpr (KIND == MP_TYPE_I8) scales = a.x.scales + row * a.x.scale_stride;
         }
-        const uint8_t* const from = static_cast<const uint8_t*>(a.x.data) + (row * a.x.stride + column) * (BYTES / 8);
+    };
+    // `column` is one of the row's: where a block's columns end behind the depth, the
+    // row's last ones stand in for them, times weights that are zeros.
+    __device__ __forceinline__ void load(const Row& row, uint32_t column) {
+        typedef uint32_t w4 __attribute__((ext_vector_type(4), aligned(2)));
+        const uint8_t* const from = row.data + column * (BYTES / 8);
         if constexpr (KIND == MP_TYPE_I8) {
             const uint2 v = *reinterpret_cast<const uint2*>(from);
             raw[0] = v.x, raw[1] = v.y;
-            scale = scale_number(a.x.scales[row * a.x.scale_stride + column / kW4Group]);
-        } else if (a.x_wide) {
+            scale = scale_number(row.scales[column / kW4Group]);
+        } else {
 #pragma unroll
             for (int i = 0; i < WORDS; i += 4) {
-                const u4 v = reinterpret_cast<const u4*>(from)[i / 4];
+                const w4 v = reinterpret_cast<const w4*>(from)[i / 4];
                 raw[i] = v[0], raw[i + 1] = v[1], raw[i + 2] = v[2], raw[i + 3] = v[3];
             }
-        } else if constexpr (KIND == MP_TYPE_F32) {
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) raw[i] = reinterpret_cast<const uint32_t*>(from)[i];
-        } else {
-            const uint16_t* const halves = reinterpret_cast<const uint16_t*>(from);
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) raw[i] = halves[2 * i] | (uint32_t)halves[2 * i + 1] << 16;
         }
     }
     __device__ __forceinline__ void split(u4 (&part)[parts_of(KIND)]) const {

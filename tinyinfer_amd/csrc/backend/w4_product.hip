@@ -73,6 +73,9 @@ __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
     u4 codes[M][NT];
     uint32_t scale[M][NT];
     Run8<KIND> run[EACH];
+    typename Run8<KIND>::Row row_at[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) row_at[i].begin(a, (int64_t)row_block * SIDE + i * ROWS_EACH + row_of);
     auto load = [&](int block) {
         const int step = block / HALVES, half = block % HALVES;
 #pragma unroll
@@ -85,7 +88,7 @@ __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
             if (i * ROWS_EACH < rows)
-                run[i].load(a, (int64_t)row_block * SIDE + i * ROWS_EACH + row_of, block * T::DEPTH + 8 * run_of);
+                run[i].load(row_at[i], min(block * T::DEPTH + 8 * run_of, a.depth - 8));
     };
     if (first < last) load(first);
     for (int block = first; block < last; ++block) {
@@ -251,7 +254,7 @@ extern "C" int mp_hip_w4_product(const mp_w4_matrix* w, const mp_w4_matrix* gate
         if (gate) a.m[1] = view(*gate);
         a.n = w->rows, a.depth = w->depth, a.rows = rows;
         a.x = rows_view(*x), a.out = rows_view(*out);
-        a.x_wide = rows_wide(*x), a.out_wide = rows_wide(*out);
+        a.out_wide = rows_wide(*out);
         a.column_blocks = (int)w4_ceil(a.n, p.side * p.column_tiles);
         a.row_blocks = (int)w4_ceil(rows, p.side);
         const hipStream_t s = static_cast<hipStream_t>(stream);

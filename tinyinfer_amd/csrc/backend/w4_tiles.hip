@@ -25,34 +25,47 @@ __device__ __forceinline__ void find_block(const ProductArgs& a, int* row_block,
 
 // A wavefront's N tiles of 32 columns from `first` on: of the matrix, or half of
 // them of it and the same of the gate. Codes come from memory to the registers as
-// they lie, lane (c, h) with row c at columns 32h ..+31 of a block of 64.
+// they lie, lane (c, h) with row c at columns 32h ..+31 of a block of 64. Places are
+// a uniform address and 32 bits of a lane's own.
 template <int N, bool GATED>
 struct Weights {
-    static constexpr int EACH = GATED ? N / 2 : N;
-    const u4* codes_at[N];
-    const uint32_t* scales_at[N];
-    u4 codes[N];
-    uint32_t scale[N];
+    static constexpr int EACH = GATED ? N / 2 : N, M = GATED ? 2 : 1;
+    struct Block {
+        u4 codes[N];
+        uint32_t scale[N];
+    };
+    const uint8_t* codes_at[M];
+    const uint8_t* scales_at[M];
+    uint32_t code_place[EACH], scale_place[EACH];
     __device__ __forceinline__ void begin(const ProductArgs& a, int first) {
-        const int lane = threadIdx.x & 63, tiles = (int)w4_tiles(a.n);
+        const int lane = threadIdx.x & 63, last = (int)w4_tiles(a.n) - 1, tile0 = min(first / kW4Rows, last);
+        const int steps = (int)w4_steps(a.depth), words = (int)w4_words(a.depth);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int m = 0; m < M; ++m) {
+            codes_at[m] = reinterpret_cast<const uint8_t*>(a.m[m].codes) + (int64_t)tile0 * steps * 1024;
+            scales_at[m] = reinterpret_cast<const uint8_t*>(a.m[m].scales) + (int64_t)tile0 * words * 256;
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
             // Columns behind the end are those at the end again, and not stored.
-            const int64_t tile = min((first + i % EACH * 32) / kW4Rows + lane % 32 / 16, tiles - 1);
-            const W4View& m = a.m[i / EACH];
-            codes_at[i] = m.codes + tile * w4_steps(a.depth) * 64 + lane / 32 * 16 + lane % 16;
-            scales_at[i] = m.scales + tile * w4_words(a.depth) * 64 + lane / 32 * 16 + lane % 16;
+            const uint32_t tile = min((first + i * 32) / kW4Rows + lane % 32 / 16, last) - tile0;
+            code_place[i] = tile * steps * 1024 + (lane / 32 * 16 + lane % 16) * 16;
+            scale_place[i] = tile * words * 256 + (lane / 32 * 16 + lane % 16) * 4;
         }
     }
-    __device__ __forceinline__ void load(int block) {
+    __device__ __forceinline__ void load(int block, Block* to) const {
+        const int step = block >> 1, half = block & 1;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            codes[i] = codes_at[i][block / 2 * 64 + block % 2 * 32];
-            scale[i] = scales_at[i][block / 2 / kW4Word * 64 + block % 2 * 32];
+        for (int m = 0; m < M; ++m) {
+            const uint8_t* const codes = codes_at[m] + step * 1024 + half * 512;
+            const uint8_t* const scales = scales_at[m] + (step >> 2) * 256 + half * 128 + (step & 3);
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                to->codes[m * EACH + i] = *reinterpret_cast<const u4*>(codes + code_place[i]);
+                to->scale[m * EACH + i] = scales[scale_place[i]];
+            }
         }
     }
-    // The scale's byte for a block, in the lowest place.
-    static __device__ __forceinline__ uint32_t byte_of(uint32_t scale, int block) { return scale >> (8 * (block / 2 % kW4Word)); }
 };
 
 // Results of 32 rows by 32 columns: lane (r, h) has row r at columns 8q + 4h ..+3.
@@ -98,7 +111,7 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a
     constexpr int EACH = ROWS * 8 / THREADS;  // runs of 8 columns a thread
     constexpr int SIZE = PARTS * TILES * 256, BUFFERS = 2 * SIZE * 16 <= 65536 ? 2 : 1;
     __shared__ u4 rows_s[BUFFERS][SIZE];  // [part][tile][run of 8 columns][row]
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane / 32;
     const int wave_columns = wave / WR, wave_rows = wave % WR;
     int row_block, column_block;
     find_block(a, &row_block, &column_block);
@@ -110,14 +123,18 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a
     const int blocks = (int)w4_ceil(a.depth, kTileDepth);
     f16v sum[N][RT] = {};
 
-    Run8<KIND> run[EACH];
     // Run i of a thread: columns 8e ..+7 of the block of a row, so that neighbours
     // read a line of memory. In LDS row r of run e lies at r ^ e: neither rows nor
     // runs share banks.
     const int e = threadIdx.x % 8, r0 = threadIdx.x / 8;
-    auto load_rows = [&](int block) {
+    Run8<KIND> run[EACH];
+    typename Run8<KIND>::Row row[EACH];
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) run[i].load(a, first_row + r0 + i * (THREADS / 8), block * kTileDepth + 8 * e);
+    for (int i = 0; i < EACH; ++i) row[i].begin(a, first_row + r0 + i * (THREADS / 8));
+    auto load_rows = [&](int block) {
+        const uint32_t column = min(block * kTileDepth + 8 * e, a.depth - 8);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) run[i].load(row[i], column);
     };
     auto keep_rows = [&](int buffer) {
 #pragma unroll
@@ -130,29 +147,25 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a
                 rows_s[buffer][((p * TILES + r / 32) * 8 + e) * 32 + (r % 32 ^ e)] = part[p];
         }
     };
-    load_rows(0);
-    w.load(0);
-    keep_rows(0);
-    __syncthreads();
-    for (int block = 0; block < blocks; ++block) {
-        const int buffer = BUFFERS == 2 ? block & 1 : 0;
-        const bool more = block + 1 < blocks;
-        u4 codes[N];
-        float power[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            codes[i] = w.codes[i];
-            power[i] = scale_power(w.byte_of(w.scale[i], block) & 0xFF);
+    // A block from the buffer and the registers that have it, while the next one's
+    // rows go from the registers to the other buffer and those behind it come from
+    // memory: what is waited for was asked for a block's products before. With one
+    // buffer the next rows are asked for here and kept behind the products.
+    typename Weights<N, GATED>::Block even, odd;
+    auto step = [&](int block, int buffer, const auto& now, auto* next) {
+        const int behind = min(block + 1, blocks - 1);  // the last again, behind it
+        if constexpr (BUFFERS == 2) {
+            keep_rows(buffer ^ 1);
+            load_rows(min(block + 2, blocks - 1));
+        } else {
+            load_rows(behind);
         }
-        if (more) {
-            load_rows(block + 1);
-            w.load(block + 1);
-        }
+        w.load(behind, next);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             b8 c[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) c[i] = weights8(codes[i][d], power[i]);
+            for (int i = 0; i < N; ++i) c[i] = weights8(now.codes[i][d], scale_power(now.scale[i]));
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
@@ -164,9 +177,21 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a
                         sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[i], x, sum[i][j], 0, 0, 0);
                 }
         }
-        if (BUFFERS == 1) __syncthreads();
-        if (more) keep_rows(BUFFERS == 2 ? buffer ^ 1 : 0);
+        if constexpr (BUFFERS == 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            keep_rows(0);
+        }
         __syncthreads();
+    };
+    load_rows(0);
+    w.load(0, &even);
+    keep_rows(0);
+    if (BUFFERS == 2) load_rows(min(1, blocks - 1));
+    __syncthreads();
+    for (int block = 0; block < blocks; block += 2) {
+        step(block, 0, even, &odd);
+        if (block + 1 < blocks) step(block + 1, BUFFERS - 1, odd, &even);
     }
     store_tiles<N, RT, GATED>(a, first_row + wave_rows * RT * 32, first_column, sum);
 }
