@@ -170,14 +170,14 @@ def test_pack_in_pieces_leaves_other_rows(torch_cuda):
 
 def test_groups_with_nan_or_infinity_are_nan(torch_cuda):
     x = np.random.default_rng(4).standard_normal((4, 128))
-    x[0, 5], x[1, 40], x[2, 127] = np.nan, np.inf, -np.inf
+    x[0, 5], x[1, 40], x[2, 127], x[3, 70] = np.nan, np.inf, -np.inf, 3.3e38  # the last: past 6 and 127 times 2^120
     m = Matrix(torch_cuda, 4, 128)
     mp.w4_pack(m.view, 0, Floats(torch_cuda, x, F32).rows, 4)
     ids = torch_cuda.arange(4, dtype=torch_cuda.int32, device="cuda")
     out = Floats(torch_cuda, np.zeros((4, 128)), F32)
     mp.w4_read(m.view, ids.data_ptr(), 4, out.rows)
     want = np.zeros((4, 4), bool)
-    want[0, 0] = want[1, 1] = want[2, 3] = True
+    want[0, 0] = want[1, 1] = want[2, 3] = want[3, 2] = True
     assert np.array_equal(np.isnan(out.back()), want.repeat(32, 1))
     eight = Eight(torch_cuda, 4, 128)
     mp.convert_rows(Floats(torch_cuda, x, F32).rows, 4, 128, eight.rows)
@@ -374,7 +374,7 @@ def test_products_to_every_type(torch_cuda, kind, to, rows, n, k, pad):
 @pytest.mark.parametrize("pad, shift", [(1, 0), (0, 1), (5, 3), (2, 2)])
 def test_products_of_any_alignment(torch_cuda, kind, pad, shift):
     rng = np.random.default_rng(pad + 10 * shift)
-    for rows, n, k in ((1, 37, 96), (20, 51, 160), (70, 35, 64), (130, 16291, 96)):
+    for rows, n, k in ((1, 37, 96), (20, 51, 160), (70, 35, 64), (130, 16291, 96), (300, 22001, 64)):
         x = ref.rounded(rng.standard_normal((rows, k)), kind)
         w = ref.held(rng.standard_normal((n, k)), E2M1)
         matrix, source = Matrix(torch_cuda, n, k, w), Floats(torch_cuda, x, kind, pad, shift)
@@ -387,10 +387,10 @@ def test_products_of_any_alignment(torch_cuda, kind, pad, shift):
 
 
 @ANY
-@pytest.mark.parametrize("rows", [3, 40, 300, 2000])
-def test_nan_stays_in_its_row_and_column(torch_cuda, kind, rows):
+@pytest.mark.parametrize("rows, n", [(3, 50), (40, 50), (300, 50), (66, 16400), (2000, 4200)])
+def test_nan_stays_in_its_row_and_column(torch_cuda, kind, rows, n):
     rng = np.random.default_rng(rows)
-    n, k = 50, 288
+    k = 288
     x = in_type(rng.standard_normal((rows, k)), kind)
     w = ref.held(rng.standard_normal((n, k)), E2M1)
     want = x @ w.T
@@ -436,12 +436,13 @@ def test_far_smaller_elements_count(torch_cuda, kind):
         close(out.back(), x @ w.T, ref.product_bound(x, w, PARTS[kind]), F32)
 
 
-def test_calls_on_a_stream_and_replayed(torch_cuda):
+@pytest.mark.parametrize("rows, n", [(1, 480), (70, 480), (70, 16384), (2049, 2080)])
+def test_calls_on_a_stream_and_replayed(torch_cuda, rows, n):
     """Norm, conversion and products captured on a stream of their own and replayed for other rows, with eager work
     between; every replay against eager calls."""
     torch = torch_cuda
     rng = np.random.default_rng(8)
-    rows, k, n = 70, 576, 480
+    k = 576
     matrix = Matrix(torch, n, k, ref.held(rng.standard_normal((n, k)), E2M1))
     gate = Matrix(torch, n, k, ref.held(rng.standard_normal((n, k)), E2M1))
     weight = torch.ones(k, device="cuda")
@@ -551,14 +552,114 @@ def test_a_decode_step_of_a_layer(torch_cuda):
 
 @ANY
 @pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
-@pytest.mark.parametrize("rows, n, k", [(129, 16500, 96), (640, 5000, 32), (1000, 4120, 192), (2049, 2000, 544), (130, 17000, 576)])
+@pytest.mark.parametrize("rows, n, k", [(129, 16500, 96), (640, 5000, 32), (1000, 4120, 192), (2049, 2000, 544), (130, 17000, 576),
+                                        (2049, 4100, 160), (300, 21900, 64)])
 def test_products_of_many_rows(torch_cuda, kind, gated, rows, n, k):
     check_product(torch_cuda, np.random.default_rng(rows + n + k), rows, n, k, kind, F32, gated)
 
 
 @ANY
 @pytest.mark.parametrize("to", [F32, BF16, F16, I8], ids=["f32", "bf16", "f16", "i8"])
-@pytest.mark.parametrize("rows, n, k, pad", [(1025, 4128, 160, 16), (4097, 1056, 64, 0)])
+@pytest.mark.parametrize("rows, n, k, pad", [(1025, 4128, 160, 16), (4097, 1056, 64, 0), (2050, 4128, 96, 0)])
 def test_products_of_many_rows_to_every_type(torch_cuda, kind, to, rows, n, k, pad):
     for gated in (False, True):
         check_product(torch_cuda, np.random.default_rng(n + k), rows, n, k, kind, to, gated, pad)
+
+
+def test_two_streams_at_once(torch_cuda):
+    """Products of prompts on two streams, each with a workspace of its own, as one after the other."""
+    torch = torch_cuda
+    rng = np.random.default_rng(13)
+    rows, n, k = 2049, 4160, 256
+    matrix = Matrix(torch, n, k, ref.held(rng.standard_normal((n, k)), E2M1))
+    x = [Eight(torch, rows, k, ref.held(rng.standard_normal((rows, k)), WHOLE)) for _ in range(2)]
+    size = mp.w4_product_workspace(matrix.view, I8, rows)
+    assert size > 0
+    want = []
+    for source in x:
+        out, space = Floats(torch, np.zeros((rows, n)), BF16), torch.empty(size, dtype=torch.uint8, device="cuda")
+        mp.w4_product(matrix.view, source.rows, rows, out.rows, workspace=space.data_ptr(), workspace_bytes=size)
+        want.append(out.back())
+    streams = [torch.cuda.Stream() for _ in x]
+    outs = [Floats(torch, np.zeros((rows, n)), BF16) for _ in x]
+    spaces = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in x]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for source, out, space, stream in zip(x, outs, spaces, streams):
+            mp.w4_product(matrix.view, source.rows, rows, out.rows, workspace=space.data_ptr(), workspace_bytes=size,
+                          stream=stream.cuda_stream)
+    for out, there in zip(outs, want):
+        assert np.array_equal(out.back(), there)
+
+
+def test_a_workspace_for_more_rows_is_enough(torch_cuda):
+    rng = np.random.default_rng(14)
+    n, k = 4160, 96
+    w = ref.held(rng.standard_normal((n, k)), E2M1)
+    matrix = Matrix(torch_cuda, n, k, w)
+    size = mp.w4_product_workspace(matrix.view, I8, 2304)
+    space = torch_cuda.empty(size, dtype=torch_cuda.uint8, device="cuda")
+    for rows in (2304, 2200, 1950, 700, 3):
+        assert mp.w4_product_workspace(matrix.view, I8, rows) <= size
+        x = ref.held(rng.standard_normal((rows, k)), WHOLE)
+        out = Floats(torch_cuda, np.zeros((rows, n)), F32)
+        mp.w4_product(matrix.view, Eight(torch_cuda, rows, k, x).rows, rows, out.rows, workspace=space.data_ptr(),
+                      workspace_bytes=size)
+        close(out.back(), x @ w.T, ref.product_bound(x, w, 1), F32)
+    x = Eight(torch_cuda, 2304, k, ref.held(rng.standard_normal((2304, k)), WHOLE))
+    out = Floats(torch_cuda, np.zeros((2304, n)), F32)
+    for bad in (dict(), dict(workspace=space.data_ptr(), workspace_bytes=size - 1),
+                dict(workspace=space.data_ptr() + 8, workspace_bytes=size)):
+        with pytest.raises(mp.BackendError, match="workspace"):
+            mp.w4_product(matrix.view, x.rows, 2304, out.rows, **bad)
+
+
+@pytest.mark.parametrize("rows, n", [(20, 96), (70, 16384)])
+def test_rows_past_4_gib(torch_cuda, rows, n):
+    """Rows 2^26 elements apart: norm, conversion and products find the last ones."""
+    torch = torch_cuda
+    rng = np.random.default_rng(rows)
+    k, stride = 96, 1 << 26
+    x = ref.rounded(rng.standard_normal((rows, k)), F32)
+    w = ref.held(rng.standard_normal((n, k)), E2M1)
+    buffer = torch.empty(rows * stride, device="cuda")
+    far = buffer.view(rows, stride)[:, :k]
+    far.copy_(torch.from_numpy(x.astype(np.float32)).cuda())
+    source = mp.Rows(buffer.data_ptr(), stride, None, 0, F32)
+    matrix, out = Matrix(torch, n, k, w), Floats(torch, np.zeros((rows, n)), F32)
+    mp.w4_product(matrix.view, source, rows, out.rows)
+    close(out.back(), x @ w.T, ref.product_bound(x, w, 3), F32)
+    weight = torch.ones(k, device="cuda")
+    near = Floats(torch, x, F32)
+    mp.rms_norm(source, weight.data_ptr(), 1e-5, rows, k, near.rows)
+    assert np.array_equal(near.back(), ref.rounded(ref.norm(x, None, np.ones(k, np.float32), 1e-5)[1], F32))
+    mp.convert_rows(near.rows, rows, k, source)
+    torch.cuda.synchronize()
+    assert np.array_equal(far.double().cpu().numpy(), near.back())
+
+
+def test_a_matrix_past_4_gib(torch_cuda):
+    """Packing, reading and multiplying with the last rows of 2^24."""
+    torch = torch_cuda
+    n, k, last = 1 << 24, 576, 40
+    rng = np.random.default_rng(15)
+    sizes = mp.w4_sizes(n, k)
+    assert sizes[0] > 1 << 32
+    codes, scales = (torch.zeros(b, dtype=torch.uint8, device="cuda") for b in sizes)
+    view = mp.W4Matrix(codes.data_ptr(), scales.data_ptr(), n, k)
+    w = ref.rounded(rng.standard_normal((last, k)), F32)
+    held = ref.held(w, E2M1)
+    mp.w4_pack(view, n - last, Floats(torch, w, F32).rows, last)
+    ids = torch.arange(n - last, n, dtype=torch.int32, device="cuda")
+    back = Floats(torch, np.zeros((last, k)), F32)
+    mp.w4_read(view, ids.data_ptr(), last, back.rows)
+    assert np.array_equal(back.back(), held)
+    for rows in (1, 33):
+        x = ref.rounded(rng.standard_normal((rows, k)), BF16)
+        source = Floats(torch, x, BF16)
+        out = torch.empty((rows, n), dtype=torch.bfloat16, device="cuda")
+        mp.w4_product(view, source.rows, rows, mp.Rows(out.data_ptr(), n, None, 0, BF16))
+        got = out[:, -last:].double().cpu().numpy()
+        close(got, x @ held.T, ref.product_bound(x, held, 1), BF16)
+        assert bool((out[:, :-last] == 0).all())
+        del out
