@@ -22,7 +22,8 @@ struct PackArgs {
 // and turns the codes round through LDS: there a lane of the result finds the 16
 // bytes of its row and group.
 //
-// Reads 4 (or 2) bytes an element and writes 17/32, which bounds it.
+// Reads 4 (or 2) bytes an element and writes 17/32, which bounds it: 49,152 x 576 in
+// FP32 32.5 us (3.9 TB/s), 12,288 x 4,096 in BF16 31 (4.1).
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads) w4_pack_kernel(PackArgs a) {
     constexpr int V = TYPE == MP_TYPE_F32 ? 4 : 8, L = kW4Group / V, RPI = 64 / L;  // elements, lanes a group, rows a load
@@ -97,8 +98,9 @@ struct ReadArgs {
 };
 
 // V consecutive columns of R rows a thread, 16 bytes of result each: the stores,
-// several times the codes' bytes, are what bounds it. Several rows share the
-// arithmetic of the places, where there are enough of them.
+// several times the codes' bytes, are what bounds it (49,152 x 576 in FP32 27.8 us,
+// 4.6 TB/s). Several rows share the arithmetic of the places, where there are enough
+// of them.
 template <int TYPE, int R>
 __global__ void __launch_bounds__(kThreads) w4_read_kernel(ReadArgs a) {
     constexpr int V = TYPE == MP_TYPE_F32 ? 4 : 8;

@@ -7,7 +7,8 @@ namespace {
 
 // Tiles of 16 by 16 (128 columns of depth a step, lane (c, g) of a tile with row
 // c at columns 32g ..+31), and of 32 by 32 (64 columns, lane (r, h) with row r at
-// columns 32h ..+31), which take less time an operation.
+// columns 32h ..+31), which take less time an operation: 1.87 PFLOP/s instead of
+// 1.29 from registers alone.
 template <int SIDE>
 struct Tile;
 template <>
@@ -40,6 +41,12 @@ struct Tile<32> {
 // the way through LDS of its own, so that wavefronts do not wait for each other.
 // Of a tile that is not full only the rows that are there are kept. What the next
 // block of depth needs is on its way while this one is multiplied.
+//
+// A single row is bounded by the weights' bytes: 12.4 to 14.5 us for the 53.5 MB of
+// a gated pair of 4,096 by 12,288 (3.7 to 4.3 TB/s; a large copy 5.1), 9.6 for
+// 12,288 by 4,096; small matrices by one chain of latencies, 4.3 us for FP32, 1,536
+// by 576. With more rows splitting FP32 into BF16 numbers takes the vector unit as
+// long as the products: 24 us for 64 rows of 4,096 by 4,096, 16 for 8 bits.
 template <int KIND, int SIDE, int NT, bool GATED>
 __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
     typedef Tile<SIDE> T;

@@ -104,7 +104,10 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& a, int64_t first_
 // A work-group of WN x WR wavefronts has 32 N WN columns (half of them of each
 // matrix of a gated pair) by 32 RT WR rows. It brings 64 columns of its rows to
 // LDS, as the BF16 numbers whose sums they are, while the columns before are
-// multiplied.
+// multiplied. 4,096 rows of 4,096 by 4,096: 124 us in BF16 (1.11 PFLOP/s; a large
+// library product of this card 1.41), 205 in FP16, 305 in FP32 (two and three BF16
+// numbers each: 1.34 and 1.35). 64 FP32 rows of 576 by 49,152, the small tiles' case,
+// take 18 to 20 us: 1.5 work-groups a CU, each 9 blocks long.
 template <int KIND, bool GATED, int N, int RT, int WN, int WR>
 __global__ void __launch_bounds__(64 * WN * WR, 2) w4_tiles_kernel(ProductArgs a) {
     constexpr int PARTS = parts_of(KIND), THREADS = 64 * WN * WR, TILES = RT * WR, ROWS = 32 * TILES;
@@ -254,6 +257,13 @@ __device__ __forceinline__ void bring(const uint8_t* from, void* to) {
 // block is multiplied from the registers, the next comes to them from LDS and the
 // one behind it from memory to LDS, so that a wavefront only ever waits for what
 // was asked for a whole block's products before.
+//
+// 4,096 rows through a gated pair of 4,096 by 12,288 take 414 to 480 us, 1.7 to 2.0
+// PFLOP/s; the products alone, from registers, take 290 to 330 (the card lowers its
+// clock), so the matrix cores, at 0.48 of the cycles, are what is nearest. Rows
+// through registers and weights straight from memory by both their readers took
+// 506 to 574: of that 82 went with the rows' loads left out, 70 with the weights',
+// 213 with both, the L1's 64 bytes a cycle being shared by the two.
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 2) w4_planes_kernel(ProductArgs a, const uint8_t* laid_rows) {
     constexpr int TILE = 1024;  // bytes of 32 columns of the matrix
