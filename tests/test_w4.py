@@ -663,3 +663,47 @@ def test_a_matrix_past_4_gib(torch_cuda):
         close(got, x @ held.T, ref.product_bound(x, held, 1), BF16)
         assert bool((out[:, :-last] == 0).all())
         del out
+
+
+@ANY
+@pytest.mark.parametrize("rows, n", [(1, 96), (5, 96), (20, 96), (70, 16384), (300, 22016)])
+def test_rows_behind_the_last_stay(torch_cuda, kind, rows, n):
+    """Results of `rows` rows in a buffer of more, beside their inputs in one matrix: everything else stays."""
+    torch = torch_cuda
+    rng = np.random.default_rng(rows)
+    k = 96
+    w = ref.held(rng.standard_normal((n, k)), E2M1)
+    matrix = Matrix(torch, n, k, w)
+    x = in_type(rng.standard_normal((rows + 3, k)), kind)
+    source = rows_of(torch, x, kind)
+    size = mp.w4_product_workspace(matrix.view, kind, rows)
+    space = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+    out = torch.full((rows + 3, n + 8), 5.0, device="cuda")
+    mp.w4_product(matrix.view, source.rows, rows, mp.Rows(out.data_ptr(), n + 8, None, 0, F32),
+                  workspace=space.data_ptr(), workspace_bytes=size)
+    got = out.double().cpu().numpy()
+    close(got[:rows, :n], x[:rows] @ w.T, ref.product_bound(x[:rows], w, PARTS[kind]), F32)
+    assert (got[rows:] == 5).all() and (got[:, n:] == 5).all()
+    eight = Eight(torch, rows + 3, n)
+    mp.w4_product(matrix.view, source.rows, rows, eight.rows, workspace=space.data_ptr(), workspace_bytes=size)
+    codes, scales = eight.bytes()
+    assert (codes[rows:] == -128).all() and (scales[rows:] == 255).all() and (scales[:rows] != 255).all()
+
+
+def test_other_calls_leave_rows_behind_the_last(torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(2)
+    for rows, width in ((3, 64), (5, 37), (2, 9000)):
+        x = rng.standard_normal((rows + 2, width))
+        source, residual = Floats(torch, x, F32), Floats(torch, x, F32)
+        out, total = Floats(torch, np.full((rows + 2, width), 5.0), F32), Floats(torch, np.full((rows + 2, width), 6.0), F32)
+        weight = torch.ones(width, device="cuda")
+        mp.rms_norm(source.rows, weight.data_ptr(), 1e-5, rows, width, out.rows, residual=residual.rows, sum=total.rows)
+        assert (out.back()[rows:] == 5).all() and (total.back()[rows:] == 6).all() and (out.back()[:rows] != 5).any()
+        mp.convert_rows(source.rows, rows, width, total.rows)
+        assert (total.back()[rows:] == 6).all() and np.array_equal(total.back()[:rows], source.back()[:rows])
+    m = Matrix(torch, 40, 64, ref.held(rng.standard_normal((40, 64)), E2M1))
+    ids = torch.arange(6, dtype=torch.int32, device="cuda")
+    out = Floats(torch, np.full((6, 64), 5.0), F32)
+    mp.w4_read(m.view, ids.data_ptr(), 4, out.rows)
+    assert (out.back()[4:] == 5).all() and (out.back()[:4] != 5).any()
