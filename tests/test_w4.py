@@ -707,3 +707,29 @@ def test_other_calls_leave_rows_behind_the_last(torch_cuda):
     out = Floats(torch, np.full((6, 64), 5.0), F32)
     mp.w4_read(m.view, ids.data_ptr(), 4, out.rows)
     assert (out.back()[4:] == 5).all() and (out.back()[:4] != 5).any()
+
+
+@ANY
+@pytest.mark.parametrize("rows, n", [(3, 250), (20, 250), (70, 16416), (300, 11008)])
+def test_gates_far_below_zero(torch_cuda, kind, rows, n):
+    """Gates down to -200, whose exp(-g) leaves FP32's range, with u up to 2^120: sums of one product each are exact, so
+    that the result is off by silu's roundings alone. The gate's few exponentials (a unit in the last place each) and
+    products are below 16 half steps."""
+    rng = np.random.default_rng(rows)
+    k = 64
+    g = -np.concatenate((np.arange(60, 128), np.arange(128, 201, 2))).astype(np.float64)  # numbers of 8 bits
+    x = np.zeros((rows, k))
+    x[:, 0], x[:, 32] = rng.permutation(np.resize(g, max(rows, len(g))))[:rows], 1.0
+    w, gate = np.zeros((n, k)), np.zeros((n, k))
+    gate[:, 0] = 1.0
+    w[:, 32] = np.exp2(120.0 - np.arange(n) % 221)
+    x = in_type(x, kind)
+    matrix, gates = Matrix(torch_cuda, n, k, w), Matrix(torch_cuda, n, k, gate)
+    source, out = rows_of(torch_cuda, x, kind), Floats(torch_cuda, np.zeros((rows, n)), F32)
+    size = mp.w4_product_workspace(matrix.view, kind, rows, True)
+    workspace = torch_cuda.empty(size + 16, dtype=torch_cuda.uint8, device="cuda")
+    mp.w4_product(matrix.view, source.rows, rows, out.rows, gate=gates.view, workspace=workspace.data_ptr(),
+                  workspace_bytes=size)
+    want = ref.product(x, w, gate)
+    assert (np.abs(want) > 2.0 ** -126).any(1).sum() > rows // 2
+    close(out.back(), want, 16 * 2.0 ** -24 * np.abs(want), F32)

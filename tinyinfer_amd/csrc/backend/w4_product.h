@@ -34,7 +34,32 @@ __device__ __forceinline__ uint32_t upper_halves(float u, float v) {
 // bits: exactly. 8-bit rows are BF16 numbers as they are.
 constexpr int parts_of(int kind) { return kind == MP_TYPE_F32 ? 3 : kind == MP_TYPE_F16 ? 2 : 1; }
 
-__device__ __forceinline__ float gated(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
+// silu(gate) * up. From -88.7 down exp(-gate) is infinite, while the product with
+// `up` can be any number. Below -80 silu is gate * exp(gate) far beyond the last bit,
+// and exp(gate) four equal factors: every number on the way is larger than the
+// result, so that only the last is rounded below the normal numbers. One branch for
+// all of a lane's results takes no time (4,096 8-bit rows through a pair of 4,096 by
+// 12,288: 451 us with it and without), one for each result 2 %.
+template <typename V>
+__device__ __forceinline__ V gated(const V& gate, const V& up) {
+    constexpr int N = sizeof(V) / sizeof(float);
+    V y;
+    float least = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        y[i] = gate[i] / (1.0f + expf(-gate[i])) * up[i];
+        least = fminf(least, gate[i]);
+    }
+    if (least < -80.0f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float quarter = expf(0.25f * gate[i]);
+            const float far = gate[i] * quarter * up[i] * quarter * quarter * quarter;
+            y[i] = gate[i] < -80.0f ? far : y[i];
+        }
+    }
+    return y;
+}
 
 // Results of `row`, columns n ..+3 of a tile.
 __device__ __forceinline__ void store_result(const ProductArgs& a, int64_t row, int n, const f4& v) {

@@ -157,10 +157,7 @@ __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
             v[m] = f4{0.f, 0.f, 0.f, 0.f};
             for (int w = 0; w < waves; ++w) v[m] += parts_s[(w * UNITS + (m * NT + i) * Q + q) * 64 + lane];
         }
-        if constexpr (GATED) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[0][k] = gated(v[1][k], v[0][k]);
-        }
+        if constexpr (GATED) v[0] = gated(v[1], v[0]);
         return v[0];
     };
     const int64_t row = (int64_t)row_block * SIDE + c;

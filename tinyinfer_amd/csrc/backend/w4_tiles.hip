@@ -91,10 +91,7 @@ __device__ __forceinline__ void store_tiles(const ProductArgs& a, int64_t first_
 #pragma unroll
         for (int i = 0; i < Weights<N, GATED>::EACH; ++i) {
             f16v v = sum[i][j];
-            if constexpr (GATED) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = gated(sum[i + N / 2][j][k], v[k]);
-            }
+            if constexpr (GATED) v = gated(sum[i + N / 2][j], v);
             store_tile(a, first_row + j * 32 + lane % 32, first_column + i * 32, lane / 32, v);
         }
 }
