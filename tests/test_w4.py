@@ -733,3 +733,27 @@ def test_gates_far_below_zero(torch_cuda, kind, rows, n):
     want = ref.product(x, w, gate)
     assert (np.abs(want) > 2.0 ** -126).any(1).sum() > rows // 2
     close(out.back(), want, 16 * 2.0 ** -24 * np.abs(want), F32)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("width", [64, 4099])
+def test_norm_below_the_normal_numbers(torch_cuda, kind, width):
+    """Results of 2^-140 to 2^-120, most of them a little beside the border of two BF16 numbers, by less than FP32 has
+    there: rounded once."""
+    rng = np.random.default_rng(width)
+    rows = 6
+    x = np.ones((rows, width))
+    x[1:, 0] = [1 + 2.0 ** -7, 0.5, 2.0, 0.75, 1.25]  # the row's root is a little more or less than 1
+    x[4] *= 1 + 2.0 ** -7
+    x = ref.rounded(x, kind)
+    halves = (2 * rng.integers(0, 128, width) + 1) * 2.0 ** -134
+    weight = np.where(rng.random(width) < 0.7, halves, np.exp2(rng.uniform(-140, -120, width))).astype(np.float32)
+    weight *= np.where(rng.random(width) < 0.5, -1, 1).astype(np.float32)
+    d_weight = torch_cuda.from_numpy(weight).cuda()
+    for epsilon in (0.0, 2.0 ** -17, 2.0 ** -12):
+        y = ref.norm(x, None, weight, epsilon)[1]
+        for to in (BF16, F16, F32):
+            out = Floats(torch_cuda, np.zeros((rows, width)), to)
+            source = Floats(torch_cuda, x, kind)
+            mp.rms_norm(source.rows, d_weight.data_ptr(), epsilon, rows, width, out.rows)
+            assert np.array_equal(out.back(), ref.rounded(y, to))
