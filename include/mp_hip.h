@@ -360,10 +360,11 @@ int mp_hip_kv8_attention_prefill(const mp_kv8_cache* cache, int32_t layer, const
  * Matrices. `rows` (1 to 2^24) by `depth` (a multiple of 32 up to 2^20)
  * weights; each is an E2M1 number (0, 0.5, 1, 1.5, 2, 3, 4, 6, or their
  * negatives) times a power of two per 32 weights along the row, chosen like
- * that of 8-bit rows (a magnitude above 6 * 2^120 makes it NaN). Codes lie by tiles of 16 rows and 128 columns,
+ * that of 8-bit rows (a magnitude above 6 * 2^120 makes it NaN). Codes lie by
+ * tiles of 16 rows and 128 columns,
  * [rows/16][depth/128][column%128/32][row%16][16 bytes], even columns in the
- * low halves of the bytes, code 8 + c the negative of c; scale bytes as above, 27
- * to 247, are
+ * low halves of the bytes, code 8 + c the negative of c; scale bytes as above (27
+ * to 247; 255: NaN) are
  * [rows/16][depth/512][column%128/32][row%16][column%512/128]: the matrix cores'
  * operands. Tiles are whole, filled up with zeros. Both are 16-byte aligned and
  * of the sizes that mp_hip_w4_sizes says. */
@@ -412,13 +413,16 @@ int mp_hip_rms_norm(const mp_rows* x, const mp_rows* residual, const mp_rows* su
  * size the gated pair g / (1 + exp(-g)) * u of g = x gate^T and u = x w^T. x and
  * out are rows of any type (8-bit results need w->rows to be a multiple of 32).
  * One to 2^20 rows: single tokens read the weights' 4 bits once, prompts are the
- * matrix cores' work. Rows and weights count as they are, sums are FP32, and the
- * result is rounded once, to out's type. A row with a NaN or an
+ * matrix cores' work. Rows and weights count as they are (an FP32 element below
+ * 2^-110 without what of it lies below 2^-133), sums are FP32 (nothing below
+ * 2^-149), and the result is rounded once, to out's type. A row with a NaN or an
  * infinity has no finite result, and a NaN scale of a matrix's row none in its
- * column; other rows and columns are as without them. The workspace (16-byte
- * aligned; mp_hip_w4_product_workspace says its size for the same or more rows; 0 is
- * possible, and then it may be NULL) holds nothing between calls; calls that may
- * overlap, replayed graphs among them, need workspaces of their own. */
+ * column; other rows and columns are as without them. Refused are products of more
+ * than 2^22 tiles of 128 rows by 256 results (by 128 of a gated pair), and of more
+ * than 2^22 blocks of 128 rows by 64 elements in 8 bits. The workspace (16-byte
+ * aligned; mp_hip_w4_product_workspace says its size for the same or more rows; 0
+ * is possible, and then it may be NULL) holds nothing between calls; calls that
+ * may overlap, replayed graphs among them, need workspaces of their own. */
 int mp_hip_w4_product_workspace(const mp_w4_matrix* w, int32_t type, int32_t rows, int32_t gated, size_t* bytes);
 int mp_hip_w4_product(const mp_w4_matrix* w, const mp_w4_matrix* gate, const mp_rows* x, int32_t rows,
                       const mp_rows* out, void* workspace, size_t workspace_bytes, void* stream);

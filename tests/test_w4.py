@@ -757,3 +757,60 @@ def test_norm_below_the_normal_numbers(torch_cuda, kind, width):
             source = Floats(torch_cuda, x, kind)
             mp.rms_norm(source.rows, d_weight.data_ptr(), epsilon, rows, width, out.rows)
             assert np.array_equal(out.back(), ref.rounded(y, to))
+
+
+# Rows and weights times these powers of two; 8-bit rows and weights have scales of 2^-100 to 2^120.
+POWERS = [(-98, 0), (-108, 0), (-122, 0), (-130, 0), (-122, 60), (-130, 60), (-90, -36), (-90, -40), (-70, -70), (-98, -98),
+          (-95, 115), (-90, 100), (5, 115), (100, -90), (117, -98), (117, -4), (3, 117)]
+
+
+@ANY
+@pytest.mark.parametrize("rows, n", [(1, 64), (20, 64), (70, 16416), (300, 22016)])
+def test_products_over_all_magnitudes(torch_cuda, kind, rows, n):
+    """Rows and weights near both ends of their ranges. Beside the ordinary bound: what of an FP32 element lies below
+    2^-133 does not count, and products and sums are multiples of 2^-149 (one step lost for each of them at the most,
+    and there are no more sums than products)."""
+    rng = np.random.default_rng(rows)
+    k = 96
+    ways = [0] if kind == F16 else range(len(POWERS))  # FP16 has no such range
+    x0, w0 = rng.standard_normal((rows, k)), ref.held(rng.standard_normal((n, k)), E2M1)
+    for i in ways:
+        a, b = (-13, 117) if kind == F16 else POWERS[i]
+        x, w = in_type(x0 * 2.0 ** a, kind), ref.held(w0 * 2.0 ** b, E2M1)
+        matrix, source = Matrix(torch_cuda, n, k, w), rows_of(torch_cuda, x, kind)
+        size = mp.w4_product_workspace(matrix.view, kind, rows)
+        workspace = torch_cuda.empty(size + 16, dtype=torch_cuda.uint8, device="cuda")
+        bound = ref.product_bound(x, w, PARTS[kind]) + 2 * 128 * PARTS[kind] * 2.0 ** -149
+        if kind == F32 and a < -105:  # else all elements but the smallest are exact, and those are lost in the bound
+            bound += 2.0 ** -133 * np.abs(w).sum(1)
+        for to in (F32, BF16):
+            out = Floats(torch_cuda, np.zeros((rows, n)), to)
+            mp.w4_product(matrix.view, source.rows, rows, out.rows, workspace=workspace.data_ptr(), workspace_bytes=size)
+            close(out.back(), x @ w.T, bound, to)
+
+
+@pytest.mark.parametrize("rows, n", [(1, 64), (20, 64), (70, 16416), (300, 22016)])
+def test_fp32_elements_are_exact_from_2_to_the_minus_110_on(torch_cuda, rows, n):
+    """One element a row, 24 bits long: its product with a power of two is the element, and below 2^-110 it is cut to a
+    multiple of 2^-133."""
+    rng = np.random.default_rng(rows)
+    k = 64
+    x = np.zeros((rows, k))
+    one = 1 + rng.integers(0, 1 << 23, rows) * 2.0 ** -23
+    x[:, 7] = one * np.exp2(-105.0 - np.arange(rows) % 30) * np.where(rng.random(rows) < 0.5, 1, -1)
+    if rows == 1:
+        x[0, 7] = 2.0 ** -110 * (2 - 2.0 ** -23)
+    x = ref.rounded(x, F32)
+    w = np.zeros((n, k))
+    w[:, 7] = np.exp2(np.arange(n) % 90)
+    matrix, source, out = Matrix(torch_cuda, n, k, w), Floats(torch_cuda, x, F32), Floats(torch_cuda, np.zeros((rows, n)), F32)
+    mp.w4_product(matrix.view, source.rows, rows, out.rows)
+    held = np.where(np.abs(x) < 2.0 ** -110, np.trunc(x * 2.0 ** 133) * 2.0 ** -133, x)
+    assert np.array_equal(out.back(), held @ w.T)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, I8], ids=["f32", "bf16", "i8"])
+@pytest.mark.parametrize("scale", [2.0 ** -40, 2.0 ** 40])
+@pytest.mark.parametrize("rows, n", [(1, 64), (20, 64), (70, 16416), (300, 11008)])
+def test_gated_products_of_small_and_large_rows(torch_cuda, kind, rows, n, scale):
+    check_product(torch_cuda, np.random.default_rng(rows), rows, n, 96, kind, F32, True, scale=scale)

@@ -177,3 +177,15 @@ def test_the_reference_itself():
         for value, byte in ((most * 2.0 ** 120, 247), (most * 2.0 ** 120 * 1.001, 255), (np.inf, 255), (np.nan, 255), (0.0, 27),
                             (most * 2.0 ** -100, 27), (most * 2.0 ** -99, 28)):
             assert ref.split(np.full((1, 32), value), grid)[2].tolist() == [[byte]]
+
+
+@pytest.mark.parametrize("count, n, depth, kind, gated", [
+    (1 << 20, (1 << 17) + 1, 32, mp.TYPE_BF16, False), (1 << 20, (1 << 16) + 1, 32, mp.TYPE_F32, True),
+    ((1 << 13) + 1, 1 << 24, 32, mp.TYPE_F16, False), (1 << 20, 4096, 32800, mp.TYPE_I8, False)])
+def test_products_too_large_for_one_call_are_refused(count, n, depth, kind, gated):
+    stride = -(-depth // 128) * 128
+    x = rows(stride=stride, type=kind) if kind != mp.TYPE_I8 else eight(stride=stride, scale_stride=stride // 32)
+    m = matrix(rows=n, depth=depth)
+    size = mp.w4_product_workspace(m, kind, count, gated)
+    refused(lambda: product(m, x, count, out(stride=n), gate=m if gated else None, workspace=P, workspace_bytes=size),
+            "too large for one call")

@@ -39,9 +39,11 @@ struct W4View {
 
 // ---- scales and codes ----------------------------------------------------------
 
-// Scales go down to 2^-100: what is smaller is rounded on that grid, and no
-// product of two scales and codes comes near the smallest FP32 numbers. They go
-// up to 2^120, so that the products' factors stay in range.
+// Scales go down to 2^-100: what is smaller is rounded on that grid, and codes times
+// scales and the scales' inverses are normal numbers. They go up to 2^120, so that
+// 127 times one is finite and the planes' scales, up to 2^7 more, have a byte.
+// Products of two small elements may be smaller than FP32's numbers: they vanish, as
+// in any FP32 sum.
 constexpr uint32_t kLeastScale = 27, kMostScale = 247, kNanScale = 255;
 
 // The scale byte of a group by the bits of its largest magnitude: the smallest

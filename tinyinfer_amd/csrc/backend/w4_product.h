@@ -31,7 +31,8 @@ __device__ __forceinline__ uint32_t upper_halves(float u, float v) {
     return __builtin_amdgcn_perm(__float_as_uint(v), __float_as_uint(u), 0x07060302u);
 }
 // A float row's elements as sums of this many BF16 numbers, each the next 8
-// bits: exactly. 8-bit rows are BF16 numbers as they are.
+// bits: exactly, but for FP32 elements below 2^-110, of which BF16 numbers, multiples
+// of 2^-133, hold no more than those. 8-bit rows are BF16 numbers as they are.
 constexpr int parts_of(int kind) { return kind == MP_TYPE_F32 ? 3 : kind == MP_TYPE_F16 ? 2 : 1; }
 
 // silu(gate) * up. From -88.7 down exp(-gate) is infinite, while the product with
