@@ -10,6 +10,7 @@ from tinyinfer_amd import backend as mp
 
 from . import w4_reference as ref
 from .w4_reference import BF16, E2M1, F16, F32, HALF_STEP, I8, LEAST, TORCH, WHOLE
+from .w4_sizes import CALLS, CALLS_EIGHT
 
 pytestmark = pytest.mark.gpu
 
@@ -814,3 +815,146 @@ def test_fp32_elements_are_exact_from_2_to_the_minus_110_on(torch_cuda, rows, n)
 @pytest.mark.parametrize("rows, n", [(1, 64), (20, 64), (70, 16416), (300, 11008)])
 def test_gated_products_of_small_and_large_rows(torch_cuda, kind, rows, n, scale):
     check_product(torch_cuda, np.random.default_rng(rows), rows, n, 96, kind, F32, True, scale=scale)
+
+
+def packed(torch, rng, n, k):
+    """A matrix of every code and scales around 2^-5, packed on the GPU, and its values."""
+    w = E2M1[rng.integers(0, 8, (n, k))] * np.exp2(rng.integers(-8, -3, (n, k // 32))).repeat(32, 1)
+    w *= 1 - 2 * rng.integers(0, 2, (n, k))
+    m = Matrix(torch, n, k)
+    mp.w4_pack(m.view, 0, Floats(torch, w, F32).rows, n)
+    torch.cuda.synchronize()
+    return m, w
+
+
+def product_of(torch, matrix, gate, source, rows, n, kind, out):
+    size = mp.w4_product_workspace(matrix.view, kind, rows, gate is not None)
+    workspace = torch.empty(size + 64, dtype=torch.uint8, device="cuda").fill_(0xFF)
+    mp.w4_product(matrix.view, source.rows, rows, out.rows, gate=gate.view if gate else None,
+                  workspace=workspace.data_ptr(), workspace_bytes=size)
+    got = out.back()
+    out.check_padding()
+    assert bool((workspace[size:] == 0xFF).all())
+    return got
+
+
+@pytest.mark.parametrize("rows, n, k", [call[:3] for call in CALLS])
+def test_every_way_of_a_product(torch_cuda, rows, n, k):
+    """Every kernel that sizes can lead to (w4_sizes.py), for every type of rows, alone and gated, results of odd rows."""
+    rng = np.random.default_rng(rows + n + k)
+    (matrix, w), (gate, g) = packed(torch_cuda, rng, n, k), packed(torch_cuda, rng, n, k)
+    for kind in (F32, BF16, F16, I8):
+        x = in_type(rng.standard_normal((rows, k)) * np.exp(rng.standard_normal(k)), kind)
+        source = rows_of(torch_cuda, x, kind, 16)
+        for gates in (None, g):
+            want = ref.product(x, w, gates)
+            bound = ref.product_bound(x, w, PARTS[kind]) if gates is None else ref.gated_bound(x, w, g, PARTS[kind])
+            for to, pad in ((F32, 3), (kind if kind != I8 else F16, 0)):
+                out = Floats(torch_cuda, np.zeros((rows, n)), to, pad)
+                got = product_of(torch_cuda, matrix, gate if gates is not None else None, source, rows, n, kind, out)
+                close(got, want, bound, to)
+                if to == F32:  # in earnest, as FP32 sums are
+                    off = np.linalg.norm(got - want) / np.linalg.norm(want)
+                    assert off < 1e-6, off
+
+
+@pytest.mark.parametrize("rows, n, k", [call[:3] for call in CALLS_EIGHT])
+def test_8_bit_results_of_every_way(torch_cuda, rows, n, k):
+    """Results in 8 bits are those of the same sums in FP32, bit for bit: codes, scales, no code below -127."""
+    rng = np.random.default_rng(rows + n + k)
+    (matrix, w), (gate, g) = packed(torch_cuda, rng, n, k), packed(torch_cuda, rng, n, k)
+    for kind in (F32, BF16, F16, I8):
+        x = in_type(rng.standard_normal((rows, k)) * np.exp(rng.standard_normal(k)), kind)
+        source = rows_of(torch_cuda, x, kind)
+        for gates in (None, g):
+            m = gate if gates is not None else None
+            sums = product_of(torch_cuda, matrix, m, source, rows, n, kind, Floats(torch_cuda, np.zeros((rows, n)), F32))
+            bound = ref.product_bound(x, w, PARTS[kind]) if gates is None else ref.gated_bound(x, w, g, PARTS[kind])
+            close(sums, ref.product(x, w, gates), bound, F32)
+            out = Eight(torch_cuda, rows, n, None, 16)
+            product_of(torch_cuda, matrix, m, source, rows, n, kind, out)
+            code, sign, s = ref.split(sums, WHOLE)
+            codes, scales = out.bytes()
+            assert np.array_equal(scales, s) and np.array_equal(codes, np.where(sign, -code, code))
+
+
+@TYPES
+@pytest.mark.parametrize("over, pad, shift", [(1, 0, 0), (7, 8, 8), (3, 3, 1)])
+def test_reads_of_many_rows(torch_cuda, kind, over, pad, shift):
+    """From 2^22 runs of 16 bytes on a thread has eight rows: counts that are no multiple of eight, ids that are no rows
+    beside others, rows behind the last."""
+    torch = torch_cuda
+    rng = np.random.default_rng(over)
+    n, k = 53, 544
+    runs = k // (4 if kind == F32 else 8)
+    count = -(-(1 << 22) // runs) // 8 * 8 + 8 + over
+    matrix, w = packed(torch, rng, n, k)
+    ids = rng.integers(0, n, count).astype(np.int32)
+    ids[rng.random(count) < 0.05] = -1
+    ids[rng.random(count) < 0.05] = n
+    ids[rng.random(count) < 0.01] = -(1 << 31)
+    ids[-1], ids[0] = n - 1, (1 << 31) - 1
+    d_ids = torch.from_numpy(ids).cuda()
+    width = k + pad
+    buffer = torch.full(((count + 3) * width + shift,), 77.0, dtype=getattr(torch, TORCH[kind]), device="cuda")
+    out = buffer[shift:].view(count + 3, width)
+    mp.w4_read(matrix.view, d_ids.data_ptr(), count, mp.Rows(out.data_ptr(), width, None, 0, kind))
+    there = torch.from_numpy((ids >= 0) & (ids < n)).cuda()
+    table = torch.from_numpy(ref.rounded(w, kind)).cuda().to(buffer.dtype)
+    want = table[d_ids.clamp(0, n - 1).long()]
+    assert bool((out[:count, :k] == want)[there].all())
+    assert bool(out[:count, :k][~there].isnan().all())
+    assert bool((out[count:] == 77).all()) and bool((out[:, k:] == 77).all()) and bool((buffer[:shift] == 77).all())
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows, width, pad, shift", [(3, 64, 0, 0), (5, 576, 3, 1), (2, 16512, 0, 0), (2, 16512, 1, 1), (9, 120, 0, 0)])
+def test_norm_from_every_type_to_every_type(torch_cuda, kind, rows, width, pad, shift):
+    rng = np.random.default_rng(width + pad)
+    x, r = (ref.rounded(rng.standard_normal((rows, width)), kind) for _ in range(2))
+    weight = (1 + 0.2 * rng.standard_normal(width)).astype(np.float32)
+    d_weight = torch_cuda.from_numpy(weight).cuda()
+    for residual in (None, r):
+        y = ref.norm(x, residual, weight, 1e-6)[1]
+        for to in (F32, BF16, F16) + ((I8,) if width % 32 == 0 else ()):
+            source = Floats(torch_cuda, x, kind, pad, shift)
+            added = Floats(torch_cuda, residual, kind, pad, shift) if residual is not None else None
+            out = empty(torch_cuda, rows, width, to, 16 * pad if to == I8 else pad)
+            mp.rms_norm(source.rows, d_weight.data_ptr(), 1e-6, rows, width, out.rows, residual=added.rows if added else None)
+            assert np.array_equal(out.back(), ref.held(y, WHOLE) if to == I8 else ref.rounded(y, to))
+            out.check_padding()
+
+
+@pytest.mark.parametrize("pad", [0, 1])
+def test_conversion_of_extremes(torch_cuda, pad):
+    """Numbers near the smallest and the largest of each type, ties among them, and 8-bit rows with the outermost scales."""
+    rng = np.random.default_rng(pad)
+    width = 256
+    x = np.exp2(rng.uniform(-149, 128, (40, width))) * rng.choice([-1, 1], (40, width))
+    x[0] = np.arange(width) * 2.0 ** -149
+    x[1] = (2 * np.arange(width) + 1) * 2.0 ** -134  # between two BF16 numbers
+    x[2] = (2 * np.arange(width) + 1) * 2.0 ** -25  # between two FP16 numbers
+    x[3] = 65504 + np.arange(width) / 8  # up to and past the border to infinity
+    x[4] = (2 - 2.0 ** -8 - np.arange(-128, 128) * 2.0 ** -23) * 2.0 ** 127
+    for kind in (F32, BF16, F16):
+        with np.errstate(over="ignore"):
+            held = ref.rounded(x, kind)
+        source = Floats(torch_cuda, held, kind, pad)
+        for to in (F32, BF16, F16):
+            out = Floats(torch_cuda, np.zeros(x.shape), to, pad)
+            mp.convert_rows(source.rows, len(x), width, out.rows)
+            assert np.array_equal(out.back(), ref.rounded(held, to))
+        eight = Eight(torch_cuda, len(x), width)
+        mp.convert_rows(source.rows, len(x), width, eight.rows)
+        code, sign, s = ref.split(held, WHOLE)
+        codes, scales = eight.bytes()
+        fine = (s != 255).repeat(32, 1)
+        assert np.array_equal(scales, s) and np.array_equal(codes[fine], np.where(sign, -code, code)[fine])
+    codes, scales = rng.integers(-127, 128, (40, width)), rng.choice([27, 28, 100, 110, 127, 140, 246, 247], (40, 8))
+    eight = Eight(torch_cuda, 40, width)
+    eight.codes.copy_(torch_cuda.from_numpy(codes.astype(np.int8)))
+    eight.scales[:, :8] = torch_cuda.from_numpy(scales.astype(np.uint8))
+    for to in (F32, BF16, F16):
+        out = Floats(torch_cuda, np.zeros((40, width)), to, pad)
+        mp.convert_rows(eight.rows, 40, width, out.rows)
+        assert np.array_equal(out.back(), ref.rounded(codes * np.exp2(scales - 127.0).repeat(32, 1), to))

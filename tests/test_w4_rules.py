@@ -10,6 +10,7 @@ import pytest
 from tinyinfer_amd import backend as mp
 
 from . import w4_reference as ref
+from .w4_sizes import CALLS, CALLS_EIGHT
 
 ROOT = Path(__file__).resolve().parent.parent
 GXX = shutil.which("g++")
@@ -189,3 +190,27 @@ def test_products_too_large_for_one_call_are_refused(count, n, depth, kind, gate
     size = mp.w4_product_workspace(m, kind, count, gated)
     refused(lambda: product(m, x, count, out(stride=n), gate=m if gated else None, workspace=P, workspace_bytes=size),
             "too large for one call")
+
+
+@pytest.mark.skipif(GXX is None, reason="g++ not available")
+def test_calls_take_every_way(tmp_path):
+    """The calls of w4_sizes.py take the ways that they are there for, and leave none out that sizes can lead to."""
+    exe = tmp_path / "w4_plan_of"
+    subprocess.run([GXX, "-std=c++17", "-O2", "-Wall", "-Werror", f"-I{ROOT / 'tinyinfer_amd' / 'csrc' / 'backend'}",
+                    str(ROOT / "tests" / "native" / "w4_plan_of.cpp"), "-o", str(exe)], check=True)
+
+    def plan(*args):
+        run = subprocess.run([str(exe), *map(str, args)], capture_output=True, text=True, check=True)
+        return [tuple(map(int, line.split())) for line in run.stdout.splitlines()]
+
+    taken = set()
+    for eight, calls in ((0, CALLS), (1, CALLS_EIGHT)):
+        for call in calls:
+            for gated, want in ((0, call.plain), (1, call.gated)):
+                for parts in (1, 2, 3):
+                    got, = plan(call.rows, call.n, call.k, parts, gated, eight)
+                    assert got[:3] == want, call
+                    if eight and len(got) == 4:  # the same sums as with results in FP32
+                        assert plan(call.rows, call.n, call.k, parts, gated, 0)[0][3] == got[3], call
+                taken.add((gated, eight, *want))
+    assert taken == set(plan())
