@@ -958,3 +958,100 @@ def test_conversion_of_extremes(torch_cuda, pad):
         out = Floats(torch_cuda, np.zeros((40, width)), to, pad)
         mp.convert_rows(eight.rows, 40, width, out.rows)
         assert np.array_equal(out.back(), ref.rounded(codes * np.exp2(scales - 127.0).repeat(32, 1), to))
+
+
+@pytest.mark.parametrize("width, pad", [(64, 0), (544, 48)])
+def test_8_bit_rows_in_place(torch_cuda, width, pad):
+    """Rows whose scales are not the smallest get those, in their own memory; values stay."""
+    rng = np.random.default_rng(width)
+    rows = 37
+    eight = Eight(torch_cuda, rows, width, None, pad)
+    codes = rng.integers(-127, 128, (rows, width // 32, 32)) >> rng.integers(0, 8, (rows, width // 32, 1))
+    codes[3, 1] = 0
+    scales = rng.integers(40, 240, (rows, width // 32))
+    scales[5, 0] = 255
+    eight.codes[:, :width] = torch_cuda.from_numpy(codes.reshape(rows, width).astype(np.int8))
+    eight.scales[:, :width // 32] = torch_cuda.from_numpy(scales.astype(np.uint8))
+    before = eight.back()
+    mp.convert_rows(eight.rows, rows, width, eight.rows)
+    assert np.array_equal(eight.back(), before, equal_nan=True)
+    code, sign, s = ref.split(before, WHOLE)
+    got, got_scales = eight.bytes()
+    fine = (s != 255).repeat(32, 1)
+    assert np.array_equal(got_scales, s) and np.array_equal(got[fine], np.where(sign, -code, code)[fine])
+    eight.check_padding()
+
+
+@pytest.mark.parametrize("n, k", [(53, 96), (4000, 544)])
+def test_packing_and_reading_replayed(torch_cuda, n, k):
+    """Captured and replayed for other weights, with eager calls between; the same id twice and more."""
+    torch = torch_cuda
+    rng = np.random.default_rng(n)
+    source = Floats(torch, np.zeros((n, k)), BF16)
+    m, out = Matrix(torch, n, k), Floats(torch, np.zeros((n + 9, k)), F32)
+    ids = torch.from_numpy(np.concatenate((rng.permutation(n), [0] * 5, [n - 1] * 4)).astype(np.int32)).cuda()
+
+    def step(stream):
+        mp.w4_pack(m.view, 0, source.rows, n, stream=stream)
+        mp.w4_read(m.view, ids.data_ptr(), n + 9, out.rows, stream=stream)
+
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        step(torch.cuda.current_stream().cuda_stream)
+    for _ in range(4):
+        x = ref.rounded(rng.standard_normal((n, k)), BF16)
+        source.matrix.copy_(torch.from_numpy(x))
+        graph.replay()
+        assert np.array_equal(out.back(), ref.held(x, E2M1)[ids.cpu().numpy()])
+        source.matrix.mul_(-1)
+        step(None)
+        assert np.array_equal(out.back(), ref.held(-x, E2M1)[ids.cpu().numpy()])
+
+
+def test_parts_of_a_tile_packed_on_two_streams(torch_cuda):
+    """Rows of one tile by calls that may overlap: each writes its own."""
+    torch = torch_cuda
+    rng = np.random.default_rng(6)
+    n, k = 16 * 40, 544
+    x = ref.rounded(rng.standard_normal((n, k)), F32)
+    want = ref.pack(x)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        m, pieces = Matrix(torch, n, k), []
+        torch.cuda.synchronize()
+        for first in range(0, n, 5):
+            count = min(5, n - first)
+            pieces.append(Floats(torch, x[first:first + count], F32))
+        torch.cuda.synchronize()
+        for i, piece in enumerate(pieces):
+            mp.w4_pack(m.view, 5 * i, piece.rows, piece.matrix.shape[0], stream=streams[i % 2].cuda_stream)
+        codes, scales = m.bytes()
+        signs = [np.where((c & 15) == 8, c & 0xF0, c) for c in (codes, want[0])]
+        signs = [np.where((c >> 4) == 8, c & 0x0F, c) for c in signs]
+        assert np.array_equal(*signs) and np.array_equal(scales, want[1])
+
+
+@ANY
+@pytest.mark.parametrize("rows", [1, 20])
+def test_the_deepest_products(torch_cuda, kind, rows):
+    rng = np.random.default_rng(rows)
+    n, k = 33, 1 << 20
+    matrix, w = packed(torch_cuda, rng, n, k)
+    x = in_type(rng.standard_normal((rows, k)), kind)
+    out = Floats(torch_cuda, np.zeros((rows, n)), F32)
+    got = product_of(torch_cuda, matrix, None, rows_of(torch_cuda, x, kind), rows, n, kind, out)
+    close(got, x @ w.T, ref.product_bound(x, w, PARTS[kind]), F32)
+
+
+@pytest.mark.parametrize("width, pad", [(1 << 20, 0), ((1 << 20) - 1, 1)])
+def test_the_widest_rows(torch_cuda, width, pad):
+    rng = np.random.default_rng(pad)
+    x = ref.rounded(rng.standard_normal((2, width)), BF16)
+    weight = np.ones(width, np.float32)
+    d_weight = torch_cuda.from_numpy(weight).cuda()
+    source, out = Floats(torch_cuda, x, BF16, pad), Floats(torch_cuda, np.zeros((2, width)), F16, pad)
+    mp.rms_norm(source.rows, d_weight.data_ptr(), 1e-5, 2, width, out.rows)
+    assert np.array_equal(out.back(), ref.rounded(ref.norm(x, None, weight, 1e-5)[1], F16))
+    mp.convert_rows(source.rows, 2, width, out.rows)
+    assert np.array_equal(out.back(), ref.rounded(x, F16))
+    out.check_padding()
