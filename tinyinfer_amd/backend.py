@@ -296,22 +296,22 @@ def kv8_append(cache: Kv8Cache, layer: int, k, k_stride: int, v, v_stride: int, 
     8-bit cache, and the rotated queries to q_out (raw device pointers;
     strides in elements). Asynchronous on `stream`."""
     _check_call(lib().mp_hip_kv8_append(cache, layer, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride,
-                                       heads, type, rope, tables, table_stride, starts, used, sequences, rows,
-                                       stream), "mp_hip_kv8_append")
+                                        heads, type, rope, tables, table_stride, starts, used, sequences, rows,
+                                        stream), "mp_hip_kv8_append")
 
 
 def kv8_read(cache: Kv8Cache, layer: int, tables, table_stride: int, starts, used, sequences: int, rows: int,
              type: int, k, k_stride: int, v, v_stride: int, stream: int | None = None):
     """Tokens of an 8-bit cache as rows of values. Asynchronous on `stream`."""
     _check_call(lib().mp_hip_kv8_read(cache, layer, tables, table_stride, starts, used, sequences, rows, type, k,
-                                     k_stride, v, v_stride, stream), "mp_hip_kv8_read")
+                                      k_stride, v, v_stride, stream), "mp_hip_kv8_read")
 
 
 def kv8_attention_workspace(cache: Kv8Cache, rows: int, sequences: int, heads: int, max_length: int) -> int:
     """Workspace bytes for the attention calls of up to these sizes."""
     size = ctypes.c_size_t()
     _check_call(lib().mp_hip_kv8_attention_workspace(cache, rows, sequences, heads, max_length, ctypes.byref(size)),
-               "mp_hip_kv8_attention_workspace")
+                "mp_hip_kv8_attention_workspace")
     return size.value
 
 
@@ -321,8 +321,8 @@ def kv8_attention_decode(cache: Kv8Cache, layer: int, q, q_stride: int, type: in
     """Attention of one query row per sequence over an 8-bit cache; `lengths`
     on the device. Asynchronous on `stream`."""
     _check_call(lib().mp_hip_kv8_attention_decode(cache, layer, q, q_stride, type, tables, table_stride, lengths, rows,
-                                                 heads, max_length, scale, out, out_stride, workspace,
-                                                 workspace_bytes, stream), "mp_hip_kv8_attention_decode")
+                                                  heads, max_length, scale, out, out_stride, workspace,
+                                                  workspace_bytes, stream), "mp_hip_kv8_attention_decode")
 
 
 def kv8_attention_prefill(cache: Kv8Cache, layer: int, q, q_stride: int, type: int, tables, table_stride: int,
@@ -331,8 +331,8 @@ def kv8_attention_prefill(cache: Kv8Cache, layer: int, q, q_stride: int, type: i
     """Causal attention of packed rows over an 8-bit cache that holds them
     already. Asynchronous on `stream`."""
     _check_call(lib().mp_hip_kv8_attention_prefill(cache, layer, q, q_stride, type, tables, table_stride, starts, used,
-                                                  sequences, rows, heads, max_length, scale, out, out_stride,
-                                                  workspace, workspace_bytes, stream), "mp_hip_kv8_attention_prefill")
+                                                   sequences, rows, heads, max_length, scale, out, out_stride,
+                                                   workspace, workspace_bytes, stream), "mp_hip_kv8_attention_prefill")
 
 
 def w4_sizes(rows: int, depth: int) -> tuple[int, int]:

@@ -223,9 +223,12 @@ __device__ __forceinline__ double inverse_root(double v) {
 // Sums, the root and the products are FP64, a single rounding an element: an
 // 8-bit code next to the border of two would go either way by the order of an
 // FP32 sum. The FP64 unit is as wide as the FP32 one: 4,096 x 4,096 BF16 rows with a
-// residual, to 8 bits, take 31 us, 3.8 TB/s in five streams, with the vector unit
+// residual, to 8 bits, take 32 us, 3.7 TB/s in five streams, with the vector unit
 // busy for half of it. One row of 576 takes 2.3 us (3.0 with one wavefront of two
-// chunks), 777 unaligned FP16 rows of 2,047 5.7: latency.
+// chunks), a chain of latencies. Rows that do not begin at 16 bytes are read by
+// elements: with a residual 777 FP16 rows of 2,047 take 9.0 us, of 2,048 5.7. Rows
+// of fewer than 512 elements leave lanes idle: 131,072 BF16 rows of 64 take 42 us (a
+// copy's 7), as many of 128 41 (13), 65,536 of 256 23 (13), 32,768 of 512 15 (13).
 template <int TYPE, int OUT, bool RESIDUAL, bool WIDE, int C>
 __global__ void __launch_bounds__(1024) rms_norm_kernel(NormArgs a, int waves) {
     __shared__ double sums[16];

@@ -42,11 +42,14 @@ struct Tile<32> {
 // Of a tile that is not full only the rows that are there are kept. What the next
 // block of depth needs is on its way while this one is multiplied.
 //
-// A single row is bounded by the weights' bytes: 12.4 to 14.5 us for the 53.5 MB of
-// a gated pair of 4,096 by 12,288 (3.7 to 4.3 TB/s; a large copy 5.1), 9.6 for
-// 12,288 by 4,096; small matrices by one chain of latencies, 4.3 us for FP32, 1,536
-// by 576. With more rows splitting FP32 into BF16 numbers takes the vector unit as
-// long as the products: 24 us for 64 rows of 4,096 by 4,096, 16 for 8 bits.
+// A single row reads the weights once. The gated pair of 4,096 by 12,288, with four
+// tiles of a wavefront on their way, is bounded by those bytes: 14.5 us for 53.5 MB,
+// 3.7 TB/s (a large copy 5.1). Square and deep matrices leave a wavefront one tile, a
+// kilobyte on its way, and are bounded by latency: 9.6 us for 12,288 by 4,096 (2.8
+// TB/s), 6.1 for 4,096 by 4,096 (1.5). Small ones are one chain of latencies, 4.3 us
+// for FP32, 1,536 by 576. With more rows every work-group reads and turns round all of
+// its rows for 32 or 64 columns, and splitting FP32 into BF16 numbers takes the vector
+// unit as long as the products: 24 us for 64 rows of 4,096 by 4,096, 16 for 8 bits.
 template <int KIND, int SIDE, int NT, bool GATED>
 __global__ void __launch_bounds__(512) w4_few_kernel(ProductArgs a) {
     typedef Tile<SIDE> T;

@@ -23,9 +23,10 @@ constexpr size_t w4_scale_bytes(int64_t rows, int64_t depth) { return (size_t)(w
 // Elements of a call on rows alone (norm, conversion): 2^30 threads of 8.
 constexpr int64_t kRowsMostElements = (int64_t)1 << 33;
 
-// Runs of 16 bytes from which on a read takes 8 rows a thread: 26.3 us instead of
-// 31.1 for 49,152 FP32 rows of 576 (7 million runs), but 15.0 instead of 13.9 for
-// 16,000 of them (2 million) and 4.1 instead of 2.4 for 64.
+// Runs of 16 bytes from which on a read takes 8 rows a thread: 34 us instead of 47
+// for 49,152 FP32 rows of 576 in order, to three buffers in turn (7 million runs).
+// Rows out of order have no lines in common: 37.2 instead of 36.2 for as many, 15.4
+// instead of 14.4 for 16,000 (2 million), 4.3 instead of 2.8 for 64.
 constexpr int64_t kW4ReadRuns = 1 << 22;
 
 // A product by wavefronts that share a block of columns and deal the depth
@@ -54,9 +55,10 @@ constexpr int64_t kW4MostGroups = 1 << 22;  // 2^31 threads of 512
 
 // Tiles of 32 from 17 rows on; as many columns a wavefront as leave a work-group
 // for every CU: with 512 instead of 256 of them 1,000 FP32 rows of 576 by 960 take
-// 12.9 us instead of 9.9, 64 BF16 rows of 4,096 by 12,288 20.7 instead of 19.1, 512
-// FP32 rows through a gated pair of 576 by 1,536 12.6 instead of 13.7; with 1,024
-// 16 rows of 576 by 49,152 12.7 instead of 10.3.
+// 13.1 us instead of 9.9, 64 BF16 rows of 4,096 by 12,288 20.9 instead of 19.0, 512
+// FP32 rows through a gated pair of 576 by 1,536 13.0 instead of 14.2; with 1,024
+// 16 rows of 576 by 49,152 12.8 instead of 10.3; with 128 one row of 4,096 by 4,096
+// 7.3 instead of 6.1.
 inline W4Plan w4_few_plan(int rows, int n, int depth, int parts, bool gated, bool eight) {
     W4Plan p{rows <= 16 ? 16 : 32, rows <= 16 ? 4 : 2, 8};
     // 8-bit results: a row's group of 32 lies in one block.
@@ -82,10 +84,12 @@ constexpr int64_t w4_tile_groups(int64_t rows, int64_t n, bool gated, bool large
                  : w4_ceil(rows, kSmallTileRows) * w4_ceil(n, gated ? kSmallTileColumns / 2 : kSmallTileColumns);
 }
 // Tiles where there is one for every CU, the largest that leave that. Small ones
-// from 128 work-groups on would take 256 BF16 rows of 4,096 by 4,096 from 18.6 us to
-// 36.1, from 512 on only 64 FP32 rows of 576 by 49,152 from 19.8 to 22.4; large ones
-// from 100 on 1,024 BF16 rows of 4,096 by 4,096 from 42.9 to 72.5 and 2,048 FP16 rows
-// of 1,024 by 2,048 from 23.5 to 39.5.
+// from 128 work-groups on would take 256 BF16 rows of 4,096 by 4,096 from 20.3 us to
+// 35.6, from 512 on only 64 FP32 rows of 576 by 49,152 from 20.0 to 22.6; large ones
+// from 100 on 1,024 BF16 rows of 4,096 by 4,096 from 43.9 to 71.4 and 2,048 FP16 rows
+// of 1,024 by 2,048 from 23.3 to 39.3, from 512 on only 2,048 8-bit rows of 4,096 by
+// 4,096 from 58.1 to 93.6. The rule does not look at columns that a tile has in vain:
+// for 32,768 BF16 rows of 576 by 64 small tiles would take 12.3 us instead of 18.6.
 constexpr W4Way w4_way(int rows, int n, bool gated) {
     return rows > 64 && w4_tile_groups(rows, n, gated, true) >= 256 ? kW4LargeTiles
            : rows > 32 && w4_tile_groups(rows, n, gated, false) >= 256 ? kW4SmallTiles

@@ -255,11 +255,12 @@ __device__ __forceinline__ void bring(const uint8_t* from, void* to) {
 // one behind it from memory to LDS, so that a wavefront only ever waits for what
 // was asked for a whole block's products before.
 //
-// 4,096 rows through a gated pair of 4,096 by 12,288 take 414 to 480 us, 1.7 to 2.0
+// 4,096 rows through a gated pair of 4,096 by 12,288 take 414 to 506 us, 1.6 to 2.0
 // PFLOP/s; the products alone, from registers, take 290 to 330 (the card lowers its
-// clock), so the matrix cores, at 0.48 of the cycles, are what is nearest. Rows
-// through registers and weights straight from memory by both their readers took
-// 506 to 574: of that 82 went with the rows' loads left out, 70 with the weights',
+// clock). The matrix cores are busy for 0.48 of the cycles: at the barrier of every 64
+// columns all loads are waited for, and half of the wavefronts' cycles go by waiting to
+// issue. Rows through registers and weights straight from memory by both their readers
+// took 506 to 574: of that 82 went with the rows' loads left out, 70 with the weights',
 // 213 with both, the L1's 64 bytes a cycle being shared by the two.
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 2) w4_planes_kernel(ProductArgs a, const uint8_t* laid_rows) {
